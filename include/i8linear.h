@@ -11,7 +11,8 @@
  *
  * "Reference" below is the jiaoch/Triton-INT8 project; file:line cites name the Python/Triton code a
  * function replaces.  Tensors are row-major and contiguous; a leading batch dimension is folded into
- * the rows.  All of rows/cols/M/N/K must be multiples of 128 (the reference has no masking either).
+ * the rows.  All of rows/cols/M/N/K must be multiples of 128 (the reference has no masking either), but for the expert
+ * layers and the product for serving at the end, which say what they take.
  */
 #ifndef I8LINEAR_H_
 #define I8LINEAR_H_
@@ -317,6 +318,61 @@ I8L_API int i8l_set_cta_limit(int max_ctas);
  * path end to end without a fault, a trap or an unbounded spin.  No counterpart in the reference.
  */
 I8L_API int i8l_test_set_wait_limit(uint32_t max_polls, int withhold_one_load);
+
+/* Element types of the expert layers. */
+#define I8L_DTYPE_BF16 0
+#define I8L_DTYPE_F16 1
+#define I8L_DTYPE_F32 2
+
+/*
+ * Tokens in the order of their experts.  x [tokens, cols] of `dtype`; ids [tokens, k], int32 or (ids64) int64: the experts of
+ * each token.  Choice i = t * k + j; an id outside [0, experts) is no expert's, the choice is dropped.  Expert e gets the rows
+ * from offsets[e] on, in the order of its choices, and offsets[e + 1] is the next multiple of `align` behind them.
+ *   out     [rows, cols]: out[pos[i]] = x[i / k]; all other rows are zeros
+ *   offsets int32 [experts + 1]
+ *   pos     int32 [tokens, k]: the row of a choice, -1 if dropped
+ *   src     int32 [rows]: the choice of a row, -1 if it has none
+ * rows >= tokens * k + min(experts, tokens * k) * (align - 1), rounded up to `align`.  The result depends on the inputs only (a
+ * stable counting sort, no atomics on places).  experts <= 1024, k <= 64, tokens * k <= 2^30, align <= 65536, any cols.
+ * Pointers are aligned to their elements; rows that are multiples of 16 bytes at 16-byte aligned pointers move 16 bytes at a
+ * time.  workspace: i8l_sort_workspace bytes, 4-byte aligned, may be NULL where that is 0.
+ * No counterpart in the reference, which has no expert layers.
+ */
+I8L_API int64_t i8l_sort_workspace(int64_t tokens, int k, int experts);
+I8L_API int i8l_sort_tokens(const void* x, const void* ids, int ids64, int64_t tokens, int64_t cols, int k, int experts,
+                   int64_t align, int dtype, int64_t rows, void* out, int32_t* offsets, int32_t* pos, int32_t* src,
+                   void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * The way back: y[t] = sum over j of weights[t, j] * rows[pos[t, j]], added in the order of j in fp32 and rounded once.  rows
+ * [n_rows, cols] and y [tokens, cols] of `dtype`, weights [tokens, k] of fp32 or `dtype` (wdtype), NULL for ones (the gradient of
+ * i8l_sort_tokens).  A choice whose pos is outside [0, n_rows) adds nothing, whatever its weight.
+ * i8l_combine_backward: drows[pos[t, j]] = weights[t, j] * dy[t], rows whose src is negative zero, and dweights[t, j] = the sum of
+ * dy[t] * rows[pos[t, j]] in fp32, zero for dropped choices; either may be NULL.  pos and src are inverse to one another, as
+ * i8l_sort_tokens makes them: a row is written by the choice that src names, and not at all if that choice names another row.
+ * No counterpart in the reference.
+ */
+I8L_API int i8l_combine(const void* rows, const void* weights, const int32_t* pos, int64_t n_rows, int64_t tokens, int64_t cols,
+                   int k, int dtype, int wdtype, void* y, void* stream);
+I8L_API int i8l_combine_backward(const void* rows, const void* weights, const int32_t* pos, const int32_t* src, const void* dy,
+                   int64_t n_rows, int64_t tokens, int64_t cols, int k, int dtype, int wdtype, void* drows, void* dweights,
+                   void* stream);
+
+/*
+ * A product whose weights stay int8, for any number of rows, by expert: rows [offsets[e], offsets[e + 1]) of x bf16 [rows, K]
+ * are quantized with one scale a row (I8L_QMODE_ROWRCP, I8L_HAD_NONE), multiplied exactly with w_q[e] (int8 [experts, N, K]) and
+ *   y = (float(acc) * x_scale[row]) * w_scale[e, n] + bias[e, n]
+ * is rounded once to bf16 (fp32 with I8L_GEMM_OUT_F32).  w_scale fp32 [experts, N]; bias bf16 [experts, N] or NULL.
+ *   offsets int32 [experts + 1] on the device, non-decreasing, or NULL: one matrix (experts = 1) for all rows.  Rows in front
+ *   of offsets[0] and from offsets[experts] on come out zero.
+ * N a multiple of 8, K of 16 and at most 131072 (the int32 sum cannot overflow), experts <= 1024, rows >= 0.  x, w_q, y, bias
+ * 16-byte aligned.  workspace: i8l_token_linear_workspace bytes, 256-byte aligned.
+ * The row and channel scales are those of the reference's double_channel variant (triton/double-channle_fwd32.py:295-311).
+ */
+I8L_API int64_t i8l_token_linear_workspace(int64_t rows, int64_t K);
+I8L_API int i8l_token_linear(const void* x, const int8_t* w_q, const float* w_scale, const int32_t* offsets, const void* bias,
+                   void* y, int64_t rows, int experts, int64_t N, int64_t K, int flags, void* workspace,
+                   int64_t workspace_bytes, int32_t* status, void* stream);
 
 /* Text of the calling thread's most recent error ("" if none). */
 I8L_API const char* i8l_last_error(void);

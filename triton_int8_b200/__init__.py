@@ -4,11 +4,11 @@ C ABI of libi8linear.so (see include/i8linear.h).  There is no CPU or eager fall
 from . import _lib
 from ._lib import I8LError
 
-__all__ = ["_lib", "I8LError", "block_channel", "double_channel", "fused", "kernels", "linear"]
+__all__ = ["_lib", "I8LError", "block_channel", "double_channel", "fused", "kernels", "linear", "moe"]
 
 
 def __getattr__(name):
-    if name in ("block_channel", "double_channel", "fused", "kernels", "linear", "tp"):
+    if name in ("block_channel", "double_channel", "fused", "kernels", "linear", "moe", "tp"):
         import importlib
         return importlib.import_module(f"{__name__}.{name}")
     raise AttributeError(name)

@@ -21,6 +21,7 @@ ASCALE_TILE, ASCALE_GROUP, ASCALE_TILE256 = 0, 1, 2
 BSCALE_CHANNEL, BSCALE_TILE, BSCALE_GROUP = 0, 1, 2
 GEMM_EXACT_ORDER, GEMM_DIVIDE, GEMM_OUT_F32, GEMM_PRODUCT_FIRST = 1, 2, 4, 8
 MAX_RANKS = 8
+DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2
 
 _P, _I64, _I, _F = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
 
@@ -48,6 +49,12 @@ SIGNATURES = {
     "i8l_set_cta_limit": [_I],
     "i8l_test_set_wait_limit": [ctypes.c_uint32, _I],
     "i8l_version": [],
+    "i8l_sort_workspace": [_I64, _I, _I],
+    "i8l_sort_tokens": [_P, _P, _I, _I64, _I64, _I, _I, _I64, _I, _I64, _P, _P, _P, _P, _P, _I64, _P],
+    "i8l_combine": [_P, _P, _P, _I64, _I64, _I64, _I, _I, _I, _P, _P],
+    "i8l_combine_backward": [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I, _I, _I, _P, _P, _P],
+    "i8l_token_linear_workspace": [_I64, _I64],
+    "i8l_token_linear": [_P, _P, _P, _P, _P, _P, _I64, _I, _I64, _I64, _I, _P, _I64, _P, _P],
 }
 
 
@@ -77,6 +84,7 @@ def load() -> ctypes.CDLL:
         lib.i8l_last_error.argtypes = []
         lib.i8l_last_error.restype = ctypes.c_char_p
         lib.i8l_status_open.restype = _P
+        lib.i8l_sort_workspace.restype = lib.i8l_token_linear_workspace.restype = _I64
         _lib = lib
         _fns.update((name, getattr(lib, name)) for name in SIGNATURES)
     return _lib

@@ -14,7 +14,7 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libi8linear.so")
 HOST_PATH = os.path.join(PKG_DIR, "_host.so")
-SOURCES = ["quant.cu", "gemm.cu", "fused.cu", "compose.cu"]
+SOURCES = ["quant.cu", "gemm.cu", "fused.cu", "compose.cu", "moe.cu", "tokens.cu"]
 HOST_SOURCE = os.path.join(CSRC, "host.cpp")
 ABI_HEADER = os.path.join(os.path.dirname(PKG_DIR), "include", "i8linear.h")
 HEADERS = [os.path.join(CSRC, "common.cuh"), os.path.join(CSRC, "ptx.cuh"), ABI_HEADER]

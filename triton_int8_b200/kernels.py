@@ -403,6 +403,140 @@ def sum_slots(slots: torch.Tensor, out: torch.Tensor | None = None) -> torch.Ten
     return out
 
 
+# ---------------------------------------------------------------------------------------- expert layers
+_DTYPES = {torch.bfloat16: L.DTYPE_BF16, torch.float16: L.DTYPE_F16, torch.float32: L.DTYPE_F32}
+
+
+def _check_rows(x: torch.Tensor, name: str) -> torch.Tensor:
+    if not x.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (no CPU path exists)")
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"{name} must be bfloat16, float16 or float32, got {x.dtype}")
+    if x.dim() != 2:
+        raise ValueError(f"{name} must have two dimensions, got {tuple(x.shape)}")
+    return x.contiguous()
+
+
+def _check_ints(t: torch.Tensor, name: str, shape: tuple) -> torch.Tensor:
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name} must be int32, got {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+    return t.contiguous()
+
+
+def sorted_rows(tokens: int, k: int, experts: int, align: int) -> int:
+    """Rows of sort_tokens' result: every choice, and the padding behind each expert that can have any."""
+    n = tokens * k
+    return -(-(n + min(experts, n) * (align - 1)) // align) * align
+
+
+def sort_tokens(x: torch.Tensor, ids: torch.Tensor, experts: int, align: int = 1):
+    """x [T, H], ids int32 or int64 [T, k] -> (rows [R, H], offsets int32 [experts + 1], pos int32 [T, k], src int32 [R]): see
+    i8l_sort_tokens."""
+    x = _check_rows(x, "x")
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"ids must be int32 or int64, got {ids.dtype}")
+    T, H = x.shape
+    if ids.dim() != 2 or ids.shape[0] != T:
+        raise ValueError(f"ids must be [{T}, k], got {tuple(ids.shape)}")
+    if experts < 1 or align < 1:
+        raise ValueError(f"experts and align must be positive, got {experts} and {align}")
+    ids = ids.contiguous()
+    k, dev = ids.shape[1], x.device
+    R = sorted_rows(T, k, experts, align)
+    rows = torch.empty((R, H), dtype=x.dtype, device=dev)
+    offsets = torch.empty((experts + 1,), dtype=torch.int32, device=dev)
+    pos = torch.empty((T, k), dtype=torch.int32, device=dev)
+    src = torch.empty((R,), dtype=torch.int32, device=dev)
+    size = L.load().i8l_sort_workspace(T, k, experts)
+    ws = torch.empty((size,), dtype=torch.int8, device=dev) if size else None
+    _call("i8l_sort_tokens", dev, x.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int64), T, H, k, experts, align, _DTYPES[x.dtype],
+          R, rows.data_ptr(), offsets.data_ptr(), pos.data_ptr(), src.data_ptr(), _ptr(ws), size, tensors=(ids,))
+    return rows, offsets, pos, src
+
+
+def _check_weights(weights, rows, shape):
+    if weights.dtype not in (torch.float32, rows.dtype):
+        raise TypeError(f"weights must be float32 or {rows.dtype}, got {weights.dtype}")
+    if tuple(weights.shape) != shape:
+        raise ValueError(f"weights have shape {tuple(weights.shape)}, expected {shape}")
+    return weights.contiguous()
+
+
+def combine(rows: torch.Tensor, weights, pos: torch.Tensor) -> torch.Tensor:
+    """rows [R, H], weights [T, k] or None (ones), pos int32 [T, k] -> y [T, H]: see i8l_combine."""
+    rows = _check_rows(rows, "rows")
+    if pos.dim() != 2:
+        raise ValueError(f"pos must be [tokens, k], got {tuple(pos.shape)}")
+    T, k = pos.shape
+    pos = _check_ints(pos, "pos", (T, k))
+    wdtype = L.DTYPE_F32
+    if weights is not None:
+        weights = _check_weights(weights, rows, (T, k))
+        wdtype = _DTYPES[weights.dtype]
+    R, H = rows.shape
+    y = torch.empty((T, H), dtype=rows.dtype, device=rows.device)
+    _call("i8l_combine", rows.device, rows.data_ptr(), _ptr(weights), pos.data_ptr(), R, T, H, k, _DTYPES[rows.dtype], wdtype, y.data_ptr(),
+          tensors=(weights, pos))
+    return y
+
+
+def combine_backward(rows, weights, pos, src, dy, need_rows=True, need_weights=True):
+    """(drows [R, H] or None, dweights [T, k] or None) of y = combine(rows, weights, pos): see i8l_combine_backward."""
+    rows, dy = _check_rows(rows, "rows"), _check_rows(dy, "dy")
+    (R, H), (T, k) = rows.shape, pos.shape
+    if dy.dtype != rows.dtype or tuple(dy.shape) != (T, H):
+        raise ValueError(f"dy is {dy.dtype} {tuple(dy.shape)}, expected {rows.dtype} {(T, H)}")
+    weights, pos, src = _check_weights(weights, rows, (T, k)), _check_ints(pos, "pos", (T, k)), _check_ints(src, "src", (R,))
+    drows = torch.empty_like(rows) if need_rows else None
+    dweights = torch.empty_like(weights) if need_weights else None
+    _call("i8l_combine_backward", rows.device, rows.data_ptr(), weights.data_ptr(), pos.data_ptr(), src.data_ptr(), dy.data_ptr(), R, T, H, k,
+          _DTYPES[rows.dtype], _DTYPES[weights.dtype], _ptr(drows), _ptr(dweights), tensors=(weights, pos, src, dy))
+    return drows, dweights
+
+
+def token_linear(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, offsets=None, bias=None, out_dtype=torch.bfloat16, status=None):
+    """x bf16 [R, K], wq int8 [E, N, K], ws fp32 [E, N], offsets int32 [E + 1] or None (E = 1), bias bf16 [E, N] -> [R, N]: see
+    i8l_token_linear."""
+    x = _check_bf16(x, "x")
+    if wq.dtype != torch.int8 or ws.dtype != torch.float32:
+        raise TypeError(f"weights must be int8 with float32 scales, got {wq.dtype} and {ws.dtype}")
+    if wq.dim() != 3 or x.dim() != 2 or wq.shape[2] != x.shape[1]:
+        raise ValueError(f"operand shapes do not match: {tuple(x.shape)} x {tuple(wq.shape)}")
+    (R, Kd), (E, N, _), dev = x.shape, wq.shape, x.device
+    if tuple(ws.shape) != (E, N):
+        raise ValueError(f"weight scales have shape {tuple(ws.shape)}, expected {(E, N)}")
+    if offsets is not None:
+        offsets = _check_ints(offsets, "offsets", (E + 1,))
+    if bias is not None:
+        if bias.dtype != torch.bfloat16 or tuple(bias.shape) != (E, N):
+            raise ValueError(f"bias is {bias.dtype} {tuple(bias.shape)}, expected bfloat16 {(E, N)}")
+        bias = _aligned(bias)
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"out_dtype must be bfloat16 or float32, got {out_dtype}")
+    x, wq, ws = _aligned(x), _aligned(wq), ws.contiguous()
+    y = torch.empty((R, N), dtype=out_dtype, device=dev)
+    size = L.load().i8l_token_linear_workspace(R, Kd)
+    work = torch.empty((size,), dtype=torch.int8, device=dev)
+    status = device_status(dev) if status is None else status
+    _call("i8l_token_linear", dev, x.data_ptr(), wq.data_ptr(), ws.data_ptr(), _ptr(offsets), _ptr(bias), y.data_ptr(), R, E, N, Kd,
+          L.GEMM_OUT_F32 if out_dtype == torch.float32 else 0, work.data_ptr(), size, status.data_ptr(),
+          tensors=(wq, ws, offsets, bias, status))
+    return y
+
+
+def refuse_gradient(name: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} has no gradient (its weights are int8): call it under torch.no_grad(), train with Int8Linear")
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous and at a 16-byte boundary, where the kernels' loads start."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 class cta_limit:
     """Context manager: GEMMs launched inside use at most `n` CTAs, leaving the other SMs to a kernel
     running beside them (a collective on another stream).  n <= 0 means no limit."""

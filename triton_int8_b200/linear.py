@@ -157,6 +157,18 @@ def linear_backward(dy2: torch.Tensor, weight: torch.Tensor, saved_xt, cfg: Int8
     return dx, dw
 
 
+def linear_w8a8(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, bias=None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The product for serving, with weights that were quantized once: x bf16 [..., K], wq int8 [N, K], ws fp32 [N], bias bf16 [N]
+    -> [..., N], bf16 or fp32.  One scale a row of x and one an output channel, as double_channel has them
+    (triton/double-channle_fwd32.py:295-311 without the rotation), any number of rows, N a multiple of 8, K of 16.  There is no
+    gradient: inputs that want one are refused."""
+    K.refuse_gradient("linear_w8a8", x, ws, bias)
+    if wq.dim() != 2 or ws.dim() != 1 or (bias is not None and bias.dim() != 1):
+        raise ValueError("linear_w8a8: wq [N, K], ws [N], bias [N]")
+    y = K.token_linear(x.reshape(-1, x.shape[-1]), wq[None], ws[None], None, None if bias is None else bias[None], out_dtype)
+    return y.view(*x.shape[:-1], wq.shape[0])
+
+
 class Int8LinearFn(torch.autograd.Function):
     """y = x @ weight^T + bias with all three GEMMs in INT8."""
 

@@ -1,0 +1,88 @@
+"""Expert layers: tokens to their experts and back.
+
+    rows, offsets, pos, src = sort_tokens(x, ids, experts)     # the rows of expert e are rows[offsets[e]:offsets[e + 1]]
+    ...                                                        # any computation that keeps the rows in their places
+    y = combine(rows, weights, pos, src)                       # y[t] = sum over j of weights[t, j] * rows[pos[t, j]]
+
+Both are differentiable and neither waits for the device: shapes depend on the sizes, not on the choices.  The reference has no
+expert layers.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib as L
+from . import kernels as K
+
+
+class _SortFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, ids, experts, align):
+        rows, offsets, pos, src = K.sort_tokens(x, ids, experts, align)
+        ctx.mark_non_differentiable(offsets, pos, src)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(pos)
+        return rows, offsets, pos, src
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, drows, *_):
+        if drows is None:
+            return None, None, None, None
+        return K.combine(drows, None, ctx.saved_tensors[0]), None, None, None   # a token's gradient is the sum of its rows'
+
+
+class _CombineFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, weights, pos, src):
+        src = K._check_ints(src, "src", (rows.shape[0],))
+        ctx.save_for_backward(rows, weights, pos, src)
+        return K.combine(rows, weights, pos)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        drows, dweights = K.combine_backward(*ctx.saved_tensors, dy, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        return drows, dweights, None, None
+
+
+def sort_tokens(x: torch.Tensor, ids: torch.Tensor, experts: int, align: int = 1):
+    """x [T, H] (bf16, fp16, fp32), ids int32 or int64 [T, k], the experts of each token -> (rows, offsets, pos, src):
+
+    rows [R, H]: a copy of x[t] for each choice ids[t, j], those of expert e from offsets[e] on in the order of (t, j).  offsets[e + 1]
+    is the next multiple of `align` behind them (128: every segment is a whole number of blocks for Int8Linear).  Rows of no
+    choice are zeros, also the ones from offsets[experts] on: R = sorted_rows(T, k, experts, align) covers any choices.
+    pos int32 [T, k]: the row of a choice, or -1 where the id is outside [0, experts): such a choice is dropped (another rank's
+    expert, or one above its capacity).  src int32 [R]: the inverse, t * k + j or -1.
+    At most 1024 experts and 64 choices a token.  Gradient: that of x, summed in 32 bits."""
+    if torch.is_grad_enabled() and x.requires_grad:
+        return _SortFn.apply(x, ids, experts, align)
+    return K.sort_tokens(x, ids, experts, align)
+
+
+def combine(rows: torch.Tensor, weights: torch.Tensor, pos: torch.Tensor, src: torch.Tensor) -> torch.Tensor:
+    """rows [R, H], weights [T, k] (fp32 or the rows' type), pos and src of sort_tokens -> y [T, H] of the rows' type,
+    y[t] = sum over j of weights[t, j] * rows[pos[t, j]], added in 32 bits and rounded once.  Dropped choices add nothing.
+    Gradients: those of rows (zero for rows of no choice) and of weights (zero for dropped choices)."""
+    if torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
+        return _CombineFn.apply(rows, weights, pos, src)
+    return K.combine(rows, weights, pos)
+
+
+def quantize_experts(weight: torch.Tensor):
+    """weight bf16 [E, N, K] (or [N, K]), K a multiple of 128 -> (int8 of its shape, fp32 scales [E, N]): one scale an output channel,
+    as double_channel quantizes it (triton/double-channle_fwd32.py:140-175)."""
+    return K.quant_row(weight, L.QMODE_ROWRCP)
+
+
+def expert_linear(rows: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, offsets: torch.Tensor, bias=None,
+                  out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The experts' products for serving: rows bf16 [R, K] in the order of their experts, wq int8 [E, N, K] and ws fp32 [E, N]
+    (quantize_experts), offsets int32 [E + 1] (sort_tokens), bias bf16 [E, N] -> [R, N], bf16 or fp32.  A row is quantized with
+    one scale, the sum over K is exact, y = (sum * row scale) * channel scale + bias is rounded once.  Rows from offsets[E] on
+    come out zero.  N a multiple of 8, K of 16; any number of rows, one included.
+    The weights are integers, there is no gradient: inputs that want one are refused.  Int8Linear trains, on segments of
+    sort_tokens(align=128)."""
+    K.refuse_gradient("expert_linear", rows, ws, bias)
+    return K.token_linear(rows, wq, ws, offsets, bias, out_dtype)
