@@ -206,3 +206,26 @@ def test_elements_beyond_32_bits():
     y = linear.linear_w8a8(x, wq, ws)
     pick = torch.tensor([0, 1, 65535, 131071, 131072, 139998, 139999], device=DEV)
     assert y.numel() > 2 ** 31 and torch.equal(y[pick].cpu(), _plain(x[pick], wq, ws, None).to(BF16))
+
+
+@pytest.mark.parametrize("R,E,N,Kd", [(200, 1, 2048, 512), (3000, 4, 1000, 272), (3000, 4, 20000, 272)])
+def test_wait_that_runs_out_and_the_next_call(R, E, N, Kd):
+    """A withheld load: the kernel returns, the status word says so, the next call is right (see test_timeout_gpu.py)."""
+    from triton_int8_b200 import _lib as L
+    lib = L.load()
+    g = torch.Generator().manual_seed(11)
+    x, (wq, ws) = _rows(g, R, Kd), _weights(g, E, N, Kd)
+    offsets = torch.tensor([R * e // E for e in range(E + 1)], dtype=torch.int32, device=DEV)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    assert lib.i8l_test_set_wait_limit(256, 1) == 0
+    try:
+        K.token_linear(x, wq, ws, offsets, status=status)
+        torch.cuda.synchronize()
+    finally:
+        assert lib.i8l_test_set_wait_limit(0, 0) == 0
+    assert status.item() == L.TIMEOUT
+    status.zero_()
+    y = K.token_linear(x, wq, ws, offsets, out_dtype=F32, status=status)
+    assert status.item() == 0
+    ref = torch.cat([_plain(x[a:b], wq[e], ws[e], None) for e, (a, b) in enumerate(zip(offsets.tolist(), offsets.tolist()[1:]))])
+    assert torch.equal(y.cpu(), ref)

@@ -19,6 +19,7 @@ int check_arch();
 // launched by this host thread may use (i8l_set_cta_limit, else the SM count).
 uint32_t gemm_wait_limit();
 int gemm_cta_budget();
+int gemm_withhold();   // test hook: whether a producer leaves out the last load of its first tile
 int sm_count();  // of the current device
 int32_t* mirror_of(const int32_t* status_word);   // see i8l_status_mirror; null without one
 
@@ -26,6 +27,8 @@ int32_t* mirror_of(const int32_t* status_word);   // see i8l_status_mirror; null
 int quant_pair(const void* a, int64_t a_batch, int64_t a_rows, int a_gran, int8_t* aq, float* as, int8_t* aqt, float* ast, const void* b,
                int64_t b_batch, int64_t b_rows, int b_gran, int8_t* bq, float* bs, int64_t cols, int qmode, int hadamard,
                cudaStream_t st);
+// x bf16 [rows, cols], cols a multiple of 8 and at most 2^20: int8 rows with one scale each, I8L_QMODE_ROWRCP without rotation.
+int quant_token_rows(const void* x, int64_t rows, int64_t cols, int8_t* q, float* scale, cudaStream_t st);
 // i8l_col_sum; in a chain it runs beside its neighbours.
 int col_sum(const void* x, int64_t rows, int64_t cols, void* out, cudaStream_t st);
 // Clears n floats; in a chain the next kernel waits for it before anything else.

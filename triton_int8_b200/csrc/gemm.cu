@@ -1107,6 +1107,19 @@ int make_tile_map_bf16(CUtensorMap* map, const void* ptr, int64_t rows, int64_t 
   return I8L_OK;
 }
 
+int make_tile_map_i8(CUtensorMap* map, const void* ptr, int64_t rows, int64_t K, int box_rows) {
+  EncodeTiledFn enc = get_encode();
+  if (!enc) return fail(I8L_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t gdim[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  cuuint64_t gstr[1] = {(cuuint64_t)K};
+  cuuint32_t box[2] = {(cuuint32_t)BK, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), gdim, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(I8L_ERR_CUDA, "cuTensorMapEncodeTiled (int8) failed with CUresult %d", (int)r);
+  return I8L_OK;
+}
+
 constexpr int MAX_DEVICES = 64;
 static int current_device() {
   int dev = 0;
@@ -1136,6 +1149,7 @@ uint32_t gemm_wait_limit() {
   const uint32_t lim = g_test_max_polls.load(std::memory_order_relaxed);
   return lim ? lim : WAIT_MAX_POLLS;
 }
+int gemm_withhold() { return g_test_withhold.load(std::memory_order_relaxed); }
 int gemm_cta_budget() {
   const int sms = sm_count();
   return (g_cta_limit > 0 && g_cta_limit < sms) ? g_cta_limit : sms;

@@ -1262,6 +1262,23 @@ extern "C" int i8l_quant_tile(const void* x, int64_t batch, int64_t rows, int64_
   return fail(I8L_ERR_ARG, "i8l_quant_tile: unsupported gran=%d qmode=%d", gran, qmode);
 }
 
+namespace i8l {
+// The rows of a product for serving: the kernels below take any multiple of 8 columns where nothing is rotated.
+int quant_token_rows(const void* x, int64_t rows, int64_t cols, int8_t* q, float* scale, cudaStream_t st) {
+  const __nv_bfloat16* xp = static_cast<const __nv_bfloat16*>(x);
+  constexpr int MODE = I8L_QMODE_ROWRCP;
+  auto cached = [&](auto kernel, int per_block) {
+    return launch(kernel, dim3((unsigned)((rows + per_block - 1) / per_block)), 256, 0, st, xp, rows, cols, q, scale, chain_first());
+  };
+  I8L_CUDA_OK(cols <= 2048    ? cached(quant_row_cached_kernel<MODE, 32>, 8)
+              : cols <= 4096  ? cached(quant_row_cached_kernel<MODE, 64>, 4)
+              : cols <= 8192  ? cached(quant_row_cached_kernel<MODE, 128>, 2)
+              : cols <= 16384 ? cached(quant_row_cached_kernel<MODE, 256>, 1)
+                              : launch(quant_row_kernel<MODE, false>, dim3((unsigned)rows), 256, 0, st, xp, cols, q, scale, chain_first()));
+  return I8L_OK;
+}
+}  // namespace i8l
+
 extern "C" int i8l_quant_row(const void* x, int64_t rows, int64_t cols, int qmode, int hadamard, int8_t* q,
                              float* scale, void* stream) {
   if (rows <= 0 || cols <= 0 || cols % 128 || rows > 0x7fffffffll || cols > (1 << 20))

@@ -1,6 +1,8 @@
 // The INT8 product for serving: bf16 rows x int8 weights that were quantized once, for any number of rows, one weight matrix an
 // expert (i8l_token_linear).  Row scales and channel scales are those of the double_channel variant, so that the sum over K is
 // exact in int32 and an output needs one product by each scale.
+#include <atomic>
+
 #include "common.cuh"
 #include "ptx.cuh"
 
@@ -162,13 +164,320 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const TokenArgs a
   }
 }
 
-constexpr int FEW_SMEM = 160 * 1024;
+// ------------------------------------------------------------------------------------------ many rows
+// The tensor cores with the operands exchanged: 128 output channels are the rows of an MMA and up to TOK tokens its columns, whose
+// number is the instruction's N and may be any multiple of 16.  A segment of 17 rows costs 32 columns that way, where tokens as
+// MMA rows would cost 128, and the weights, which bound the product until a segment has some hundred rows, are read once.
+//
+// Persistent, a CTA per SM, 384 threads: warp 0 brings K blocks of 128 bytes by TMA (128 weight rows and the tokens of the tile) into a
+// ring, warp 1 issues tcgen05.mma kind::i8 into one of several accumulators in tensor memory, warps 4 to 11 take a finished one
+// out: a lane is a channel there, a register a token, so a bf16 tile is turned in shared memory and leaves 16 bytes a lane.
+// Warps 2 and 3 clear the rows of no expert.  Tiles come from the offsets in device memory: nothing waits for the host.
+// All waits are bounded, as in gemm.cu: on expiry every role leaves, the status word says so.
+constexpr int GRP_THREADS = 384, GRP_EPI_WARPS = 8, CHANNELS = 128, KBYTES = 128;
+constexpr int A_BYTES = CHANNELS * KBYTES;
+constexpr int BIG_BOX = 64, SMALL_BOX = 16;   // tokens of a TMA box
+constexpr int EPI_BYTES = 32 * 32 * 2;        // 32 tokens x 32 channels in bf16
+constexpr int RASTER = 16;                    // token tiles whose rows should stay in L2 while the channels are gone through
+
+template <int TOK> struct Grp {
+  static constexpr int STAGES = TOK == 256 ? 4 : 8, BUFS = 512 / TOK < 4 ? 512 / TOK : 4, COLUMNS = BUFS * TOK;
+  static constexpr int B_BYTES = TOK * KBYTES;
+  static constexpr int RING = STAGES * (A_BYTES + B_BYTES);
+  static constexpr int TABLE = RING + GRP_EPI_WARPS * EPI_BYTES;   // then experts x (first row, rows), experts + 1 tile counts
+  static int smem(int experts) { return TABLE + experts * 12 + 4 + 1024; }
+};
+
+struct GroupArgs {
+  TokenArgs t;
+  const float* xs;
+  int32_t *status, *mirror;
+  uint32_t max_polls;
+  int n_tiles, withhold;
+};
+struct __align__(16) GroupCtl {
+  uint64_t full[8], empty[8], tfull[4], tempty[4], done;
+  int abort_flag;
+  uint32_t tmem_base;
+};
+struct Tile {
+  int expert, channel;
+  int64_t row;
+  int rows, columns;   // tokens, and those rounded up to the MMA's N
+};
+
+// Instruction descriptor of kind::i8: D s32, A and B s8, K-major, M = 128.
+__device__ __forceinline__ uint32_t mma_desc(int n) { return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(CHANNELS >> 4) << 24); }
+
+template <int TOK>
+__device__ __forceinline__ Tile tile_of(int t, int experts, int n_tiles, const int2* seg, const int* first) {
+  int lo = 0, hi = experts;   // first[lo] <= t < first[hi]; experts without rows have no tiles and are stepped over
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (first[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  const int rows = seg[lo].y, tiles = (rows + TOK - 1) / TOK;
+  const int share = ((rows + tiles - 1) / tiles + 15) & ~15;   // tokens of a tile: equal ones rather than full ones and a rest
+  const int local = t - first[lo], group = local / (RASTER * n_tiles), g0 = group * RASTER;
+  const int width = tiles - g0 < RASTER ? tiles - g0 : RASTER, at = local - group * RASTER * n_tiles;
+  const int n = at / width, m = g0 + at - n * width;
+  Tile r;
+  r.expert = lo;
+  r.channel = n * CHANNELS;
+  r.row = seg[lo].x + (int64_t)m * share;
+  r.rows = rows - m * share < share ? rows - m * share : share;
+  r.columns = (r.rows + 15) & ~15;
+  return r;
+}
+
+template <int TOK>
+__global__ void __launch_bounds__(GRP_THREADS, 1)
+group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_big, const __grid_constant__ CUtensorMap map_small,
+             const GroupArgs p) {
+  using G = Grp<TOK>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ GroupCtl ctl;
+  uint8_t* const smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  const uint32_t smem_a = smem_u32(smem), smem_b = smem_a + G::STAGES * A_BYTES;
+  int2* const seg = reinterpret_cast<int2*>(smem + G::TABLE);
+  int* const first = reinterpret_cast<int*>(seg + p.t.experts);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort_flag = &ctl.abort_flag;
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&map_w);
+    prefetch_tensormap(&map_big);
+    prefetch_tensormap(&map_small);
+    for (int s = 0; s < G::STAGES; ++s) {
+      mbar_init(smem_u32(&ctl.full[s]), 1);
+      mbar_init(smem_u32(&ctl.empty[s]), 1);
+    }
+    for (int b = 0; b < G::BUFS; ++b) {
+      mbar_init(smem_u32(&ctl.tfull[b]), 1);
+      mbar_init(smem_u32(&ctl.tempty[b]), GRP_EPI_WARPS);
+    }
+    mbar_init(smem_u32(&ctl.done), 1);
+    ctl.abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem_base)), "r"(G::COLUMNS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  chain_wait();   // offsets, the quantized rows and whatever still uses the output's memory
+  for (int e = threadIdx.x; e < p.t.experts; e += GRP_THREADS) {
+    int64_t b, n;
+    segment(p.t, e, b, n);
+    seg[e] = make_int2((int)b, (int)(n - b));
+    first[e + 1] = (int)(n - b + TOK - 1) / TOK * p.n_tiles;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) {   // running sum of the tiles
+    int carry = 0;
+    if (lane == 0) first[0] = 0;
+    for (int e0 = 0; e0 < p.t.experts; e0 += 32) {
+      int up = e0 + lane < p.t.experts ? first[e0 + lane + 1] : 0;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, up, d);
+        if (lane >= d) up += v;
+      }
+      if (e0 + lane < p.t.experts) first[e0 + lane + 1] = carry + up;
+      carry += __shfl_sync(0xffffffffu, up, 31);
+    }
+  }
+  __syncthreads();
+  const uint32_t tmem_base = ctl.tmem_base;
+  const int total = first[p.t.experts], KB = (int)((p.t.K + KBYTES - 1) / KBYTES);
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    int s = 0;
+    uint32_t ph = 0, issued = 0, issued_ph = 0;   // bit s: a load into stage s is (or was) in flight, with parity
+    bool ok = true;
+    for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+      const Tile tile = tile_of<TOK>(t, p.t.experts, p.n_tiles, seg, first);
+      const int w_row = (int)((int64_t)tile.expert * p.t.N) + tile.channel;
+      for (int kb = 0; kb < KB; ++kb) {
+        if (!(ok = mbar_wait(smem_u32(&ctl.empty[s]), ph ^ 1u, abort_flag, p.max_polls))) break;
+        if (p.withhold && t == (int)blockIdx.x && kb == KB - 1) {   // test hook: the waits that depend on this stage run out
+          if (++s == G::STAGES) { s = 0; ph ^= 1u; }
+          continue;
+        }
+        if (lane == 0) {
+          const uint32_t bar = smem_u32(&ctl.full[s]);
+          mbar_expect_tx(bar, A_BYTES + tile.columns * KBYTES);
+          tma_load_2d(smem_a + s * A_BYTES, &map_w, bar, kb * KBYTES, w_row);
+          int c = 0;
+          for (; tile.columns - c >= BIG_BOX; c += BIG_BOX) tma_load_2d(smem_b + s * G::B_BYTES + c * KBYTES, &map_big, bar, kb * KBYTES, (int)tile.row + c);
+          for (; c < tile.columns; c += SMALL_BOX) tma_load_2d(smem_b + s * G::B_BYTES + c * KBYTES, &map_small, bar, kb * KBYTES, (int)tile.row + c);
+        }
+        issued |= 1u << s;
+        issued_ph = (issued_ph & ~(1u << s)) | (ph << s);
+        if (++s == G::STAGES) { s = 0; ph ^= 1u; }
+      }
+    }
+    if (!ok) {   // copies in flight land before the CTA's shared memory is released
+      for (int k = 0; k < G::STAGES; ++k)
+        if (issued & (1u << k)) {
+          int dummy = 0;
+          mbar_wait(smem_u32(&ctl.full[k]), (issued_ph >> k) & 1u, &dummy, 1u << 15);
+        }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    const bool elected = elect_one();
+    int s = 0, ab = 0;
+    uint32_t ph = 0, aph = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+      const uint32_t idesc = mma_desc(tile_of<TOK>(t, p.t.experts, p.n_tiles, seg, first).columns), d = tmem_base + ab * TOK;
+      if (!(ok = mbar_wait(smem_u32(&ctl.tempty[ab]), aph ^ 1u, abort_flag, p.max_polls))) break;
+      for (int kb = 0; kb < KB; ++kb) {
+        if (!(ok = mbar_wait(smem_u32(&ctl.full[s]), ph, abort_flag, p.max_polls))) break;
+        tc_fence_after();
+        if (elected) {
+          const uint64_t da = smem_desc(smem_a + s * A_BYTES), db = smem_desc(smem_b + s * G::B_BYTES);
+#pragma unroll
+          for (int k4 = 0; k4 < KBYTES / 32; ++k4) tc_mma_i8(d, da + 2 * k4, db + 2 * k4, idesc, (k4 > 0 || kb > 0) ? 1u : 0u);
+          tc_commit(smem_u32(&ctl.empty[s]));
+          if (kb == KB - 1) tc_commit(smem_u32(&ctl.tfull[ab]));
+        }
+        __syncwarp();
+        if (++s == G::STAGES) { s = 0; ph ^= 1u; }
+      }
+      if (++ab == G::BUFS) { ab = 0; aph ^= 1u; }
+    }
+    if (elected) tc_commit(smem_u32(&ctl.done));   // all MMAs have retired before tensor memory is freed
+    __syncwarp();
+    int dummy = 0;
+    mbar_wait(smem_u32(&ctl.done), 0, &dummy);
+  } else if (warp < 4) {
+    // ------------------------------------------------------------------ rows of no expert
+    const int64_t before = seg[0].x, behind = (int64_t)seg[p.t.experts - 1].x + seg[p.t.experts - 1].y, dead = before + p.t.rows - behind;
+    const int64_t pieces = p.t.N * (p.t.out_f32 ? 4 : 2) / 16;
+    for (int64_t i = (int64_t)blockIdx.x * 64 + threadIdx.x - 64; i < dead * pieces; i += (int64_t)gridDim.x * 64) {
+      const int64_t r = i / pieces;
+      static_cast<uint4*>(p.t.y)[(r < before ? r : behind + r - before) * pieces + i - r * pieces] = make_uint4(0, 0, 0, 0);
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue
+    const int q = warp & 3, half = (warp - 4) >> 2;   // a quarter of the channels, every other 32 tokens
+    uint8_t* const turn = smem + G::RING + (warp - 4) * EPI_BYTES;
+    int ab = 0;
+    uint32_t aph = 0;
+    for (int t = blockIdx.x; t < total; t += gridDim.x) {
+      const Tile tile = tile_of<TOK>(t, p.t.experts, p.n_tiles, seg, first);
+      const int n = tile.channel + q * 32 + lane;
+      const bool live = n < p.t.N;
+      const int64_t c = (int64_t)tile.expert * p.t.N + n;
+      const float sw = live ? p.t.ws[c] : 0.f, bias = live && p.t.bias ? __bfloat162float(p.t.bias[c]) : 0.f;
+      if (!mbar_wait(smem_u32(&ctl.tfull[ab]), aph, abort_flag, p.max_polls)) break;
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + ab * TOK;
+      for (int j0 = half * 32; j0 < tile.rows; j0 += 64) {
+        const int left = tile.rows - j0;
+        const float mine = lane < left ? p.xs[tile.row + j0 + lane] : 0.f;
+        uint32_t r[32];
+        tc_ld16(taddr + j0, r);
+        tc_ld16(taddr + j0 + 16, r + 16);
+        tc_ld_wait();
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          v[j] = __fmul_rn(__fmul_rn(__int2float_rn((int)r[j]), __shfl_sync(0xffffffffu, mine, j)), sw);
+          if (p.t.bias) v[j] = __fadd_rn(v[j], bias);
+        }
+        const int64_t row = tile.row + j0;
+        if (p.t.out_f32) {
+          float* y = static_cast<float*>(p.t.y) + row * p.t.N + n;
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (live && j < left) y[j * p.t.N] = v[j];
+        } else {
+          __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(turn) + lane;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) to[j * 32] = __float2bfloat16_rn(v[j]);
+          __syncwarp();
+          const int piece = lane & 3, n8 = tile.channel + q * 32 + piece * 8;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int j = i * 8 + (lane >> 2);
+            if (j < left && n8 < p.t.N)
+              *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.t.y) + (row + j) * p.t.N + n8) = *reinterpret_cast<const uint4*>(turn + j * 64 + piece * 16);
+          }
+          __syncwarp();
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&ctl.tempty[ab]));
+      if (++ab == G::BUFS) { ab = 0; aph ^= 1u; }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && ctl.abort_flag && p.status) {
+    atomicExch(p.status, I8L_ERR_TIMEOUT);
+    if (p.mirror) {
+      __threadfence_system();   // who sees the mirror finds the word set
+      *static_cast<volatile int32_t*>(p.mirror) = I8L_ERR_TIMEOUT;
+    }
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(G::COLUMNS) : "memory");
+  }
+}
+
+// ------------------------------------------------------------------------------------------ host
+// Once a device: the shared memory that a kernel may be launched with.
+template <typename Kernel>
+cudaError_t allow_smem(Kernel kernel, std::atomic<int>* allowed, int bytes) {
+  constexpr int DEVICES = 64;
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return e;
+  const bool known = dev >= 0 && dev < DEVICES;
+  if (known && allowed[dev].load(std::memory_order_acquire) >= bytes) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && known) allowed[dev].store(bytes, std::memory_order_release);
+  return e;
+}
+
+constexpr int FEW_SMEM = 64 * 1024;
 template <int MT> int launch_few(const TokenArgs& a, cudaStream_t st) {
-  const size_t smem = (size_t)(MT * a.K);
-  if (smem > 48 * 1024) I8L_CUDA_OK(cudaFuncSetAttribute(few_rows_kernel<MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  static std::atomic<int> allowed[64];
+  I8L_CUDA_OK(allow_smem(few_rows_kernel<MT>, allowed, FEW_SMEM));
   const int64_t segments = a.offsets ? (a.experts < a.rows ? a.experts : a.rows) : 1;
-  few_rows_kernel<MT><<<dim3((unsigned)((a.N + FEW_COLS - 1) / FEW_COLS), (unsigned)segments), FEW_THREADS, smem, st>>>(a);
+  few_rows_kernel<MT><<<dim3((unsigned)((a.N + FEW_COLS - 1) / FEW_COLS), (unsigned)segments), FEW_THREADS, MT * a.K, st>>>(a);
   I8L_CUDA_OK(cudaGetLastError());
+  return I8L_OK;
+}
+
+template <int TOK> int launch_group(const int8_t* xq, GroupArgs& p, cudaStream_t st) {
+  using G = Grp<TOK>;
+  static std::atomic<int> allowed[64];
+  const TokenArgs& a = p.t;
+  I8L_CUDA_OK(allow_smem(group_kernel<TOK>, allowed, G::smem(MAX_EXPERTS)));
+  p.n_tiles = (int)((a.N + CHANNELS - 1) / CHANNELS);
+  const int64_t most = (a.rows / TOK + (a.experts < a.rows ? a.experts : a.rows)) * p.n_tiles;   // tiles, whatever the offsets
+  if (most >= (1ll << 31)) return fail(I8L_ERR_SHAPE, "i8l_token_linear: too large for 32-bit tile numbers");
+  CUtensorMap mw, mb, ms;
+  if (int e = make_tile_map_i8(&mw, a.wq, a.experts * a.N, a.K, CHANNELS)) return e;
+  if (int e = make_tile_map_i8(&mb, xq, a.rows, a.K, BIG_BOX)) return e;
+  if (int e = make_tile_map_i8(&ms, xq, a.rows, a.K, SMALL_BOX)) return e;
+  const int budget = gemm_cta_budget();
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attrs[1];
+  cfg.gridDim = dim3((unsigned)(most < budget ? most : budget), 1, 1);
+  cfg.blockDim = dim3(GRP_THREADS, 1, 1);
+  cfg.dynamicSmemBytes = G::smem(a.experts);
+  cfg.stream = st;
+  chain_attribute(cfg, attrs);
+  I8L_CUDA_OK(cudaLaunchKernelEx(&cfg, group_kernel<TOK>, mw, mb, ms, p));
   return I8L_OK;
 }
 
@@ -203,9 +512,22 @@ extern "C" int i8l_token_linear(const void* x, const int8_t* w_q, const float* w
   a.bias = static_cast<const __nv_bfloat16*>(bias); a.y = y;
   a.rows = rows; a.N = N; a.K = K; a.experts = experts; a.out_f32 = (flags & I8L_GEMM_OUT_F32) ? 1 : 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  (void)status;
-  if (rows == 1 || K > FEW_SMEM / 2) return launch_few<1>(a, st);
-  if (rows == 2 || K > FEW_SMEM / 4) return launch_few<2>(a, st);
-  if (rows <= 4 || K > FEW_SMEM / 8) return launch_few<4>(a, st);
-  return launch_few<8>(a, st);
+  if (rows == 1 && K <= FEW_SMEM) return launch_few<1>(a, st);
+  if (rows == 2 && K <= FEW_SMEM / 2) return launch_few<2>(a, st);
+  if (rows <= 4 && K <= FEW_SMEM / 4) return launch_few<4>(a, st);
+  if (rows <= 8 && K <= FEW_SMEM / 8) return launch_few<8>(a, st);
+  GroupArgs p{};
+  p.t = a;
+  int8_t* xq = static_cast<int8_t*>(workspace);
+  float* xs = reinterpret_cast<float*>(xq + (rows * K + 255) / 256 * 256);
+  p.xs = xs;
+  p.status = status;
+  p.mirror = status ? mirror_of(status) : nullptr;
+  p.max_polls = gemm_wait_limit();
+  p.withhold = gemm_withhold();
+  const LaunchChain chain(st);
+  if (int e = quant_token_rows(x, rows, K, xq, xs, st)) return e;
+  (void)chain_first();
+  // Tiles of 256 tokens read the weights least often; with few rows an expert they only take ring space from the weights.
+  return rows / experts > 64 ? launch_group<256>(xq, p, st) : launch_group<64>(xq, p, st);
 }
