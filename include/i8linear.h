@@ -366,7 +366,7 @@ I8L_API int i8l_combine_backward(const void* rows, const void* weights, const in
  *   offsets int32 [experts + 1] on the device, non-decreasing, or NULL: one matrix (experts = 1) for all rows.  Rows in front
  *   of offsets[0] and from offsets[experts] on come out zero.
  * N a multiple of 8, K of 16 and at most 131072 (the int32 sum cannot overflow), experts <= 1024, rows >= 0.  x, w_q, y, bias
- * 16-byte aligned.  workspace: i8l_token_linear_workspace bytes, 256-byte aligned.
+ * 16-byte aligned.  workspace: i8l_token_linear_workspace bytes, 256-byte aligned, may be NULL where that is 0.
  * The row and channel scales are those of the reference's double_channel variant (triton/double-channle_fwd32.py:295-311).
  */
 I8L_API int64_t i8l_token_linear_workspace(int64_t rows, int64_t K);

@@ -74,7 +74,7 @@ def test_combine_refusals(lib, p, change, code):
     (dict(wq=8), -2), (dict(y=8), -2), (dict(bias=8), -2), (dict(bias=0), NO_DEVICE), (dict(space=0), -6), (dict(work=16), -2), (dict(work=None), -6),
 ])
 def test_token_linear_refusals(lib, p, change, code):
-    a = dict(x=0, wq=0, ws=0, offsets=0, bias=None, y=0, rows=5, experts=4, N=16, K=32, flags=0, work=0, space=1 << 14)
+    a = dict(x=0, wq=0, ws=0, offsets=0, bias=None, y=0, rows=9, experts=4, N=16, K=32, flags=0, work=0, space=1 << 14)
     a.update(change)
     at = lambda off: None if off is None else p + off  # noqa: E731
     rc = lib.i8l_token_linear(at(a["x"]), at(a["wq"]), at(a["ws"]), at(a["offsets"]), at(a["bias"]), at(a["y"]), a["rows"], a["experts"], a["N"],
@@ -86,7 +86,9 @@ def test_workspace_sizes(lib):
     assert lib.i8l_sort_workspace(512, 2, 8) == 0                      # few choices need none
     assert lib.i8l_sort_workspace(513, 2, 8) == 2 * 8 * 4              # chunks of 1024 choices
     assert lib.i8l_sort_workspace(1 << 20, 8, 1024) == 2048 * 1024 * 4
-    assert lib.i8l_token_linear_workspace(3, 48) == 256 + 256
+    assert lib.i8l_token_linear_workspace(9, 48) == 512 + 256
+    assert lib.i8l_token_linear_workspace(8, 48) == 0                  # few rows: one launch
+    assert lib.i8l_token_linear_workspace(1, 131072) == 131072 + 256   # but long ones
     assert lib.i8l_token_linear_workspace(0, 48) == 0
 
 

@@ -12,6 +12,15 @@ if torch.cuda.is_available():
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 
 
+@pytest.fixture(params=["native", "python"])
+def path(request, monkeypatch):
+    """The native host path, and the Python one that takes what it leaves."""
+    if request.param == "python":
+        class Leaves:
+            sort_tokens = combine = token_linear = staticmethod(lambda *a: None)
+        monkeypatch.setattr(K, "host", lambda: Leaves)
+
+
 def _plain_layout(ids, experts, align, rows):
     """offsets, pos, src by a loop over the choices."""
     flat = ids.reshape(-1).tolist()
@@ -67,7 +76,7 @@ def _ids(g, T, k, E, dtype, drop):
 
 
 @pytest.mark.parametrize("T,H,k,E,align,dtype,idt,drop", CASES)
-def test_sort_and_its_gradient(T, H, k, E, align, dtype, idt, drop):
+def test_sort_and_its_gradient(path, T, H, k, E, align, dtype, idt, drop):
     g = torch.Generator().manual_seed(T + H)
     x, ids = _values(g, (T, H), dtype).requires_grad_(), _ids(g, T, k, E, idt, drop)
     rows, offsets, pos, src = moe.sort_tokens(x, ids.to(DEV), E, align)
@@ -93,7 +102,7 @@ def test_sort_and_its_gradient(T, H, k, E, align, dtype, idt, drop):
 
 @pytest.mark.parametrize("T,H,k,E,align,dtype,idt,drop", CASES)
 @pytest.mark.parametrize("wide_weights", [True, False])
-def test_combine_and_its_gradients(T, H, k, E, align, dtype, idt, drop, wide_weights):
+def test_combine_and_its_gradients(path, T, H, k, E, align, dtype, idt, drop, wide_weights):
     g = torch.Generator().manual_seed(T + 3 * H)
     R = K.sorted_rows(T, k, E, align)
     _, pos, src = _plain_layout(_ids(g, T, k, E, idt, drop), E, align, R)
@@ -132,7 +141,7 @@ def test_combine_and_its_gradients(T, H, k, E, align, dtype, idt, drop, wide_wei
     assert (dweights[(pos < 0).to(DEV)] == 0).all()
 
 
-def test_gradients_against_differences():
+def test_gradients_against_differences(path):
     """y is linear in x and in the weights: a difference over a whole step is the derivative, up to the roundings of 32 bits."""
     g = torch.Generator().manual_seed(5)
     T, H, k, E = 37, 100, 3, 5
@@ -152,7 +161,7 @@ def test_gradients_against_differences():
             assert abs(a - b) <= 2.0 ** -24 * 375 * T * H, (a, b)
 
 
-def test_only_the_gradients_that_are_wanted():
+def test_only_the_gradients_that_are_wanted(path):
     g = torch.Generator().manual_seed(6)
     x, ids = _values(g, (6, 16), BF16), torch.randint(0, 3, (6, 2), generator=g).to(DEV)
     rows, offsets, pos, src = moe.sort_tokens(x, ids, 3)
@@ -166,6 +175,19 @@ def test_only_the_gradients_that_are_wanted():
         assert torch.equal(torch.autograd.grad(moe.combine(*t, pos, src).sum(), t[i])[0], want[i])
     with torch.no_grad():
         assert not moe.combine(*both, pos, src).requires_grad
+
+
+def test_a_second_gradient_is_refused(path):
+    x, ids = torch.randn(6, 16, device=DEV).requires_grad_(), torch.randint(0, 3, (6, 2), device=DEV)
+    w = torch.rand(6, 2, device=DEV).requires_grad_()
+    rows, offsets, pos, src = moe.sort_tokens(x, ids, 3)
+    (dx,) = torch.autograd.grad(rows.square().sum(), x, create_graph=True)   # its incoming gradient depends on x
+    with pytest.raises(RuntimeError, match="twice"):
+        dx.sum().backward()
+    y = moe.combine(rows.detach().requires_grad_(), w, pos, src)
+    (dw,) = torch.autograd.grad(y.sum(), w, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        dw.sum().backward()
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
@@ -218,7 +240,7 @@ def test_infinities_and_nan_pass_through():
     assert torch.equal(torch.nan_to_num(y, 7.0, 9.0), torch.nan_to_num(x, 7.0, 9.0))
 
 
-def test_streams_and_graphs():
+def test_streams_and_graphs(path):
     """On a stream of its own, captured and replayed on new values and new choices, the backward pass in the graph too."""
     g = torch.Generator().manual_seed(8)
     for T in (4, 900):   # one launch, three
@@ -251,7 +273,7 @@ def test_streams_and_graphs():
             assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
-def test_wrappers_refuse_shapes_and_types():
+def test_wrappers_refuse_shapes_and_types(path):
     x, ids = torch.zeros(4, 8, dtype=BF16, device=DEV), torch.zeros(4, 2, dtype=torch.int64, device=DEV)
     for bad in (dict(x=x.double()), dict(x=x.int()), dict(x=x[0]), dict(x=x[None]), dict(ids=ids.short()), dict(ids=ids.float()), dict(ids=ids[:3]),
                 dict(ids=ids[:, 0]), dict(experts=0), dict(align=0), dict(ids=ids.cpu())):

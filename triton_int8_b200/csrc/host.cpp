@@ -1,9 +1,9 @@
-// Host side of the composed calls for plain tensors: argument checks, allocations and the autograd node of the INT8
-// linear without the Python interpreter in between.  Small calls are bound by it: 128x1024x1024 forward 47 us a call in
+// Host side of the composed calls and of the expert layers for plain tensors: argument checks, allocations and the autograd nodes
+// without the Python interpreter in between.  Small calls are bound by it: 128x1024x1024 forward 47 us a call in
 // Python against 18 us on the device, forward and backward of 512x1024x1024 205 us against 58.
 //
-// Everything here handles one case, contiguous bf16 CUDA tensors of matching shapes outside of tracing, transforms and
-// modes, and returns None for any other: the callers in kernels.py and linear.py then take the Python path, which
+// Everything here handles one case, contiguous CUDA tensors (bf16, in the expert layers fp16 and fp32 too) of matching shapes outside of
+// tracing, transforms and modes, and returns None for any other: the callers in kernels.py and linear.py then take the Python path, which
 // accepts or refuses it.  The entry points of libi8linear.so are passed in by address (setup), so that the library in
 // use is the one that _lib.py has loaded.
 #define PY_SSIZE_T_CLEAN
@@ -18,6 +18,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <array>
@@ -34,6 +35,12 @@ using torch::autograd::variable_list;
 decltype(&i8l_quant_gemm) lib_quant_gemm = nullptr;
 decltype(&i8l_linear_backward_bias) lib_linear_backward = nullptr;
 decltype(&i8l_status_peek) lib_status_peek = nullptr;
+decltype(&i8l_sort_workspace) lib_sort_workspace = nullptr;
+decltype(&i8l_sort_tokens) lib_sort_tokens = nullptr;
+decltype(&i8l_combine) lib_combine = nullptr;
+decltype(&i8l_combine_backward) lib_combine_backward = nullptr;
+decltype(&i8l_token_linear_workspace) lib_token_workspace = nullptr;
+decltype(&i8l_token_linear) lib_token_linear = nullptr;
 PyObject* on_error = nullptr;       // (entry point, code, device index): raises
 PyObject* on_timeout = nullptr;     // (device index): raises, or returns where there is nothing to report now
 PyObject* open_status = nullptr;    // (device index) -> (status word, poller), as integers
@@ -102,11 +109,10 @@ void report_timeout(int dev) {   // an earlier GEMM gave up a wait
   Py_DECREF(r);
 }
 
-// A dense bf16 CUDA tensor with its own memory and nothing that a dispatcher would have to see.
-bool plain(const Tensor& t) {
+// A dense CUDA tensor with its own memory and nothing that a dispatcher would have to see.
+bool dense(const Tensor& t) {
   const auto ks = t.key_set();
-  return t.is_cuda() && t.scalar_type() == at::kBFloat16 && t.layout() == at::kStrided && t.is_contiguous() &&
-         t.get_device() < MAX_DEVICES &&
+  return t.is_cuda() && t.layout() == at::kStrided && t.is_contiguous() && t.get_device() < MAX_DEVICES &&
          !ks.has_any(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot,
                                           c10::DispatchKey::Functionalize, c10::DispatchKey::Conjugate,
                                           c10::DispatchKey::Negative, c10::DispatchKey::ZeroTensor,
@@ -114,6 +120,7 @@ bool plain(const Tensor& t) {
                                           c10::DispatchKey::FuncTorchBatchedDecomposition, c10::DispatchKey::BatchedNestedTensor,
                                           c10::DispatchKey::Batched}));
 }
+bool plain(const Tensor& t) { return t.scalar_type() == at::kBFloat16 && dense(t); }
 // No mode, transform or tracer looks at what this thread does.
 bool plain_thread() {
   const auto inc = c10::impl::tls_local_dispatch_key_set().included_;
@@ -273,8 +280,219 @@ struct Int8LinearNode : torch::autograd::Function<Int8LinearNode> {
   }
 };
 
+// ------------------------------------------------------------------------------------------------ expert layers
+int dtype_of(const Tensor& t) {   // negative: a type that the kernels do not take
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return I8L_DTYPE_BF16;
+    case at::kHalf: return I8L_DTYPE_F16;
+    case at::kFloat: return I8L_DTYPE_F32;
+    default: return -1;
+  }
+}
+void* stream_of(int dev) { return c10::cuda::getCurrentCUDAStream(dev).stream(); }
+template <typename T> T* at_of(const Tensor& t) { return static_cast<T*>(t.data_ptr()); }
+
+struct Sorted {
+  Tensor rows, offsets, pos, src;
+};
+Sorted sort_tokens(const Tensor& x, const Tensor& ids, int experts, int64_t align) {
+  const int64_t T = x.size(0), H = x.size(1), k = ids.size(1), n = T * k;
+  const int64_t R = (n + std::min<int64_t>(experts, n) * (align - 1) + align - 1) / align * align;
+  const int dev = x.get_device();
+  const c10::cuda::CUDAGuard guard(dev);
+  const auto i32 = x.options().dtype(at::kInt);
+  Sorted s{at::empty({R, H}, x.options()), at::empty({experts + 1}, i32), at::empty({T, k}, i32), at::empty({R}, i32)};
+  const int64_t size = lib_sort_workspace(T, (int)k, experts);
+  const Tensor ws = size ? bytes(size, x) : Tensor();
+  check("i8l_sort_tokens",
+        lib_sort_tokens(x.data_ptr(), ids.data_ptr(), ids.scalar_type() == at::kLong, T, H, (int)k, experts, align, dtype_of(x), R,
+                        s.rows.data_ptr(), at_of<int32_t>(s.offsets), at_of<int32_t>(s.pos), at_of<int32_t>(s.src),
+                        size ? ws.data_ptr() : nullptr, size, stream_of(dev)),
+        dev);
+  return s;
+}
+// weights undefined: ones
+Tensor combine(const Tensor& rows, const Tensor& weights, const Tensor& pos) {
+  const int64_t T = pos.size(0), k = pos.size(1), R = rows.size(0), H = rows.size(1);
+  const int dev = rows.get_device();
+  const c10::cuda::CUDAGuard guard(dev);
+  Tensor y = at::empty({T, H}, rows.options());
+  check("i8l_combine",
+        lib_combine(rows.data_ptr(), weights.defined() ? weights.data_ptr() : nullptr, at_of<int32_t>(pos), R, T, H, (int)k, dtype_of(rows),
+                    weights.defined() ? dtype_of(weights) : I8L_DTYPE_F32, y.data_ptr(), stream_of(dev)),
+        dev);
+  return y;
+}
+// A gradient that came in, as the kernels read it.
+Tensor incoming(const char* name, const Tensor& d) {
+  const Tensor dy = d.contiguous();
+  TORCH_CHECK(plain_thread() && dense(dy), name, ": its gradient cannot be taken under a transform or of a tensor subclass");
+  return dy;
+}
+// The gradients have no gradient of their own: where a graph of them is made, going back through it is an error.
+Tensor once(const char* name, const Tensor& result, const Tensor& dy) {
+  if (!result.defined() || !at::GradMode::is_enabled() || !dy.requires_grad()) return result;
+  const auto error = std::make_shared<torch::autograd::DelayedError>(std::string("trying to differentiate twice ") + name + ", which has a first gradient only", 1);
+  return (*error)({result.detach().requires_grad_(true)})[0];
+}
+
+struct SortNode : torch::autograd::Function<SortNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& ids, int64_t experts, int64_t align) {
+    const Sorted s = sort_tokens(x, ids, (int)experts, align);
+    ctx->mark_non_differentiable({s.offsets, s.pos, s.src});
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({s.pos});
+    return {s.rows, s.offsets, s.pos, s.src};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    const Tensor pos = ctx->get_saved_variables()[0], dy = incoming("sort_tokens", grads[0]);
+    return {once("sort_tokens", combine(dy.detach(), Tensor(), pos), grads[0]), Tensor(), Tensor(), Tensor()};   // the sum of a token's rows
+  }
+};
+
+struct CombineNode : torch::autograd::Function<CombineNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& weights, const Tensor& pos, const Tensor& src) {
+    ctx->save_for_backward({rows, weights, pos, src});
+    return combine(rows, weights, pos);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &rows = saved[0], &weights = saved[1], &pos = saved[2], &src = saved[3], dy = incoming("combine", grads[0]);
+    const int64_t T = pos.size(0), k = pos.size(1), R = rows.size(0), H = rows.size(1);
+    const int dev = rows.get_device();
+    const c10::cuda::CUDAGuard guard(dev);
+    Tensor drows, dweights;
+    if (ctx->needs_input_grad(0)) drows = at::empty({R, H}, rows.options());
+    if (ctx->needs_input_grad(1)) dweights = at::empty({T, k}, weights.options());
+    check("i8l_combine_backward",
+          lib_combine_backward(rows.data_ptr(), weights.data_ptr(), at_of<int32_t>(pos), at_of<int32_t>(src), dy.data_ptr(), R, T, H, (int)k,
+                               dtype_of(rows), dtype_of(weights), drows.defined() ? drows.data_ptr() : nullptr,
+                               dweights.defined() ? dweights.data_ptr() : nullptr, stream_of(dev)),
+          dev);
+    // a graph of the gradients would lead to dy, the rows and the weights alike
+    const Tensor& any = rows.requires_grad() ? rows : weights.requires_grad() ? weights : grads[0];
+    return {once("combine", drows, any), once("combine", dweights, any), Tensor(), Tensor()};
+  }
+};
+
+Tensor token_linear(const Tensor& x, const Tensor& wq, const Tensor& ws, const Tensor& offsets, const Tensor& bias, int64_t E, bool f32) {
+  const int64_t N = wq.size(-2), K = wq.size(-1), R = x.numel() / K;
+  const int dev = x.get_device();
+  const c10::cuda::CUDAGuard guard(dev);
+  Status& status = status_of(dev);
+  auto shape = x.sizes().vec();
+  shape.back() = N;
+  Tensor y = at::empty(shape, x.options().dtype(f32 ? at::kFloat : at::kBFloat16));
+  const int64_t size = lib_token_workspace(R, K);
+  const Tensor work = size ? bytes(size, x) : Tensor();
+  check("i8l_token_linear",
+        lib_token_linear(x.data_ptr(), at_of<int8_t>(wq), at_of<float>(ws), offsets.defined() ? at_of<int32_t>(offsets) : nullptr,
+                         bias.defined() ? bias.data_ptr() : nullptr, y.data_ptr(), R, (int)E, N, K, f32 ? I8L_GEMM_OUT_F32 : 0,
+                         size ? work.data_ptr() : nullptr, size, status.word.load(std::memory_order_relaxed), stream_of(dev)),
+        dev);
+  return y;
+}
+
 // ------------------------------------------------------------------------------------------------ Python
 bool exact_tensor(PyObject* o) { return THPVariable_CheckExact(o); }
+bool ints(const Tensor& t, const Tensor& like, at::IntArrayRef shape) {
+  return t.scalar_type() == at::kInt && dense(t) && t.device() == like.device() && t.sizes() == shape;
+}
+bool forward_mode(const Tensor& t) { return t._fw_grad(0).defined(); }
+bool at_16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+
+// sort_tokens(x, ids, experts, align) -> (rows, offsets, pos, src), or None
+PyObject* py_sort_tokens(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4) {
+    PyErr_SetString(PyExc_TypeError, "sort_tokens takes 4 arguments");
+    return nullptr;
+  }
+  if (!exact_tensor(args[0]) || !exact_tensor(args[1])) Py_RETURN_NONE;
+  const Tensor x = THPVariable_Unpack(args[0]), ids = THPVariable_Unpack(args[1]);
+  const long long experts = PyLong_AsLongLong(args[2]), align = PyLong_AsLongLong(args[3]);
+  if (PyErr_Occurred()) return nullptr;
+  constexpr int64_t MOST = 1ll << 30;   // sizes whose products fit 64 bits; the library refuses what is too large for it
+  if (!plain_thread() || !dense(x) || dtype_of(x) < 0 || x.dim() != 2 || !dense(ids) || ids.dim() != 2 || ids.device() != x.device() ||
+      (ids.scalar_type() != at::kInt && ids.scalar_type() != at::kLong) || ids.size(0) != x.size(0) || x.size(0) > MOST || ids.size(1) > MOST ||
+      experts < 1 || experts > 65536 || align < 1 || align > 65536 || forward_mode(x))
+    Py_RETURN_NONE;
+  Sorted s;
+  {
+    const WithoutGil no_gil;
+    if (at::GradMode::is_enabled() && x.requires_grad()) {
+      const variable_list r = SortNode::apply(x, ids, (int64_t)experts, (int64_t)align);
+      s = Sorted{r[0], r[1], r[2], r[3]};
+    } else {
+      const at::AutoGradMode off(false);
+      s = sort_tokens(x, ids, (int)experts, align);
+    }
+  }
+  return Py_BuildValue("NNNN", THPVariable_Wrap(s.rows), THPVariable_Wrap(s.offsets), THPVariable_Wrap(s.pos), THPVariable_Wrap(s.src));
+  END_HANDLE_TH_ERRORS
+}
+
+// combine(rows, weights, pos, src) -> y, or None
+PyObject* py_combine(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4) {
+    PyErr_SetString(PyExc_TypeError, "combine takes 4 arguments");
+    return nullptr;
+  }
+  for (int i = 0; i < 4; ++i)
+    if (!exact_tensor(args[i])) Py_RETURN_NONE;
+  const Tensor rows = THPVariable_Unpack(args[0]), weights = THPVariable_Unpack(args[1]), pos = THPVariable_Unpack(args[2]),
+               src = THPVariable_Unpack(args[3]);
+  if (!plain_thread() || !dense(rows) || dtype_of(rows) < 0 || rows.dim() != 2 || !dense(weights) || weights.dim() != 2 ||
+      (weights.scalar_type() != at::kFloat && weights.scalar_type() != rows.scalar_type()) || weights.device() != rows.device() ||
+      !ints(pos, rows, weights.sizes()) || !ints(src, rows, {rows.size(0)}) || forward_mode(rows) || forward_mode(weights))
+    Py_RETURN_NONE;
+  Tensor y;
+  {
+    const WithoutGil no_gil;
+    if (at::GradMode::is_enabled() && (rows.requires_grad() || weights.requires_grad())) y = CombineNode::apply(rows, weights, pos, src);
+    else {
+      const at::AutoGradMode off(false);
+      y = combine(rows, weights, pos);
+    }
+  }
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+// token_linear(x, wq, ws, offsets or None, bias or None, fp32 output) -> y, or None.  wq [N, K] without offsets, [E, N, K] with them.
+PyObject* py_token_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6) {
+    PyErr_SetString(PyExc_TypeError, "token_linear takes 6 arguments");
+    return nullptr;
+  }
+  for (int i = 0; i < 5; ++i)
+    if (!exact_tensor(args[i]) && !(i >= 3 && args[i] == Py_None)) Py_RETURN_NONE;
+  const Tensor x = THPVariable_Unpack(args[0]), wq = THPVariable_Unpack(args[1]), ws = THPVariable_Unpack(args[2]);
+  Tensor offsets, bias;
+  if (args[3] != Py_None) offsets = THPVariable_Unpack(args[3]);
+  if (args[4] != Py_None) bias = THPVariable_Unpack(args[4]);
+  const int dims = offsets.defined() ? 3 : 2;
+  if (!plain_thread() || !plain(x) || !dense(wq) || !dense(ws) || wq.scalar_type() != at::kChar || ws.scalar_type() != at::kFloat ||
+      wq.dim() != dims || (dims == 3 ? x.dim() != 2 : x.dim() < 1) || x.size(-1) != wq.size(-1) || wq.size(-1) == 0 ||
+      ws.sizes() != wq.sizes().slice(0, dims - 1) || wq.device() != x.device() || ws.device() != x.device() ||
+      (offsets.defined() && !ints(offsets, x, {wq.size(0) + 1})) || wq.size(0) > 65536 * (dims == 2 ? 65536ll : 1) ||
+      (bias.defined() && (!plain(bias) || bias.device() != x.device() || bias.sizes() != ws.sizes() || !at_16(bias))) || !at_16(x) || !at_16(wq) ||
+      forward_mode(x) || forward_mode(ws) || (bias.defined() && forward_mode(bias)) ||
+      (at::GradMode::is_enabled() && (x.requires_grad() || ws.requires_grad() || (bias.defined() && bias.requires_grad()))))
+    Py_RETURN_NONE;
+  Tensor y;
+  {
+    const WithoutGil no_gil;
+    report_timeout(x.get_device());
+    const at::AutoGradMode off(false);
+    y = token_linear(x, wq, ws, offsets, bias, dims == 3 ? wq.size(0) : 1, args[5] == Py_True);
+  }
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
 
 // linear(x, weight, bias or None, gran, qmode, hadamard, flags, whole_k) -> y, or None
 PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -361,10 +579,28 @@ PyObject* py_setup(PyObject*, PyObject* args) {
   Py_RETURN_NONE;
 }
 
+// setup_experts(addresses of i8l_sort_workspace, i8l_sort_tokens, i8l_combine, i8l_combine_backward, i8l_token_linear_workspace,
+// i8l_token_linear)
+PyObject* py_setup_experts(PyObject*, PyObject* args) {
+  unsigned long long a[6];
+  if (!PyArg_ParseTuple(args, "KKKKKK", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5])) return nullptr;
+  lib_sort_workspace = reinterpret_cast<decltype(lib_sort_workspace)>(a[0]);
+  lib_sort_tokens = reinterpret_cast<decltype(lib_sort_tokens)>(a[1]);
+  lib_combine = reinterpret_cast<decltype(lib_combine)>(a[2]);
+  lib_combine_backward = reinterpret_cast<decltype(lib_combine_backward)>(a[3]);
+  lib_token_workspace = reinterpret_cast<decltype(lib_token_workspace)>(a[4]);
+  lib_token_linear = reinterpret_cast<decltype(lib_token_linear)>(a[5]);
+  Py_RETURN_NONE;
+}
+
 PyMethodDef methods[] = {
     {"setup", py_setup, METH_VARARGS, nullptr},
     {"linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_linear)), METH_FASTCALL, nullptr},
     {"quant_gemm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_quant_gemm)), METH_FASTCALL, nullptr},
+    {"setup_experts", py_setup_experts, METH_VARARGS, nullptr},
+    {"sort_tokens", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_sort_tokens)), METH_FASTCALL, nullptr},
+    {"combine", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_combine)), METH_FASTCALL, nullptr},
+    {"token_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_token_linear)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -447,7 +447,12 @@ cudaError_t allow_smem(Kernel kernel, std::atomic<int>* allowed, int bytes) {
   return e;
 }
 
+// The rows that the kernel for few of them takes at once, 0: too many, or too long for its shared memory.
 constexpr int FEW_SMEM = 64 * 1024;
+int few_rows(int64_t rows, int64_t K) {
+  const int mt = rows == 1 ? 1 : rows == 2 ? 2 : rows <= 4 ? 4 : 8;
+  return rows <= 8 && mt * K <= FEW_SMEM ? mt : 0;
+}
 template <int MT> int launch_few(const TokenArgs& a, cudaStream_t st) {
   static std::atomic<int> allowed[64];
   I8L_CUDA_OK(allow_smem(few_rows_kernel<MT>, allowed, FEW_SMEM));
@@ -487,7 +492,7 @@ template <int TOK> int launch_group(const int8_t* xq, GroupArgs& p, cudaStream_t
 using namespace i8l;
 
 extern "C" int64_t i8l_token_linear_workspace(int64_t rows, int64_t K) {
-  if (rows <= 0 || K <= 0 || rows >= (1ll << 31) || K > MAX_K) return 0;
+  if (rows <= 0 || K <= 0 || rows >= (1ll << 31) || K > MAX_K || few_rows(rows, K)) return 0;
   return (rows * K + 255) / 256 * 256 + (4 * rows + 255) / 256 * 256;
 }
 
@@ -500,10 +505,11 @@ extern "C" int i8l_token_linear(const void* x, const int8_t* w_q, const float* w
   if (experts < 1 || experts > MAX_EXPERTS || (!offsets && experts != 1) || experts * N >= (1ll << 31))
     return fail(I8L_ERR_SHAPE, "i8l_token_linear: %d experts, 1 to %d are possible, and one without offsets", experts, MAX_EXPERTS);
   if (flags & ~I8L_GEMM_OUT_F32) return fail(I8L_ERR_ARG, "i8l_token_linear: unknown flags %d", flags);
-  if (!w_q || !w_scale || (rows && (!x || !y || !workspace))) return fail(I8L_ERR_ARG, "i8l_token_linear: null pointer");
+  if (!w_q || !w_scale || (rows && (!x || !y))) return fail(I8L_ERR_ARG, "i8l_token_linear: null pointer");
   if (!aligned16(x) || !aligned16(w_q) || !aligned16(y) || !aligned16(bias) || (reinterpret_cast<uintptr_t>(workspace) & 255))
     return fail(I8L_ERR_ALIGN, "i8l_token_linear: x, w_q, y and bias must be 16-byte aligned, the workspace 256-byte");
-  if (workspace_bytes < i8l_token_linear_workspace(rows, K))
+  const int64_t need = i8l_token_linear_workspace(rows, K);
+  if (need && (!workspace || workspace_bytes < need))
     return fail(I8L_ERR_ARG, "i8l_token_linear: workspace of %lld bytes is too small", (long long)workspace_bytes);
   if (!rows) return I8L_OK;
   if (int e = check_arch()) return e;
@@ -512,10 +518,12 @@ extern "C" int i8l_token_linear(const void* x, const int8_t* w_q, const float* w
   a.bias = static_cast<const __nv_bfloat16*>(bias); a.y = y;
   a.rows = rows; a.N = N; a.K = K; a.experts = experts; a.out_f32 = (flags & I8L_GEMM_OUT_F32) ? 1 : 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (rows == 1 && K <= FEW_SMEM) return launch_few<1>(a, st);
-  if (rows == 2 && K <= FEW_SMEM / 2) return launch_few<2>(a, st);
-  if (rows <= 4 && K <= FEW_SMEM / 4) return launch_few<4>(a, st);
-  if (rows <= 8 && K <= FEW_SMEM / 8) return launch_few<8>(a, st);
+  switch (few_rows(rows, K)) {
+    case 1: return launch_few<1>(a, st);
+    case 2: return launch_few<2>(a, st);
+    case 4: return launch_few<4>(a, st);
+    case 8: return launch_few<8>(a, st);
+  }
   GroupArgs p{};
   p.t = a;
   int8_t* xq = static_cast<int8_t*>(workspace);

@@ -152,6 +152,8 @@ def host():
                               f"`python -m triton_int8_b200.build` ({e})") from e
         mod.setup(L.address("i8l_quant_gemm"), L.address("i8l_linear_backward_bias"), L.address("i8l_status_peek"), _on_error,
                   _on_timeout, _open_status, _backward_in_python)
+        mod.setup_experts(*(L.address(n) for n in ("i8l_sort_workspace", "i8l_sort_tokens", "i8l_combine", "i8l_combine_backward",
+                                                   "i8l_token_linear_workspace", "i8l_token_linear")))
         _host = mod
     return _host
 
@@ -518,10 +520,12 @@ def token_linear(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, offsets=No
     x, wq, ws = _aligned(x), _aligned(wq), ws.contiguous()
     y = torch.empty((R, N), dtype=out_dtype, device=dev)
     size = L.load().i8l_token_linear_workspace(R, Kd)
-    work = torch.empty((size,), dtype=torch.int8, device=dev)
-    status = device_status(dev) if status is None else status
+    work = torch.empty((size,), dtype=torch.int8, device=dev) if size else None
+    if status is None:
+        poll_status(dev)   # an earlier kernel that gave up a wait
+        status = device_status(dev)
     _call("i8l_token_linear", dev, x.data_ptr(), wq.data_ptr(), ws.data_ptr(), _ptr(offsets), _ptr(bias), y.data_ptr(), R, E, N, Kd,
-          L.GEMM_OUT_F32 if out_dtype == torch.float32 else 0, work.data_ptr(), size, status.data_ptr(),
+          L.GEMM_OUT_F32 if out_dtype == torch.float32 else 0, _ptr(work), size, status.data_ptr(),
           tensors=(wq, ws, offsets, bias, status))
     return y
 

@@ -162,6 +162,10 @@ def linear_w8a8(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, bias=None, 
     -> [..., N], bf16 or fp32.  One scale a row of x and one an output channel, as double_channel has them
     (triton/double-channle_fwd32.py:295-311 without the rotation), any number of rows, N a multiple of 8, K of 16.  There is no
     gradient: inputs that want one are refused."""
+    if out_dtype in (torch.bfloat16, torch.float32) and not torch.compiler.is_compiling():   # plain tensors
+        y = K.host().token_linear(x, wq, ws, None, bias, out_dtype == torch.float32)
+        if y is not None:
+            return y
     K.refuse_gradient("linear_w8a8", x, ws, bias)
     if wq.dim() != 2 or ws.dim() != 1 or (bias is not None and bias.dim() != 1):
         raise ValueError("linear_w8a8: wq [N, K], ws [N], bias [N]")

@@ -10,10 +10,17 @@ expert layers.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from . import kernels as K
+
+
+def _once(name: str, inputs, *results):
+    """The gradients have no gradient of their own: where a graph of them is made, going back through it is an error."""
+    if not torch.is_grad_enabled() or not any(t.requires_grad for t in inputs):
+        return results
+    error = torch._C._functions.DelayedError(f"trying to differentiate twice {name}, which has a first gradient only".encode(), 1)
+    return tuple(None if r is None else error(r.detach().requires_grad_()) for r in results)
 
 
 class _SortFn(torch.autograd.Function):
@@ -26,11 +33,11 @@ class _SortFn(torch.autograd.Function):
         return rows, offsets, pos, src
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, drows, *_):
         if drows is None:
             return None, None, None, None
-        return K.combine(drows, None, ctx.saved_tensors[0]), None, None, None   # a token's gradient is the sum of its rows'
+        dx = K.combine(drows.detach(), None, ctx.saved_tensors[0])   # a token's gradient is the sum of its rows'
+        return *_once("sort_tokens", [drows], dx), None, None, None
 
 
 class _CombineFn(torch.autograd.Function):
@@ -41,10 +48,10 @@ class _CombineFn(torch.autograd.Function):
         return K.combine(rows, weights, pos)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        drows, dweights = K.combine_backward(*ctx.saved_tensors, dy, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
-        return drows, dweights, None, None
+        saved = ctx.saved_tensors
+        grads = K.combine_backward(*(t.detach() for t in saved), dy.detach(), ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        return *_once("combine", [dy, *saved], *grads), None, None
 
 
 def sort_tokens(x: torch.Tensor, ids: torch.Tensor, experts: int, align: int = 1):
@@ -56,6 +63,10 @@ def sort_tokens(x: torch.Tensor, ids: torch.Tensor, experts: int, align: int = 1
     pos int32 [T, k]: the row of a choice, or -1 where the id is outside [0, experts): such a choice is dropped (another rank's
     expert, or one above its capacity).  src int32 [R]: the inverse, t * k + j or -1.
     At most 1024 experts and 64 choices a token.  Gradient: that of x, summed in 32 bits."""
+    if not torch.compiler.is_compiling():   # plain tensors: the same calls and autograd node without the interpreter
+        done = K.host().sort_tokens(x, ids, experts, align)
+        if done is not None:
+            return done
     if torch.is_grad_enabled() and x.requires_grad:
         return _SortFn.apply(x, ids, experts, align)
     return K.sort_tokens(x, ids, experts, align)
@@ -65,6 +76,10 @@ def combine(rows: torch.Tensor, weights: torch.Tensor, pos: torch.Tensor, src: t
     """rows [R, H], weights [T, k] (fp32 or the rows' type), pos and src of sort_tokens -> y [T, H] of the rows' type,
     y[t] = sum over j of weights[t, j] * rows[pos[t, j]], added in 32 bits and rounded once.  Dropped choices add nothing.
     Gradients: those of rows (zero for rows of no choice) and of weights (zero for dropped choices)."""
+    if not torch.compiler.is_compiling():
+        y = K.host().combine(rows, weights, pos, src)
+        if y is not None:
+            return y
     if torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
         return _CombineFn.apply(rows, weights, pos, src)
     return K.combine(rows, weights, pos)
@@ -84,5 +99,11 @@ def expert_linear(rows: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, offset
     come out zero.  N a multiple of 8, K of 16; any number of rows, one included.
     The weights are integers, there is no gradient: inputs that want one are refused.  Int8Linear trains, on segments of
     sort_tokens(align=128)."""
+    if out_dtype in (torch.bfloat16, torch.float32) and offsets is not None and not torch.compiler.is_compiling():
+        y = K.host().token_linear(rows, wq, ws, offsets, bias, out_dtype == torch.float32)
+        if y is not None:
+            return y
     K.refuse_gradient("expert_linear", rows, ws, bias)
+    if offsets is None:
+        raise ValueError("expert_linear: offsets are needed (linear_w8a8 takes one matrix for all rows)")
     return K.token_linear(rows, wq, ws, offsets, bias, out_dtype)
