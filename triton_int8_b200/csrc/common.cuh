@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/i8linear.h"
 
 namespace i8l {
@@ -47,6 +49,19 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
     if (_e != cudaSuccess)                                                                 \
       return i8l::fail(I8L_ERR_CUDA, "%s failed: %s", #expr, cudaGetErrorString(_e));      \
   } while (0)
+
+// Once a device: the shared memory that a kernel may be launched with.
+constexpr int MAX_SMEM_DEVICES = 64;
+template <typename Kernel>
+inline cudaError_t allow_smem(Kernel kernel, std::atomic<int>* allowed, int bytes) {
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return e;
+  const bool known = dev >= 0 && dev < MAX_SMEM_DEVICES;
+  if (known && allowed[dev].load(std::memory_order_acquire) >= bytes) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && known) allowed[dev].store(bytes, std::memory_order_release);
+  return e;
+}
 
 // ---------------------------------------------------------------- chains of launches
 // The kernels of one composed call (compose.cu) follow one another on a stream and are launched with programmatic

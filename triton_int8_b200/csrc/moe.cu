@@ -7,20 +7,17 @@
 // of a choice (-1: the id is no expert's), src its inverse (-1: a row of no choice, which is zero).
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace i8l {
 namespace {
 
 constexpr int MAX_EXPERTS = 1024, MAX_CHOICES = 64;
-constexpr int THREADS = 256;
+constexpr int THREADS = 256, MIN_LANES = 8;   // of a block; of a token
 
-// ------------------------------------------------------------------------------------------ types
-// One access of a row: 16 bytes, or an element where rows or pointers are not 16-byte aligned.
-template <typename T, bool WIDE> struct Piece;
-template <typename T> struct Piece<T, true> { using type = uint4; static constexpr int N = 16 / sizeof(T); };
-template <typename T> struct Piece<T, false> { using type = T; static constexpr int N = 1; };
-
+// ------------------------------------------------------------------------------------------ rows, 16 bytes at a time
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -29,19 +26,57 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-template <typename T, bool WIDE>
-__device__ __forceinline__ void unpack(const typename Piece<T, WIDE>::type& p, float* v) {
+template <typename T> constexpr int PER_PIECE = 16 / sizeof(T);
+template <typename T> __device__ __forceinline__ void unpack(const uint4& p, float* v) {
   const T* e = reinterpret_cast<const T*>(&p);
 #pragma unroll
-  for (int i = 0; i < Piece<T, WIDE>::N; ++i) v[i] = to_float(e[i]);
+  for (int i = 0; i < PER_PIECE<T>; ++i) v[i] = to_float(e[i]);
 }
-template <typename T, bool WIDE>
-__device__ __forceinline__ typename Piece<T, WIDE>::type pack(const float* v) {
-  typename Piece<T, WIDE>::type p;
+template <typename T> __device__ __forceinline__ uint4 pack(const float* v) {
+  uint4 p;
   T* e = reinterpret_cast<T*>(&p);
 #pragma unroll
-  for (int i = 0; i < Piece<T, WIDE>::N; ++i) e[i] = from_float<T>(v[i]);
+  for (int i = 0; i < PER_PIECE<T>; ++i) e[i] = from_float<T>(v[i]);
   return p;
+}
+
+// Rows that are no multiple of 16 bytes, or do not start on one, still move 16 bytes at a time: stores go to the aligned pieces of the
+// row that is written, and what belongs there is put together from the two aligned pieces that it lies across in the row that is
+// read.  Element by element a row of 1405 fp16 took 2 bytes an access: sort of 4099 tokens 41 us, its gradient 38.
+// Only pieces that the row itself has bytes in are read (memory comes in whole ones); of a piece at the row's ends the
+// elements that belong to the row are written.
+// Aligned piece q of a row written at `to` begins at this byte of the row, negative for the first one of a row that starts inside it.
+__device__ __forceinline__ int64_t piece_begin(const void* to, int64_t q) { return 16 * q - (int64_t)(reinterpret_cast<uintptr_t>(to) & 15); }
+__device__ __forceinline__ int64_t pieces_of(const void* to, int64_t bytes) { return (bytes + (int64_t)(reinterpret_cast<uintptr_t>(to) & 15) + 15) / 16; }
+__device__ __forceinline__ uint4 load_across(const char* row, int64_t bytes, int64_t at) {   // 16 bytes from byte `at` of the row on
+  const char* p = row + at;
+  const int off = (int)(reinterpret_cast<uintptr_t>(p) & 15);
+  p -= off;
+  uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+  if (p + 16 > row && p < row + bytes) lo = *reinterpret_cast<const uint4*>(p);
+  if (off && p + 32 > row && p + 16 < row + bytes) hi = *reinterpret_cast<const uint4*>(p + 16);
+  uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+  for (int i = 0; i < 6; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
+  const int bits = (off & 3) * 8;
+  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+}
+template <typename T> __device__ __forceinline__ void store_piece(char* row, int64_t bytes, int64_t at, const uint4& v) {   // an aligned one
+  if (at >= 0 && at + 16 <= bytes) {
+    *reinterpret_cast<uint4*>(row + at) = v;
+    return;
+  }
+  const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+  for (int i = 0; i < PER_PIECE<T>; ++i)
+    if (at + i * (int)sizeof(T) >= 0 && at + i * (int)sizeof(T) < bytes) *reinterpret_cast<T*>(row + at + i * (int)sizeof(T)) = e[i];
+}
+// Zeros a row, a warp's work.
+template <typename T> __device__ __forceinline__ void clear_row(void* rows, int64_t bytes, int64_t r, int lane) {
+  char* row = static_cast<char*>(rows) + r * bytes;
+  for (int64_t q = lane; q < pieces_of(row, bytes); q += 32) store_piece<T>(row, bytes, piece_begin(row, q), make_uint4(0, 0, 0, 0));
 }
 
 __device__ __forceinline__ int64_t load_id(const void* ids, int wide, int64_t i) {
@@ -60,7 +95,7 @@ struct SortArgs {
   void* rows;
   int32_t *offsets, *pos, *src;
   int32_t* hist;        // [blocks, experts]: choices of each expert in each chunk
-  int64_t tokens, pieces;   // pieces of a row
+  int64_t tokens, bytes;   // bytes of a row
   int n, k, experts, align, n_rows, ids64;
   int chunk, blocks;    // choices of a block in the counting and placing kernels
   int lanes;            // threads of a token in the copying kernels, a power of two
@@ -86,41 +121,54 @@ __device__ __forceinline__ void scan_offsets(const int* count, int* offsets, int
   }
 }
 
-// Copies the row of token t to the rows of its choices, `lanes` threads a token.
-template <typename P>
+// Copies the row of token t to the rows of its choices, `lanes` threads a token, four pieces in flight each.  ODD: see load_across.
+template <typename T, bool ODD>
 __device__ __forceinline__ void copy_row(const SortArgs& a, int64_t t, int l, const int32_t* pos) {
-  const P* from = static_cast<const P*>(a.x) + t * a.pieces;
-  for (int64_t c0 = l; c0 < a.pieces; c0 += 4 * a.lanes) {
-    P v[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (c0 + u * a.lanes < a.pieces) v[u] = from[c0 + u * a.lanes];
+  constexpr int U = 4;
+  const char* from = static_cast<const char*>(a.x) + t * a.bytes;
+  if (ODD) {
     for (int j = 0; j < a.k; ++j) {
       const int r = pos[j];
       if (r < 0) continue;
-      P* to = static_cast<P*>(a.rows) + (int64_t)r * a.pieces;
+      char* to = static_cast<char*>(a.rows) + (int64_t)r * a.bytes;
+      const int64_t pieces = pieces_of(to, a.bytes);
+      for (int64_t q0 = l; q0 < pieces; q0 += U * a.lanes) {
+        uint4 v[U];
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (c0 + u * a.lanes < a.pieces) to[c0 + u * a.lanes] = v[u];
+        for (int u = 0; u < U; ++u)
+          if (q0 + u * a.lanes < pieces) v[u] = load_across(from, a.bytes, piece_begin(to, q0 + u * a.lanes));
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (q0 + u * a.lanes < pieces) store_piece<T>(to, a.bytes, piece_begin(to, q0 + u * a.lanes), v[u]);
+      }
+    }
+    return;
+  }
+  const int64_t pieces = a.bytes / 16;
+  for (int64_t c0 = l; c0 < pieces; c0 += U * a.lanes) {
+    uint4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (c0 + u * a.lanes < pieces) v[u] = reinterpret_cast<const uint4*>(from)[c0 + u * a.lanes];
+    for (int j = 0; j < a.k; ++j) {
+      const int r = pos[j];
+      if (r < 0) continue;
+      uint4* to = reinterpret_cast<uint4*>(static_cast<char*>(a.rows) + (int64_t)r * a.bytes);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (c0 + u * a.lanes < pieces) to[c0 + u * a.lanes] = v[u];
     }
   }
-}
-template <typename P>
-__device__ __forceinline__ void clear_row(void* rows, int64_t pieces, int64_t r, int lane) {
-  P zero;
-  memset(&zero, 0, sizeof(P));
-  P* to = static_cast<P*>(rows) + r * pieces;
-  for (int64_t c = lane; c < pieces; c += 32) to[c] = zero;
 }
 
 // Few choices: one launch.  Every block counts all of them for itself (they fit its shared memory) and copies the rows of its
 // tokens; the rows of no choice are spread over all warps.
 constexpr int SMALL_SORT = 1024;
-template <typename P>
+template <typename T, bool ODD>
 __global__ void __launch_bounds__(THREADS) sort_small_kernel(const SortArgs a) {
   __shared__ int16_t expert[SMALL_SORT];
   __shared__ int count[MAX_EXPERTS], offsets[MAX_EXPERTS + 1];
-  __shared__ int32_t pos[THREADS / 32][MAX_CHOICES];   // of the block's tokens: at most one a warp
+  __shared__ int32_t pos[THREADS / MIN_LANES][MAX_CHOICES];   // of the block's tokens
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   for (int e = tid; e < a.experts; e += THREADS) count[e] = 0;
   __syncthreads();
@@ -154,7 +202,7 @@ __global__ void __launch_bounds__(THREADS) sort_small_kernel(const SortArgs a) {
   }
   __syncthreads();
   const int64_t t = t0 + tid / a.lanes;
-  if (t < a.tokens) copy_row<P>(a, t, tid & (a.lanes - 1), pos[tid / a.lanes]);
+  if (t < a.tokens) copy_row<T, ODD>(a, t, tid & (a.lanes - 1), pos[tid / a.lanes]);
   for (int64_t r = (int64_t)blockIdx.x * (THREADS / 32) + warp; r < a.n_rows; r += (int64_t)gridDim.x * (THREADS / 32)) {
     int lo = 0, hi = a.experts;   // the expert whose rows r is among: offsets[lo] <= r < offsets[hi], or lo = experts
     if (r >= offsets[a.experts]) lo = a.experts;
@@ -166,7 +214,7 @@ __global__ void __launch_bounds__(THREADS) sort_small_kernel(const SortArgs a) {
       }
     if (lo < a.experts && r - offsets[lo] < count[lo]) continue;
     if (lane == 0) a.src[r] = -1;
-    clear_row<P>(a.rows, a.pieces, r, lane);
+    clear_row<T>(a.rows, a.bytes, r, lane);
   }
 }
 
@@ -242,14 +290,14 @@ __global__ void __launch_bounds__(THREADS) sort_place_kernel(const SortArgs a) {
   }
 }
 
-template <typename P>
+template <typename T, bool ODD>
 __global__ void __launch_bounds__(THREADS) sort_copy_kernel(const SortArgs a) {
   chain_wait();
   const int64_t t = (int64_t)blockIdx.x * (THREADS / a.lanes) + threadIdx.x / a.lanes;
-  if (t < a.tokens) copy_row<P>(a, t, threadIdx.x & (a.lanes - 1), a.pos + t * a.k);
+  if (t < a.tokens) copy_row<T, ODD>(a, t, threadIdx.x & (a.lanes - 1), a.pos + t * a.k);
   const int lane = threadIdx.x & 31;
   for (int64_t r = (int64_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5); r < a.n_rows; r += (int64_t)gridDim.x * (THREADS / 32))
-    if (a.src[r] < 0) clear_row<P>(a.rows, a.pieces, r, lane);
+    if (a.src[r] < 0) clear_row<T>(a.rows, a.bytes, r, lane);
 }
 
 // ------------------------------------------------------------------------------------------ the way back
@@ -258,7 +306,7 @@ struct CombineArgs {
   const int32_t *pos, *src;
   const void* dy;
   void *y, *drows, *dweights;
-  int64_t tokens, pieces, n_rows;
+  int64_t tokens, bytes, n_rows;   // bytes of a row
   int k, lanes;
 };
 
@@ -268,87 +316,133 @@ __device__ __forceinline__ int row_of(const CombineArgs& a, int64_t i) {
   const int r = a.pos[i];
   return r >= 0 && r < a.n_rows ? r : -1;
 }
+template <bool ODD> __device__ __forceinline__ uint4 load_piece(const char* row, int64_t bytes, int64_t at) {
+  return ODD ? load_across(row, bytes, at) : *reinterpret_cast<const uint4*>(row + at);
+}
 
-// y[t] = sum over j of w[t, j] * rows[pos[t, j]], in the order of j, in 32 bits and rounded once.  Choices four at a time, so that
-// their loads are in flight together.
-template <typename T, typename W, bool WIDE>
+// y[t] = sum over j of w[t, j] * rows[pos[t, j]], in the order of j, in 32 bits and rounded once.  J choices at a time and U
+// pieces of their rows, so that J * U loads are in flight together.
+template <typename T, typename W, bool ODD, int J, int U>
 __global__ void __launch_bounds__(THREADS) combine_kernel(const CombineArgs a) {
-  using P = typename Piece<T, WIDE>::type;
-  constexpr int N = Piece<T, WIDE>::N;
+  constexpr int N = PER_PIECE<T>;
   const int64_t t = (int64_t)blockIdx.x * (THREADS / a.lanes) + threadIdx.x / a.lanes;
   if (t >= a.tokens) return;
-  for (int64_t c = threadIdx.x & (a.lanes - 1); c < a.pieces; c += a.lanes) {
-    float acc[N];
+  char* y = static_cast<char*>(a.y) + t * a.bytes;
+  const int64_t pieces = pieces_of(y, a.bytes);
+  for (int64_t q0 = threadIdx.x & (a.lanes - 1); q0 < pieces; q0 += U * a.lanes) {
+    float acc[U][N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] = 0.f;
-    for (int j0 = 0; j0 < a.k; j0 += 4) {
-      P v[4];
-      float w[4];
-      int r[4];
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) r[u] = j0 + u < a.k ? row_of(a, t * a.k + j0 + u) : -1;
+      for (int i = 0; i < N; ++i) acc[u][i] = 0.f;
+    for (int j0 = 0; j0 < a.k; j0 += J) {
+      uint4 v[J][U];
+      float w[J];
+      int r[J];
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (r[u] >= 0) {
-          v[u] = static_cast<const P*>(a.rows)[(int64_t)r[u] * a.pieces + c];
-          w[u] = weight_of<W>(a.weights, t * a.k + j0 + u);
-        }
+      for (int j = 0; j < J; ++j) {
+        r[j] = j0 + j < a.k ? row_of(a, t * a.k + j0 + j) : -1;
+        w[j] = r[j] >= 0 ? weight_of<W>(a.weights, t * a.k + j0 + j) : 0.f;
+      }
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (r[u] >= 0) {
-          float f[N];
-          unpack<T, WIDE>(v[u], f);
+      for (int j = 0; j < J; ++j)
 #pragma unroll
-          for (int i = 0; i < N; ++i) acc[i] = fmaf(w[u], f[i], acc[i]);
+        for (int u = 0; u < U; ++u)
+          if (r[j] >= 0 && q0 + u * a.lanes < pieces)
+            v[j][u] = load_piece<ODD>(static_cast<const char*>(a.rows) + (int64_t)r[j] * a.bytes, a.bytes, piece_begin(y, q0 + u * a.lanes));
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        if (r[j] >= 0) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            float f[N];
+            unpack<T>(v[j][u], f);
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[u][i] = fmaf(w[j], f[i], acc[u][i]);
+          }
         }
     }
-    static_cast<P*>(a.y)[t * a.pieces + c] = pack<T, WIDE>(acc);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (q0 + u * a.lanes < pieces) store_piece<T>(y, a.bytes, piece_begin(y, q0 + u * a.lanes), pack<T>(acc[u]));
   }
 }
 
 // drows[pos[t, j]] = w[t, j] * dy[t], rows of no choice zero; dw[t, j] = the sum of dy[t] * rows[pos[t, j]], added in an order that
-// depends on the sizes only.  A row is written by the choice that src names, so that rows are written once whatever pos holds.
-template <typename T, typename W, bool WIDE>
+// depends on the sizes and the alignment only.  A row is written by the choice that src names, so that rows are written once whatever pos
+// holds.  J choices at a time share the loads of dy; of ODD rows each has pieces of its own, so those come one by one.
+template <typename T, typename W, bool ODD, int J, int U>
 __global__ void __launch_bounds__(THREADS) combine_backward_kernel(const CombineArgs a) {
-  using P = typename Piece<T, WIDE>::type;
-  constexpr int N = Piece<T, WIDE>::N;
+  static_assert(!ODD || J == 1, "one choice at a time");
+  constexpr int N = PER_PIECE<T>;
   __shared__ float part[THREADS / 32][MAX_CHOICES];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = threadIdx.x & (a.lanes - 1);
   const int64_t t = (int64_t)blockIdx.x * (THREADS / a.lanes) + threadIdx.x / a.lanes;
-  if (t < a.tokens) {   // the same for all threads of a warp
-    const P* dy = static_cast<const P*>(a.dy) + t * a.pieces;
-    for (int j = 0; j < a.k; ++j) {
-      const int64_t i = t * a.k + j;
-      const int r = row_of(a, i);
-      float dot = 0.f;
-      if (r >= 0) {
-        const float w = weight_of<W>(a.weights, i);
-        const bool owner = a.drows && a.src[r] == (int32_t)i;
-        const P* row = static_cast<const P*>(a.rows) + (int64_t)r * a.pieces;
-        P* drow = static_cast<P*>(a.drows) + (int64_t)r * a.pieces;
-        for (int64_t c = threadIdx.x & (a.lanes - 1); c < a.pieces; c += a.lanes) {
-          float g[N], f[N];
-          unpack<T, WIDE>(dy[c], g);
-          if (a.dweights) {
-            unpack<T, WIDE>(row[c], f);
+  const bool live = t < a.tokens;
+  const char* dy = static_cast<const char*>(a.dy) + t * a.bytes;
+  for (int j0 = 0; j0 < a.k; j0 += J) {
+    float w[J], dot[J];
+    const char* from[J];   // the choice's row, null: nothing to read, or to write
+    char* to[J];
 #pragma unroll
-            for (int q = 0; q < N; ++q) dot = fmaf(g[q], f[q], dot);
+    for (int j = 0; j < J; ++j) {
+      const int64_t i = t * a.k + j0 + j;
+      const int r = live && j0 + j < a.k ? row_of(a, i) : -1;
+      w[j] = r >= 0 ? weight_of<W>(a.weights, i) : 0.f;
+      from[j] = r >= 0 && a.dweights ? static_cast<const char*>(a.rows) + (int64_t)r * a.bytes : nullptr;
+      to[j] = r >= 0 && a.drows && a.src[r] == (int32_t)i ? static_cast<char*>(a.drows) + (int64_t)r * a.bytes : nullptr;
+      dot[j] = 0.f;
+    }
+    // pieces of the row written; without one, of the row read
+    const void* grid = ODD ? (to[0] ? to[0] : from[0]) : nullptr;
+    const int64_t pieces = live && (!ODD || grid) ? pieces_of(grid, a.bytes) : 0;
+    for (int64_t q0 = l; q0 < pieces; q0 += U * a.lanes) {
+      uint4 g[U], v[J][U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (q0 + u * a.lanes < pieces) g[u] = load_piece<ODD>(dy, a.bytes, piece_begin(grid, q0 + u * a.lanes));
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (from[j] && q0 + u * a.lanes < pieces) v[j][u] = load_piece<ODD>(from[j], a.bytes, piece_begin(grid, q0 + u * a.lanes));
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (q0 + u * a.lanes >= pieces) break;
+        const int64_t at = piece_begin(grid, q0 + u * a.lanes);
+        float d[N];
+        unpack<T>(g[u], d);
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          if (from[j]) {
+            float f[N];
+            unpack<T>(v[j][u], f);
+#pragma unroll
+            for (int q = 0; q < N; ++q)
+              if (!ODD || (at + q * (int)sizeof(T) >= 0 && at + q * (int)sizeof(T) < a.bytes)) dot[j] = fmaf(d[q], f[q], dot[j]);   // what lies around the row is others'
           }
-          if (owner) {
+          if (to[j]) {
+            float f[N];
 #pragma unroll
-            for (int q = 0; q < N; ++q) g[q] *= w;
-            drow[c] = pack<T, WIDE>(g);
+            for (int q = 0; q < N; ++q) f[q] = d[q] * w[j];
+            store_piece<T>(to[j], a.bytes, at, pack<T>(f));
           }
         }
       }
-      if (a.dweights) {
+    }
+    if (a.dweights) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-        if (lane == 0) part[warp][j] = dot;
+      for (int j = 0; j < J; ++j) {
+        for (int o = (a.lanes < 32 ? a.lanes : 32) / 2; o > 0; o >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
+        if (j0 + j >= a.k) continue;
+        if (a.lanes >= 32) {
+          if (lane == 0) part[warp][j0 + j] = dot[j];
+        } else if (l == 0 && live)
+          static_cast<W*>(a.dweights)[t * a.k + j0 + j] = from_float<W>(dot[j]);
       }
     }
   }
-  if (a.dweights) {
+  if (a.dweights && a.lanes >= 32) {
     __syncthreads();
     const int warps = a.lanes / 32, per_block = THREADS / a.lanes;
     for (int q = threadIdx.x; q < per_block * a.k; q += THREADS) {
@@ -356,20 +450,187 @@ __global__ void __launch_bounds__(THREADS) combine_backward_kernel(const Combine
       const int64_t at = (int64_t)blockIdx.x * per_block + g;
       if (at >= a.tokens) break;
       float sum = 0.f;
-      for (int w = 0; w < warps; ++w) sum += part[g * warps + w][j];
+      for (int i = 0; i < warps; ++i) sum += part[g * warps + i][j];
       static_cast<W*>(a.dweights)[at * a.k + j] = from_float<W>(sum);
     }
   }
   if (a.drows)
     for (int64_t r = (int64_t)blockIdx.x * (THREADS / 32) + warp; r < a.n_rows; r += (int64_t)gridDim.x * (THREADS / 32))
-      if (a.src[r] < 0) clear_row<P>(a.drows, a.pieces, r, lane);
+      if (a.src[r] < 0) clear_row<T>(a.drows, a.bytes, r, lane);
+}
+
+// The same two for many tokens with rows of whole 16 bytes.  What bounds them is how many bytes are in flight: with loads into registers
+// 14 warps of an SM waited for 64 KB at most, and for their positions first.  Here every lane copies its pieces asynchronously into a
+// ring of its own in shared memory, two stages of two choices' (and dy's) pieces, and reads back what it copied itself, so nobody waits
+// for anybody else.  The positions of a token are loaded while the one before it is copied; a warp goes through whole tokens.
+// 16384 x 4096 bf16, 2 choices: 82 -> 65 us (6.2 TB/s) and 149 -> 120 (5.7).  8 warps and twice the stages 73 and 129, half the
+// pieces and twice the stages 65 and 125.
+constexpr int RING_THREADS = 512, RING_STAGES = 2, RING_PIECES = 4, RING_J = 2, RING_SEG = 32 * RING_PIECES;   // a stage holds a segment of each row
+constexpr int RING_MAX_CHOICES = 32;   // one a lane
+template <bool BACKWARD> constexpr int RING_ROWS = RING_J + (BACKWARD ? 1 : 0);
+template <bool BACKWARD> constexpr int RING_SMEM = RING_THREADS / 32 * RING_STAGES * RING_ROWS<BACKWARD> * RING_SEG * 16;
+
+__device__ __forceinline__ void copy_async(uint32_t to, const uint4* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ uint4 load_shared(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+
+template <typename T, typename W, bool BACKWARD>
+__global__ void __launch_bounds__(RING_THREADS) combine_ring_kernel(const CombineArgs a) {
+  constexpr int N = PER_PIECE<T>, ROWS = RING_ROWS<BACKWARD>, STAGE = ROWS * RING_SEG * 16;
+  extern __shared__ __align__(16) uint8_t ring_raw[];
+  const int lane = threadIdx.x & 31;
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(ring_raw) + (threadIdx.x >> 5) * RING_STAGES * STAGE + lane * 16;
+  const int64_t warps = (int64_t)gridDim.x * (RING_THREADS / 32), me = (int64_t)(threadIdx.x >> 5) * gridDim.x + blockIdx.x;
+  const int64_t pieces = a.bytes / 16;
+  const int segments = (int)((pieces + RING_SEG - 1) / RING_SEG);
+  const bool dots = BACKWARD && a.dweights;
+
+  // Where a walk over the warp's stages is.
+  struct Walk {
+    int64_t token;
+    int segment, choice;   // the first choice of the stage
+  };
+  auto step = [&](Walk& w) {   // whether it enters another token
+    w.choice += RING_J;
+    if (w.choice < a.k) return false;
+    w.choice = 0;
+    if (++w.segment < segments) return false;
+    w.segment = 0;
+    w.token += warps;
+    return true;
+  };
+  // The lane's choice of a token: its row, or -1.
+  auto choice_of = [&](int64_t token) { return token < a.tokens && lane < a.k ? row_of(a, token * a.k + lane) : -1; };
+
+  Walk issue{me, 0, 0}, use{me, 0, 0};
+  int issue_row = choice_of(me), next_row = choice_of(me + warps), slot = 0;
+  auto issue_stage = [&]() {
+    if (issue.token < a.tokens) {
+      const uint32_t to = ring + slot * STAGE;
+      const int64_t c0 = (int64_t)issue.segment * RING_SEG + lane;
+      if (BACKWARD && issue.choice == 0) {
+#pragma unroll
+        for (int p = 0; p < RING_PIECES; ++p)
+          if (c0 + p * 32 < pieces) copy_async(to + (RING_J * RING_PIECES + p) * 512, static_cast<const uint4*>(a.dy) + issue.token * pieces + c0 + p * 32);
+      }
+      if (!BACKWARD || dots) {
+#pragma unroll
+        for (int j = 0; j < RING_J; ++j) {
+          const int r = __shfl_sync(0xffffffffu, issue_row, (issue.choice + j) & 31);
+          if (issue.choice + j < a.k && r >= 0) {
+#pragma unroll
+            for (int p = 0; p < RING_PIECES; ++p)
+              if (c0 + p * 32 < pieces) copy_async(to + (j * RING_PIECES + p) * 512, static_cast<const uint4*>(a.rows) + (int64_t)r * pieces + c0 + p * 32);
+          }
+        }
+      }
+      if (step(issue)) {
+        issue_row = next_row;
+        next_row = choice_of(issue.token + warps);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");   // a group a stage, also where there is nothing to copy
+    slot = slot + 1 == RING_STAGES ? 0 : slot + 1;
+  };
+
+  // What the lane's choice of the token in use needs: row, weight, and the choice that may write the row.
+  auto weight_at = [&](int64_t token) { return token < a.tokens && lane < a.k ? weight_of<W>(a.weights, token * a.k + lane) : 0.f; };
+  auto owner_of = [&](int row) { return BACKWARD && a.drows && row >= 0 ? a.src[row] : -1; };
+  int row = choice_of(me), later_row = choice_of(me + warps), owner = owner_of(row), later_owner = owner_of(later_row);
+  float weight = weight_at(me), later_weight = weight_at(me + warps), dot = 0.f;   // dot: of the lane's choice
+
+  for (int i = 0; i < RING_STAGES - 1; ++i) issue_stage();
+  uint4 g[RING_PIECES];
+  float acc[RING_PIECES][N];
+  for (int at = 0; use.token < a.tokens; at = at + 1 == RING_STAGES ? 0 : at + 1) {
+    issue_stage();
+    asm volatile("cp.async.wait_group %0;" ::"n"(RING_STAGES - 1) : "memory");
+    const uint32_t from = ring + at * STAGE;
+    const int64_t c0 = (int64_t)use.segment * RING_SEG + lane;
+    if (use.choice == 0) {
+#pragma unroll
+      for (int p = 0; p < RING_PIECES; ++p) {
+        if (BACKWARD) g[p] = load_shared(from + (RING_J * RING_PIECES + p) * 512);
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[p][i] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < RING_J; ++j) {
+      const int c = use.choice + j, r = __shfl_sync(0xffffffffu, row, c & 31);
+      const float w = __shfl_sync(0xffffffffu, weight, c & 31);
+      const bool mine = BACKWARD && __shfl_sync(0xffffffffu, owner, c & 31) == (int32_t)(use.token * a.k + c);
+      if (c >= a.k || r < 0) continue;
+      float sum = 0.f;
+#pragma unroll
+      for (int p = 0; p < RING_PIECES; ++p) {
+        if (c0 + p * 32 >= pieces) break;
+        float f[N];
+        if (!BACKWARD) {
+          unpack<T>(load_shared(from + (j * RING_PIECES + p) * 512), f);
+#pragma unroll
+          for (int i = 0; i < N; ++i) acc[p][i] = fmaf(w, f[i], acc[p][i]);
+        } else {
+          float d[N];
+          unpack<T>(g[p], d);
+          if (dots) {
+            unpack<T>(load_shared(from + (j * RING_PIECES + p) * 512), f);
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum = fmaf(d[i], f[i], sum);
+          }
+          if (mine) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) d[i] *= w;
+            static_cast<uint4*>(a.drows)[(int64_t)r * pieces + c0 + p * 32] = pack<T>(d);
+          }
+        }
+      }
+      if (dots) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == c) dot += sum;
+      }
+    }
+    const Walk done = use;
+    if (!BACKWARD && use.choice + RING_J >= a.k) {
+#pragma unroll
+      for (int p = 0; p < RING_PIECES; ++p)
+        if (c0 + p * 32 < pieces) static_cast<uint4*>(a.y)[use.token * pieces + c0 + p * 32] = pack<T>(acc[p]);
+    }
+    if (step(use)) {
+      if (dots && lane < a.k) static_cast<W*>(a.dweights)[done.token * a.k + lane] = from_float<W>(dot);
+      dot = 0.f;
+      row = later_row;
+      weight = later_weight;
+      owner = later_owner;
+      later_row = choice_of(use.token + warps);
+      later_weight = weight_at(use.token + warps);
+      later_owner = owner_of(later_row);
+    }
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (BACKWARD && a.drows)
+    for (int64_t r = me; r < a.n_rows; r += warps)
+      if (a.src[r] < 0) clear_row<T>(a.drows, a.bytes, r, lane);
 }
 
 // ------------------------------------------------------------------------------------------ host
-// Threads of a token: a warp's worth at least (dot products are added up within warps), at most the block, four pieces each in between.
-int lanes_for(int64_t pieces) {
-  int lanes = 32;
-  while (lanes < THREADS && lanes * 4 < pieces) lanes *= 2;
+// The ring wants a token or more for most of its 2368 warps, and rows that fill a warp's pieces: forward, 2 choices of bf16,
+// 1024 x 4096 5.6 us against 5.1, 2048 x 4096 9.4 against 12.1; backward 512 x 4096 7.3 against 4.5, 1024 x 4096 8.9 against 9.2,
+// 1037 x 2176 fp32 8.8 against 12.3.
+bool ring_fits(const CombineArgs& a, bool backward) {
+  return a.k <= RING_MAX_CHOICES && a.bytes > 512 && a.tokens >= (backward ? 1024 : 2048);
+}
+// Threads of a token: one a piece for short rows, else what has four pieces each in flight, up to the block.
+int lanes_for(int64_t bytes) {
+  int lanes = MIN_LANES;
+  while (lanes < 32 && lanes * 16 < bytes) lanes *= 2;
+  while (lanes >= 32 && lanes < THREADS && lanes * 64 < bytes) lanes *= 2;
   return lanes;
 }
 int elem_size(int dtype) { return dtype == I8L_DTYPE_F32 ? 4 : 2; }
@@ -384,30 +645,46 @@ int check_rows(const char* name, int64_t tokens, int64_t cols, int64_t rows, int
 }
 bool aligned_to(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
+template <typename T, typename W, bool BACKWARD>
+int launch_ring(const CombineArgs& a, cudaStream_t st) {
+  static std::atomic<int> allowed[MAX_SMEM_DEVICES];
+  auto kernel = combine_ring_kernel<T, W, BACKWARD>;
+  I8L_CUDA_OK(allow_smem(kernel, allowed, RING_SMEM<BACKWARD>));
+  kernel<<<sm_count(), RING_THREADS, RING_SMEM<BACKWARD>, st>>>(a);
+  I8L_CUDA_OK(cudaGetLastError());
+  return I8L_OK;
+}
 template <typename T, typename W>
-int launch_combine(CombineArgs a, bool backward, bool wide, cudaStream_t st) {
-  const unsigned grid = (unsigned)((a.tokens + THREADS / a.lanes - 1) / (THREADS / a.lanes));
+int launch_combine(const CombineArgs& a, bool backward, bool odd, cudaStream_t st) {
+  if (!odd && ring_fits(a, backward)) return backward ? launch_ring<T, W, true>(a, st) : launch_ring<T, W, false>(a, st);
+  const unsigned tokens = (unsigned)((a.tokens + THREADS / a.lanes - 1) / (THREADS / a.lanes));
+  const unsigned grid = tokens ? tokens : 1;   // without tokens there still are gradients of rows to clear
+  const bool one = a.bytes <= 16 * a.lanes;    // a piece a thread: fewer registers, more blocks on an SM
   if (backward) {
-    const unsigned blocks = grid ? grid : 1;   // without tokens there still are rows to clear
-    if (wide) combine_backward_kernel<T, W, true><<<blocks, THREADS, 0, st>>>(a);
-    else combine_backward_kernel<T, W, false><<<blocks, THREADS, 0, st>>>(a);
+    if (odd) combine_backward_kernel<T, W, true, 1, 2><<<grid, THREADS, 0, st>>>(a);
+    else if (one) combine_backward_kernel<T, W, false, 2, 1><<<grid, THREADS, 0, st>>>(a);
+    else if (a.k <= 2) combine_backward_kernel<T, W, false, 2, 2><<<grid, THREADS, 0, st>>>(a);
+    else combine_backward_kernel<T, W, false, 4, 2><<<grid, THREADS, 0, st>>>(a);
   } else {
-    if (wide) combine_kernel<T, W, true><<<grid, THREADS, 0, st>>>(a);
-    else combine_kernel<T, W, false><<<grid, THREADS, 0, st>>>(a);
+    if (odd) combine_kernel<T, W, true, 2, 2><<<grid, THREADS, 0, st>>>(a);
+    else if (one) combine_kernel<T, W, false, 4, 1><<<grid, THREADS, 0, st>>>(a);
+    else if (a.k <= 2) combine_kernel<T, W, false, 2, 4><<<grid, THREADS, 0, st>>>(a);
+    else combine_kernel<T, W, false, 4, 2><<<grid, THREADS, 0, st>>>(a);
   }
   I8L_CUDA_OK(cudaGetLastError());
   return I8L_OK;
 }
 template <typename T>
-int launch_combine(const CombineArgs& a, int wdtype, int dtype, bool backward, bool wide, cudaStream_t st) {
-  return wdtype == I8L_DTYPE_F32 ? launch_combine<T, float>(a, backward, wide, st) : launch_combine<T, T>(a, backward, wide, st);
+int launch_combine(const CombineArgs& a, int wdtype, bool backward, bool odd, cudaStream_t st) {
+  return wdtype == I8L_DTYPE_F32 ? launch_combine<T, float>(a, backward, odd, st) : launch_combine<T, T>(a, backward, odd, st);
 }
-int run_combine(CombineArgs a, int64_t cols, int dtype, int wdtype, bool backward, bool wide, cudaStream_t st) {
-  a.pieces = wide ? cols * elem_size(dtype) / 16 : cols;
-  a.lanes = lanes_for(a.pieces);
-  if (dtype == I8L_DTYPE_F32) return launch_combine<float, float>(a, backward, wide, st);
-  if (dtype == I8L_DTYPE_F16) return launch_combine<__half>(a, wdtype, dtype, backward, wide, st);
-  return launch_combine<__nv_bfloat16>(a, wdtype, dtype, backward, wide, st);
+int run_combine(CombineArgs a, int64_t cols, int dtype, int wdtype, bool backward, cudaStream_t st) {
+  a.bytes = cols * elem_size(dtype);
+  a.lanes = lanes_for(a.bytes);
+  const bool odd = a.bytes % 16 || !aligned16(a.rows) || !aligned16(a.y) || !aligned16(a.dy) || !aligned16(a.drows);
+  if (dtype == I8L_DTYPE_F32) return launch_combine<float, float>(a, backward, odd, st);
+  if (dtype == I8L_DTYPE_F16) return launch_combine<__half>(a, wdtype, backward, odd, st);
+  return launch_combine<__nv_bfloat16>(a, wdtype, backward, odd, st);
 }
 
 }  // namespace
@@ -438,19 +715,19 @@ extern "C" int i8l_sort_tokens(const void* x, const void* ids, int ids64, int64_
     return fail(I8L_ERR_ARG, "i8l_sort_tokens: workspace of %lld bytes is too small", (long long)workspace_bytes);
   if (int e = check_arch()) return e;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool wide = cols * size % 16 == 0 && aligned16(x) && aligned16(out);
+  const bool odd = cols * size % 16 || !aligned16(x) || !aligned16(out);
   SortArgs a{};
   a.x = x; a.ids = ids; a.rows = out; a.offsets = offsets; a.pos = pos; a.src = src;
   a.hist = static_cast<int32_t*>(workspace);
-  a.tokens = tokens; a.pieces = wide ? cols * size / 16 : cols;
+  a.tokens = tokens; a.bytes = cols * size;
   a.n = (int)n; a.k = k; a.experts = experts; a.align = (int)align; a.n_rows = (int)rows; a.ids64 = ids64 ? 1 : 0;
-  a.lanes = lanes_for(a.pieces);
+  a.lanes = lanes_for(a.bytes);
   const unsigned copies = (unsigned)((tokens + THREADS / a.lanes - 1) / (THREADS / a.lanes));
   const unsigned grid = copies ? copies : 1;
   if (n <= SMALL_SORT) {
-    if (wide) sort_small_kernel<uint4><<<grid, THREADS, 0, st>>>(a);
-    else if (size == 4) sort_small_kernel<uint32_t><<<grid, THREADS, 0, st>>>(a);
-    else sort_small_kernel<uint16_t><<<grid, THREADS, 0, st>>>(a);
+    if (!odd) sort_small_kernel<uint32_t, false><<<grid, THREADS, 0, st>>>(a);
+    else if (size == 4) sort_small_kernel<uint32_t, true><<<grid, THREADS, 0, st>>>(a);
+    else sort_small_kernel<uint16_t, true><<<grid, THREADS, 0, st>>>(a);
     I8L_CUDA_OK(cudaGetLastError());
     return I8L_OK;
   }
@@ -460,9 +737,9 @@ extern "C" int i8l_sort_tokens(const void* x, const void* ids, int ids64, int64_
   (void)chain_first();
   I8L_CUDA_OK(launch(sort_count_kernel, dim3(a.blocks), THREADS, 0, st, a));
   I8L_CUDA_OK(launch(sort_place_kernel, dim3(a.blocks), THREADS, THREADS / 32 * experts * sizeof(int), st, a));
-  I8L_CUDA_OK(wide        ? launch(sort_copy_kernel<uint4>, dim3(grid), THREADS, 0, st, a)
-              : size == 4 ? launch(sort_copy_kernel<uint32_t>, dim3(grid), THREADS, 0, st, a)
-                          : launch(sort_copy_kernel<uint16_t>, dim3(grid), THREADS, 0, st, a));
+  I8L_CUDA_OK(!odd        ? launch(sort_copy_kernel<uint32_t, false>, dim3(grid), THREADS, 0, st, a)
+              : size == 4 ? launch(sort_copy_kernel<uint32_t, true>, dim3(grid), THREADS, 0, st, a)
+                          : launch(sort_copy_kernel<uint16_t, true>, dim3(grid), THREADS, 0, st, a));
   return I8L_OK;
 }
 
@@ -478,8 +755,7 @@ extern "C" int i8l_combine(const void* rows, const void* weights, const int32_t*
   CombineArgs a{};
   a.rows = rows; a.weights = weights; a.pos = pos; a.y = y;
   a.tokens = tokens; a.n_rows = n_rows; a.k = k;
-  const bool wide = cols * size % 16 == 0 && aligned16(rows) && aligned16(y);
-  return run_combine(a, cols, dtype, wdtype, false, wide, static_cast<cudaStream_t>(stream));
+  return run_combine(a, cols, dtype, wdtype, false, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int i8l_combine_backward(const void* rows, const void* weights, const int32_t* pos, const int32_t* src, const void* dy,
@@ -496,6 +772,5 @@ extern "C" int i8l_combine_backward(const void* rows, const void* weights, const
   CombineArgs a{};
   a.rows = rows; a.weights = weights; a.pos = pos; a.src = src; a.dy = dy; a.drows = drows; a.dweights = dweights;
   a.tokens = tokens; a.n_rows = n_rows; a.k = k;
-  const bool wide = cols * size % 16 == 0 && aligned16(rows) && aligned16(dy) && aligned16(drows);
-  return run_combine(a, cols, dtype, wdtype, true, wide, static_cast<cudaStream_t>(stream));
+  return run_combine(a, cols, dtype, wdtype, true, static_cast<cudaStream_t>(stream));
 }

@@ -434,19 +434,6 @@ group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
 }
 
 // ------------------------------------------------------------------------------------------ host
-// Once a device: the shared memory that a kernel may be launched with.
-template <typename Kernel>
-cudaError_t allow_smem(Kernel kernel, std::atomic<int>* allowed, int bytes) {
-  constexpr int DEVICES = 64;
-  int dev = 0;
-  if (cudaError_t e = cudaGetDevice(&dev)) return e;
-  const bool known = dev >= 0 && dev < DEVICES;
-  if (known && allowed[dev].load(std::memory_order_acquire) >= bytes) return cudaSuccess;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && known) allowed[dev].store(bytes, std::memory_order_release);
-  return e;
-}
-
 // The rows that the kernel for few of them takes at once, 0: too many, or too long for its shared memory.
 constexpr int FEW_SMEM = 64 * 1024;
 int few_rows(int64_t rows, int64_t K) {
@@ -454,7 +441,7 @@ int few_rows(int64_t rows, int64_t K) {
   return rows <= 8 && mt * K <= FEW_SMEM ? mt : 0;
 }
 template <int MT> int launch_few(const TokenArgs& a, cudaStream_t st) {
-  static std::atomic<int> allowed[64];
+  static std::atomic<int> allowed[MAX_SMEM_DEVICES];
   I8L_CUDA_OK(allow_smem(few_rows_kernel<MT>, allowed, FEW_SMEM));
   const int64_t segments = a.offsets ? (a.experts < a.rows ? a.experts : a.rows) : 1;
   few_rows_kernel<MT><<<dim3((unsigned)((a.N + FEW_COLS - 1) / FEW_COLS), (unsigned)segments), FEW_THREADS, MT * a.K, st>>>(a);
@@ -464,7 +451,7 @@ template <int MT> int launch_few(const TokenArgs& a, cudaStream_t st) {
 
 template <int TOK> int launch_group(const int8_t* xq, GroupArgs& p, cudaStream_t st) {
   using G = Grp<TOK>;
-  static std::atomic<int> allowed[64];
+  static std::atomic<int> allowed[MAX_SMEM_DEVICES];
   const TokenArgs& a = p.t;
   I8L_CUDA_OK(allow_smem(group_kernel<TOK>, allowed, G::smem(MAX_EXPERTS)));
   p.n_tiles = (int)((a.N + CHANNELS - 1) / CHANNELS);
