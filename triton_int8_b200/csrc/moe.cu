@@ -290,14 +290,37 @@ __global__ void __launch_bounds__(THREADS) sort_place_kernel(const SortArgs a) {
   }
 }
 
-template <typename T, bool ODD>
+// A token's row is read once and written to each of its places.
 __global__ void __launch_bounds__(THREADS) sort_copy_kernel(const SortArgs a) {
   chain_wait();
   const int64_t t = (int64_t)blockIdx.x * (THREADS / a.lanes) + threadIdx.x / a.lanes;
-  if (t < a.tokens) copy_row<T, ODD>(a, t, threadIdx.x & (a.lanes - 1), a.pos + t * a.k);
+  if (t < a.tokens) copy_row<uint32_t, false>(a, t, threadIdx.x & (a.lanes - 1), a.pos + t * a.k);
   const int lane = threadIdx.x & 31;
   for (int64_t r = (int64_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5); r < a.n_rows; r += (int64_t)gridDim.x * (THREADS / 32))
-    if (a.src[r] < 0) clear_row<T>(a.rows, a.bytes, r, lane);
+    if (a.src[r] < 0) clear_row<uint32_t>(a.rows, a.bytes, r, lane);
+}
+// Odd rows are put together for each place anyway: row by row, the rows of no choice among them, which are all alike much work.
+template <typename T>
+__global__ void __launch_bounds__(THREADS) sort_copy_odd_kernel(const SortArgs a) {
+  constexpr int U = 4;
+  chain_wait();
+  const int64_t r = (int64_t)blockIdx.x * (THREADS / a.lanes) + threadIdx.x / a.lanes;
+  if (r >= a.n_rows) return;
+  const int i = a.src[r];
+  const char* from = static_cast<const char*>(a.x) + (i < 0 ? 0 : i / a.k) * a.bytes;
+  char* to = static_cast<char*>(a.rows) + r * a.bytes;
+  const int64_t pieces = pieces_of(to, a.bytes);
+  for (int64_t q0 = threadIdx.x & (a.lanes - 1); q0 < pieces; q0 += U * a.lanes) {
+    uint4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      v[u] = make_uint4(0, 0, 0, 0);
+      if (i >= 0 && q0 + u * a.lanes < pieces) v[u] = load_across(from, a.bytes, piece_begin(to, q0 + u * a.lanes));
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (q0 + u * a.lanes < pieces) store_piece<T>(to, a.bytes, piece_begin(to, q0 + u * a.lanes), v[u]);
+  }
 }
 
 // ------------------------------------------------------------------------------------------ the way back
@@ -626,12 +649,20 @@ __global__ void __launch_bounds__(RING_THREADS) combine_ring_kernel(const Combin
 bool ring_fits(const CombineArgs& a, bool backward) {
   return a.k <= RING_MAX_CHOICES && a.bytes > 512 && a.tokens >= (backward ? 1024 : 2048);
 }
-// Threads of a token: one a piece for short rows, else what has four pieces each in flight, up to the block.
-int lanes_for(int64_t bytes) {
+// Threads of a token: one a piece for short rows and where there are few tokens to fill the SMs with, else what has four pieces each
+// in flight, up to the block.
+int lanes_for(int64_t bytes, int64_t tokens) {
+  const int64_t few = 2048ll * sm_count();
   int lanes = MIN_LANES;
-  while (lanes < 32 && lanes * 16 < bytes) lanes *= 2;
-  while (lanes >= 32 && lanes < THREADS && lanes * 64 < bytes) lanes *= 2;
+  while (lanes < THREADS && lanes * 16 < bytes && (lanes < 32 || lanes * 64 < bytes || tokens * lanes < few)) lanes *= 2;
   return lanes;
+}
+// Choices of a block that counts and places them: one a thread, more where all blocks' counts, which every block adds up, would be
+// over 16384.
+int64_t sort_chunk(int64_t n, int64_t experts) {
+  int64_t chunk = THREADS;
+  while ((n + chunk - 1) / chunk * experts > 16384) chunk *= 2;
+  return chunk;
 }
 int elem_size(int dtype) { return dtype == I8L_DTYPE_F32 ? 4 : 2; }
 
@@ -666,7 +697,7 @@ int launch_combine(const CombineArgs& a, bool backward, bool odd, cudaStream_t s
     else if (a.k <= 2) combine_backward_kernel<T, W, false, 2, 2><<<grid, THREADS, 0, st>>>(a);
     else combine_backward_kernel<T, W, false, 4, 2><<<grid, THREADS, 0, st>>>(a);
   } else {
-    if (odd) combine_kernel<T, W, true, 2, 2><<<grid, THREADS, 0, st>>>(a);
+    if (odd) combine_kernel<T, W, true, 4, 2><<<grid, THREADS, 0, st>>>(a);
     else if (one) combine_kernel<T, W, false, 4, 1><<<grid, THREADS, 0, st>>>(a);
     else if (a.k <= 2) combine_kernel<T, W, false, 2, 4><<<grid, THREADS, 0, st>>>(a);
     else combine_kernel<T, W, false, 4, 2><<<grid, THREADS, 0, st>>>(a);
@@ -680,7 +711,7 @@ int launch_combine(const CombineArgs& a, int wdtype, bool backward, bool odd, cu
 }
 int run_combine(CombineArgs a, int64_t cols, int dtype, int wdtype, bool backward, cudaStream_t st) {
   a.bytes = cols * elem_size(dtype);
-  a.lanes = lanes_for(a.bytes);
+  a.lanes = lanes_for(a.bytes, a.tokens);
   const bool odd = a.bytes % 16 || !aligned16(a.rows) || !aligned16(a.y) || !aligned16(a.dy) || !aligned16(a.drows);
   if (dtype == I8L_DTYPE_F32) return launch_combine<float, float>(a, backward, odd, st);
   if (dtype == I8L_DTYPE_F16) return launch_combine<__half>(a, wdtype, backward, odd, st);
@@ -694,7 +725,7 @@ using namespace i8l;
 
 extern "C" int64_t i8l_sort_workspace(int64_t tokens, int k, int experts) {
   if (tokens < 0 || k < 1 || experts < 1 || tokens * k <= SMALL_SORT) return 0;
-  const int64_t chunk = experts * 4 > 1024 ? experts * 4 : 1024;
+  const int64_t chunk = sort_chunk(tokens * k, experts);
   return (tokens * k + chunk - 1) / chunk * experts * (int64_t)sizeof(int32_t);
 }
 
@@ -721,7 +752,7 @@ extern "C" int i8l_sort_tokens(const void* x, const void* ids, int ids64, int64_
   a.hist = static_cast<int32_t*>(workspace);
   a.tokens = tokens; a.bytes = cols * size;
   a.n = (int)n; a.k = k; a.experts = experts; a.align = (int)align; a.n_rows = (int)rows; a.ids64 = ids64 ? 1 : 0;
-  a.lanes = lanes_for(a.bytes);
+  a.lanes = lanes_for(a.bytes, tokens);
   const unsigned copies = (unsigned)((tokens + THREADS / a.lanes - 1) / (THREADS / a.lanes));
   const unsigned grid = copies ? copies : 1;
   if (n <= SMALL_SORT) {
@@ -731,15 +762,17 @@ extern "C" int i8l_sort_tokens(const void* x, const void* ids, int ids64, int64_
     I8L_CUDA_OK(cudaGetLastError());
     return I8L_OK;
   }
-  a.chunk = experts * 4 > 1024 ? experts * 4 : 1024;
+  a.chunk = (int)sort_chunk(n, experts);
   a.blocks = (int)((n + a.chunk - 1) / a.chunk);
   const LaunchChain chain(st);
   (void)chain_first();
   I8L_CUDA_OK(launch(sort_count_kernel, dim3(a.blocks), THREADS, 0, st, a));
   I8L_CUDA_OK(launch(sort_place_kernel, dim3(a.blocks), THREADS, THREADS / 32 * experts * sizeof(int), st, a));
-  I8L_CUDA_OK(!odd        ? launch(sort_copy_kernel<uint32_t, false>, dim3(grid), THREADS, 0, st, a)
-              : size == 4 ? launch(sort_copy_kernel<uint32_t, true>, dim3(grid), THREADS, 0, st, a)
-                          : launch(sort_copy_kernel<uint16_t, true>, dim3(grid), THREADS, 0, st, a));
+  if (odd) a.lanes = lanes_for(a.bytes, rows);
+  const dim3 by_row((unsigned)((rows + THREADS / a.lanes - 1) / (THREADS / a.lanes)));
+  I8L_CUDA_OK(!odd        ? launch(sort_copy_kernel, dim3(grid), THREADS, 0, st, a)
+              : size == 4 ? launch(sort_copy_odd_kernel<uint32_t>, by_row, THREADS, 0, st, a)
+                          : launch(sort_copy_odd_kernel<uint16_t>, by_row, THREADS, 0, st, a));
   return I8L_OK;
 }
 

@@ -2,6 +2,7 @@
 // expert (i8l_token_linear).  Row scales and channel scales are those of the double_channel variant, so that the sum over K is
 // exact in int32 and an output needs one product by each scale.
 #include <atomic>
+#include <cstddef>
 
 #include "common.cuh"
 #include "ptx.cuh"
@@ -42,17 +43,16 @@ __device__ __forceinline__ uint4 load_weights(const int8_t* p) {   // read once:
 }
 
 // ------------------------------------------------------------------------------------------ few rows
-// One launch: a block takes 32 channels of one expert, quantizes up to MT of its rows into shared memory and multiplies them with the
-// channels' weights by dp4a, a warp four channels at a time, so that a piece of x read from shared memory serves four loads of
-// weights.  Bound by the weights' bytes.
-constexpr int FEW_THREADS = 256, FEW_WARP_COLS = 4, FEW_COLS = FEW_THREADS / 32 * FEW_WARP_COLS;
+// Up to eight rows: a warp multiplies two channels' weights with the rows of their expert by dp4a, 512 bytes of K a step.  Bound by
+// the weights' bytes, so it is the loads that matter: a warp has eight of 16 bytes a lane in flight ahead of those it works on, and
+// the first go out before the rows have been quantized (the weights and offsets were there before the chain).  The rows then come
+// to shared memory; a piece of them read there serves two loads of weights.
+constexpr int FEW_THREADS = 256, FEW_WARP_COLS = 2, FEW_COLS = FEW_THREADS / 32 * FEW_WARP_COLS, FEW_STEPS = 4, FEW_BATCH = FEW_STEPS * 512;
 
 template <int MT>
-__global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const TokenArgs a) {
-  extern __shared__ __align__(16) int8_t xq[];   // [MT, K]
-  __shared__ float xs[MT], red[FEW_THREADS / 32];
+__global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const TokenArgs a, const int8_t* xq, const float* xs) {
+  extern __shared__ __align__(16) int8_t rows[];   // [MT, K]
   __shared__ int s_expert;
-  constexpr int LANES = FEW_THREADS / MT;        // threads that quantize a row
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int K = (int)a.K;
   int64_t begin, end;
@@ -76,6 +76,18 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const TokenArgs a
     e = s_expert;
   }
   const int64_t n0 = (int64_t)blockIdx.x * FEW_COLS + warp * FEW_WARP_COLS;
+  const int8_t* w = a.wq + ((int64_t)(e < 0 ? 0 : e) * a.N + n0) * a.K + lane * 16;
+  const bool live = e >= 0 && n0 < a.N;   // N is a multiple of 8: both channels or none
+  uint4 now[FEW_WARP_COLS][FEW_STEPS], next[FEW_WARP_COLS][FEW_STEPS];
+  auto load = [&](uint4 (&to)[FEW_WARP_COLS][FEW_STEPS], int k0) {
+#pragma unroll
+    for (int s = 0; s < FEW_STEPS; ++s)
+#pragma unroll
+      for (int j = 0; j < FEW_WARP_COLS; ++j)
+        if (live && k0 + s * 512 + lane * 16 < K) to[j][s] = load_weights(w + (int64_t)j * K + k0 + s * 512);
+  };
+  load(now, 0);
+  chain_wait();
   if (a.offsets && blockIdx.y == 0) {   // rows of no expert
     int64_t b, n, last_b, last_n;
     segment(a, 0, b, n);
@@ -92,75 +104,55 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const TokenArgs a
   }
   if (e < 0) return;
   segment(a, e, begin, end);
-  const int8_t* w = a.wq + ((int64_t)e * a.N + n0) * a.K;
-  for (int64_t r0 = begin; r0 < end; r0 += MT) {
-    // the rows in int8, a scale each
-    {
-      const int t = tid / LANES, l = tid & (LANES - 1);
-      const bool live = r0 + t < end;
-      const uint4* row = reinterpret_cast<const uint4*>(a.x + (r0 + t) * a.K);
-      float m = 0.f;
-      if (live)
-        for (int c = l; c < K / 8; c += LANES) {
-          float v[8];
-          unpack8(row[c], v);
+  const int count = (int)(end - begin);
+  for (int i = tid; i < MT * K / 16; i += FEW_THREADS)
+    reinterpret_cast<uint4*>(rows)[i] = i < count * K / 16 ? reinterpret_cast<const uint4*>(xq + begin * K)[i] : make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  if (!live) return;
+  int acc[FEW_WARP_COLS][MT];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[i]));
-        }
+  for (int j = 0; j < FEW_WARP_COLS; ++j)
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      __syncthreads();   // also: the rows in front of these have been multiplied
-      if (lane == 0) red[warp] = m;
-      __syncthreads();
-      m = red[t * (LANES / 32)];
+    for (int t = 0; t < MT; ++t) acc[j][t] = 0;
+  auto multiply = [&](const uint4 (&u)[FEW_WARP_COLS][FEW_STEPS], int k0) {
 #pragma unroll
-      for (int i = 1; i < LANES / 32; ++i) m = fmaxf(m, red[t * (LANES / 32) + i]);
-      float s, stored;
-      make_scale<I8L_QMODE_ROWRCP>(m, s, stored);
-      if (l == 0) xs[t] = stored;
-      uint2* q = reinterpret_cast<uint2*>(xq + (int64_t)t * K);
-      for (int c = l; c < K / 8; c += LANES) q[c] = live ? quant_piece<I8L_QMODE_ROWRCP>(row[c], s) : make_uint2(0, 0);
-      __syncthreads();
-    }
-    if (n0 >= a.N) continue;
-    int acc[FEW_WARP_COLS][MT];
-#pragma unroll
-    for (int j = 0; j < FEW_WARP_COLS; ++j)
-#pragma unroll
-      for (int t = 0; t < MT; ++t) acc[j][t] = 0;
-#pragma unroll 2
-    for (int k = lane * 16; k < K; k += 512) {
-      uint4 u[FEW_WARP_COLS];
-#pragma unroll
-      for (int j = 0; j < FEW_WARP_COLS; ++j) u[j] = load_weights(w + (int64_t)j * K + k);
+    for (int s = 0; s < FEW_STEPS; ++s) {
+      const int k = k0 + s * 512 + lane * 16;
+      if (k >= K) break;
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
-        const uint4 v = *reinterpret_cast<const uint4*>(xq + (int64_t)t * K + k);
+        const uint4 v = *reinterpret_cast<const uint4*>(rows + t * K + k);
 #pragma unroll
         for (int j = 0; j < FEW_WARP_COLS; ++j) {
-          acc[j][t] = __dp4a((int)u[j].x, (int)v.x, acc[j][t]);
-          acc[j][t] = __dp4a((int)u[j].y, (int)v.y, acc[j][t]);
-          acc[j][t] = __dp4a((int)u[j].z, (int)v.z, acc[j][t]);
-          acc[j][t] = __dp4a((int)u[j].w, (int)v.w, acc[j][t]);
+          acc[j][t] = __dp4a((int)u[j][s].x, (int)v.x, acc[j][t]);
+          acc[j][t] = __dp4a((int)u[j][s].y, (int)v.y, acc[j][t]);
+          acc[j][t] = __dp4a((int)u[j][s].z, (int)v.z, acc[j][t]);
+          acc[j][t] = __dp4a((int)u[j][s].w, (int)v.w, acc[j][t]);
         }
       }
     }
-    int mine = 0;   // lane j * MT + t has the sum of channel j and row t
+  };
+  for (int k0 = 0; k0 < K; k0 += 2 * FEW_BATCH) {
+    load(next, k0 + FEW_BATCH);
+    multiply(now, k0);
+    load(now, k0 + 2 * FEW_BATCH);
+    multiply(next, k0 + FEW_BATCH);
+  }
+  int mine = 0;   // lane j * MT + t has the sum of channel j and row t
 #pragma unroll
-    for (int j = 0; j < FEW_WARP_COLS; ++j)
+  for (int j = 0; j < FEW_WARP_COLS; ++j)
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        const int sum = __reduce_add_sync(0xffffffffu, acc[j][t]);
-        if (lane == j * MT + t) mine = sum;
-      }
-    const int j = lane / MT, t = lane % MT;
-    if (j < FEW_WARP_COLS && r0 + t < end) {
-      const int64_t n = n0 + j, c = (int64_t)e * a.N + n, at = (r0 + t) * a.N + n;
-      float v = __fmul_rn(__fmul_rn(__int2float_rn(mine), xs[t]), a.ws[c]);
-      if (a.bias) v = __fadd_rn(v, __bfloat162float(a.bias[c]));
-      if (a.out_f32) static_cast<float*>(a.y)[at] = v;
-      else static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(v);
+    for (int t = 0; t < MT; ++t) {
+      const int sum = __reduce_add_sync(0xffffffffu, acc[j][t]);
+      if (lane == j * MT + t) mine = sum;
     }
+  const int j = lane / MT, t = lane % MT;
+  if (j < FEW_WARP_COLS && t < count) {
+    const int64_t n = n0 + j, c = (int64_t)e * a.N + n, at = (begin + t) * a.N + n;
+    float v = __fmul_rn(__fmul_rn(__int2float_rn(mine), xs[begin + t]), a.ws[c]);
+    if (a.bias) v = __fadd_rn(v, __bfloat162float(a.bias[c]));
+    if (a.out_f32) static_cast<float*>(a.y)[at] = v;
+    else static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(v);
   }
 }
 
@@ -176,16 +168,21 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const TokenArgs a
 // All waits are bounded, as in gemm.cu: on expiry every role leaves, the status word says so.
 constexpr int GRP_THREADS = 384, GRP_EPI_WARPS = 8, CHANNELS = 128, KBYTES = 128;
 constexpr int A_BYTES = CHANNELS * KBYTES;
-constexpr int BIG_BOX = 64, SMALL_BOX = 16;   // tokens of a TMA box
+constexpr int BOXES = 5;   // maps of 16, 32, 64, 128 and 256 tokens
 constexpr int EPI_BYTES = 32 * 32 * 2;        // 32 tokens x 32 channels in bf16
 constexpr int RASTER = 16;                    // token tiles whose rows should stay in L2 while the channels are gone through
 
+struct __align__(16) Segment {
+  int row, rows;   // of an expert
+  int share;       // tokens of each of its tiles
+  int first;       // number of its first tile
+};
 template <int TOK> struct Grp {
-  static constexpr int STAGES = TOK == 256 ? 4 : 8, BUFS = 512 / TOK < 4 ? 512 / TOK : 4, COLUMNS = BUFS * TOK;
+  static constexpr int STAGES = TOK == 256 ? 4 : TOK == 128 ? 6 : 8, BUFS = 512 / TOK < 4 ? 512 / TOK : 4, COLUMNS = BUFS * TOK;
   static constexpr int B_BYTES = TOK * KBYTES;
   static constexpr int RING = STAGES * (A_BYTES + B_BYTES);
-  static constexpr int TABLE = RING + GRP_EPI_WARPS * EPI_BYTES;   // then experts x (first row, rows), experts + 1 tile counts
-  static int smem(int experts) { return TABLE + experts * 12 + 4 + 1024; }
+  static constexpr int TABLE = RING + GRP_EPI_WARPS * EPI_BYTES;   // then experts + 1 segments
+  static int smem(int experts) { return TABLE + (experts + 1) * (int)sizeof(Segment) + 1024; }
 };
 
 struct GroupArgs {
@@ -198,7 +195,12 @@ struct GroupArgs {
 struct __align__(16) GroupCtl {
   uint64_t full[8], empty[8], tfull[4], tempty[4], done;
   int abort_flag;
-  uint32_t tmem_base;
+  uint32_t tmem_base, by[RASTER + 1];
+  __align__(16) float scale[GRP_EPI_WARPS][32];   // of the tokens that a warp takes out, read four at a time
+};
+static_assert(offsetof(GroupCtl, scale) % 16 == 0, "vector reads");
+struct TokenMaps {
+  CUtensorMap box[BOXES];   // of 16 << i tokens
 };
 struct Tile {
   int expert, channel;
@@ -209,45 +211,58 @@ struct Tile {
 // Instruction descriptor of kind::i8: D s32, A and B s8, K-major, M = 128.
 __device__ __forceinline__ uint32_t mma_desc(int n) { return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(CHANNELS >> 4) << 24); }
 
+// The tokens of a tile come in one or two boxes: one of the next power of two where that is at most a quarter more, else the power of
+// two below and one for the rest.
+struct Boxes {
+  int first, second;   // numbers of maps, second < 0: none
+  __device__ __forceinline__ int tokens() const { return (16 << first) + (second < 0 ? 0 : 16 << second); }
+};
+__device__ __forceinline__ Boxes boxes_of(int columns) {
+  const int up = columns <= 16 ? 0 : 32 - __clz((columns - 1) >> 4);   // 16 << up >= columns
+  if ((16 << up) * 4 <= columns * 5) return Boxes{up, -1};
+  const int rest = columns - (16 << (up - 1));
+  return Boxes{up - 1, rest <= 16 ? 0 : 32 - __clz((rest - 1) >> 4)};
+}
+
+// Divisions by numbers that are not known at compile time cost a tile some 500 cycles, which every role goes through: the quotient
+// that the rows of a segment need is in the table, more than one group of token tiles makes a tile long enough, and the last one is a
+// multiplication.  by[w]: 2^32 / w rounded up, exact for numbers below 2^28 (16 * channels / 128) and w up to 16.
 template <int TOK>
-__device__ __forceinline__ Tile tile_of(int t, int experts, int n_tiles, const int2* seg, const int* first) {
-  int lo = 0, hi = experts;   // first[lo] <= t < first[hi]; experts without rows have no tiles and are stepped over
+__device__ __forceinline__ Tile tile_of(int t, const GroupArgs& p, const Segment* seg, const uint32_t* by) {
+  int lo = 0, hi = p.t.experts;   // seg[lo].first <= t < seg[hi].first; experts without rows have no tiles and are stepped over
   while (hi - lo > 1) {
     const int mid = (lo + hi) / 2;
-    if (first[mid] <= t) lo = mid;
+    if (seg[mid].first <= t) lo = mid;
     else hi = mid;
   }
-  const int rows = seg[lo].y, tiles = (rows + TOK - 1) / TOK;
-  const int share = ((rows + tiles - 1) / tiles + 15) & ~15;   // tokens of a tile: equal ones rather than full ones and a rest
-  const int local = t - first[lo], group = local / (RASTER * n_tiles), g0 = group * RASTER;
-  const int width = tiles - g0 < RASTER ? tiles - g0 : RASTER, at = local - group * RASTER * n_tiles;
-  const int n = at / width, m = g0 + at - n * width;
+  const Segment s = seg[lo];
+  const int tiles = (s.rows + TOK - 1) / TOK, local = t - s.first, per_group = RASTER * p.n_tiles;
+  const int group = tiles <= RASTER ? 0 : local / per_group, g0 = group * RASTER;
+  const int width = tiles - g0 < RASTER ? tiles - g0 : RASTER, at = local - group * per_group;
+  const int n = width == 1 ? at : (int)__umulhi((uint32_t)at, by[width]), m = g0 + at - n * width;
   Tile r;
   r.expert = lo;
   r.channel = n * CHANNELS;
-  r.row = seg[lo].x + (int64_t)m * share;
-  r.rows = rows - m * share < share ? rows - m * share : share;
+  r.row = s.row + (int64_t)m * s.share;
+  r.rows = s.rows - m * s.share < s.share ? s.rows - m * s.share : s.share;
   r.columns = (r.rows + 15) & ~15;
   return r;
 }
 
 template <int TOK>
 __global__ void __launch_bounds__(GRP_THREADS, 1)
-group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_big, const __grid_constant__ CUtensorMap map_small,
-             const GroupArgs p) {
+group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ TokenMaps map_x, const GroupArgs p) {
   using G = Grp<TOK>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ GroupCtl ctl;
   uint8_t* const smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   const uint32_t smem_a = smem_u32(smem), smem_b = smem_a + G::STAGES * A_BYTES;
-  int2* const seg = reinterpret_cast<int2*>(smem + G::TABLE);
-  int* const first = reinterpret_cast<int*>(seg + p.t.experts);
+  Segment* const seg = reinterpret_cast<Segment*>(smem + G::TABLE);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = &ctl.abort_flag;
   if (threadIdx.x == 0) {
     prefetch_tensormap(&map_w);
-    prefetch_tensormap(&map_big);
-    prefetch_tensormap(&map_small);
+    for (int i = 0; i < BOXES; ++i) prefetch_tensormap(&map_x.box[i]);
     for (int s = 0; s < G::STAGES; ++s) {
       mbar_init(smem_u32(&ctl.full[s]), 1);
       mbar_init(smem_u32(&ctl.empty[s]), 1);
@@ -265,55 +280,76 @@ group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem_base)), "r"(G::COLUMNS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  chain_wait();   // offsets, the quantized rows and whatever still uses the output's memory
+  // The offsets and the weights were there before the chain; only who reads the quantized rows and their scales waits for them.
   for (int e = threadIdx.x; e < p.t.experts; e += GRP_THREADS) {
     int64_t b, n;
     segment(p.t, e, b, n);
-    seg[e] = make_int2((int)b, (int)(n - b));
-    first[e + 1] = (int)(n - b + TOK - 1) / TOK * p.n_tiles;
+    const int count = (int)(n - b), tiles = (count + TOK - 1) / TOK;
+    seg[e].row = (int)b;
+    seg[e].rows = count;
+    seg[e].share = tiles ? ((count + tiles - 1) / tiles + 15) & ~15 : 0;   // equal tiles rather than full ones and a rest
+    seg[e + 1].first = tiles * p.n_tiles;
   }
+  if (threadIdx.x >= 2 && threadIdx.x <= RASTER) ctl.by[threadIdx.x] = 0xffffffffu / threadIdx.x + 1;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   if (warp == 0) {   // running sum of the tiles
     int carry = 0;
-    if (lane == 0) first[0] = 0;
+    if (lane == 0) seg[0].first = 0;
     for (int e0 = 0; e0 < p.t.experts; e0 += 32) {
-      int up = e0 + lane < p.t.experts ? first[e0 + lane + 1] : 0;
+      int up = e0 + lane < p.t.experts ? seg[e0 + lane + 1].first : 0;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, up, d);
         if (lane >= d) up += v;
       }
-      if (e0 + lane < p.t.experts) first[e0 + lane + 1] = carry + up;
+      if (e0 + lane < p.t.experts) seg[e0 + lane + 1].first = carry + up;
       carry += __shfl_sync(0xffffffffu, up, 31);
     }
   }
   __syncthreads();
   const uint32_t tmem_base = ctl.tmem_base;
-  const int total = first[p.t.experts], KB = (int)((p.t.K + KBYTES - 1) / KBYTES);
+  const int total = seg[p.t.experts].first, KB = (int)((p.t.K + KBYTES - 1) / KBYTES);
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
+    const bool elected = elect_one();
     int s = 0;
     uint32_t ph = 0, issued = 0, issued_ph = 0;   // bit s: a load into stage s is (or was) in flight, with parity
     bool ok = true;
+    int ahead = 0;   // K blocks of the first tile whose weights are on their way before the rows have been quantized
+    if ((int)blockIdx.x < total && !p.withhold) {
+      const Tile tile = tile_of<TOK>(blockIdx.x, p, seg, ctl.by);
+      ahead = KB < G::STAGES ? KB : G::STAGES;
+      const uint32_t bytes = A_BYTES + boxes_of(tile.columns).tokens() * KBYTES;
+      if (elected)
+        for (int kb = 0; kb < ahead; ++kb) {
+          mbar_expect_tx(smem_u32(&ctl.full[kb]), bytes);
+          tma_load_2d(smem_a + kb * A_BYTES, &map_w, smem_u32(&ctl.full[kb]), kb * KBYTES, (int)((int64_t)tile.expert * p.t.N) + tile.channel);
+        }
+    }
+    chain_wait();
     for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-      const Tile tile = tile_of<TOK>(t, p.t.experts, p.n_tiles, seg, first);
+      const Tile tile = tile_of<TOK>(t, p, seg, ctl.by);
       const int w_row = (int)((int64_t)tile.expert * p.t.N) + tile.channel;
+      const Boxes box = boxes_of(tile.columns);
+      const uint32_t bytes = A_BYTES + box.tokens() * KBYTES;
       for (int kb = 0; kb < KB; ++kb) {
         if (!(ok = mbar_wait(smem_u32(&ctl.empty[s]), ph ^ 1u, abort_flag, p.max_polls))) break;
         if (p.withhold && t == (int)blockIdx.x && kb == KB - 1) {   // test hook: the waits that depend on this stage run out
           if (++s == G::STAGES) { s = 0; ph ^= 1u; }
           continue;
         }
-        if (lane == 0) {
+        if (elected) {
           const uint32_t bar = smem_u32(&ctl.full[s]);
-          mbar_expect_tx(bar, A_BYTES + tile.columns * KBYTES);
-          tma_load_2d(smem_a + s * A_BYTES, &map_w, bar, kb * KBYTES, w_row);
-          int c = 0;
-          for (; tile.columns - c >= BIG_BOX; c += BIG_BOX) tma_load_2d(smem_b + s * G::B_BYTES + c * KBYTES, &map_big, bar, kb * KBYTES, (int)tile.row + c);
-          for (; c < tile.columns; c += SMALL_BOX) tma_load_2d(smem_b + s * G::B_BYTES + c * KBYTES, &map_small, bar, kb * KBYTES, (int)tile.row + c);
+          if (t != (int)blockIdx.x || kb >= ahead) {
+            mbar_expect_tx(bar, bytes);
+            tma_load_2d(smem_a + s * A_BYTES, &map_w, bar, kb * KBYTES, w_row);
+          }
+          const uint32_t to = smem_b + s * G::B_BYTES;
+          tma_load_2d(to, &map_x.box[box.first], bar, kb * KBYTES, (int)tile.row);
+          if (box.second >= 0) tma_load_2d(to + (16 << box.first) * KBYTES, &map_x.box[box.second], bar, kb * KBYTES, (int)tile.row + (16 << box.first));
         }
         issued |= 1u << s;
         issued_ph = (issued_ph & ~(1u << s)) | (ph << s);
@@ -334,7 +370,7 @@ group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     uint32_t ph = 0, aph = 0;
     bool ok = true;
     for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-      const uint32_t idesc = mma_desc(tile_of<TOK>(t, p.t.experts, p.n_tiles, seg, first).columns), d = tmem_base + ab * TOK;
+      const uint32_t idesc = mma_desc(tile_of<TOK>(t, p, seg, ctl.by).columns), d = tmem_base + ab * TOK;
       if (!(ok = mbar_wait(smem_u32(&ctl.tempty[ab]), aph ^ 1u, abort_flag, p.max_polls))) break;
       for (int kb = 0; kb < KB; ++kb) {
         if (!(ok = mbar_wait(smem_u32(&ctl.full[s]), ph, abort_flag, p.max_polls))) break;
@@ -357,7 +393,7 @@ group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     mbar_wait(smem_u32(&ctl.done), 0, &dummy);
   } else if (warp < 4) {
     // ------------------------------------------------------------------ rows of no expert
-    const int64_t before = seg[0].x, behind = (int64_t)seg[p.t.experts - 1].x + seg[p.t.experts - 1].y, dead = before + p.t.rows - behind;
+    const int64_t before = seg[0].row, behind = (int64_t)seg[p.t.experts - 1].row + seg[p.t.experts - 1].rows, dead = before + p.t.rows - behind;
     const int64_t pieces = p.t.N * (p.t.out_f32 ? 4 : 2) / 16;
     for (int64_t i = (int64_t)blockIdx.x * 64 + threadIdx.x - 64; i < dead * pieces; i += (int64_t)gridDim.x * 64) {
       const int64_t r = i / pieces;
@@ -367,47 +403,88 @@ group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     // ------------------------------------------------------------------ epilogue
     const int q = warp & 3, half = (warp - 4) >> 2;   // a quarter of the channels, every other 32 tokens
     uint8_t* const turn = smem + G::RING + (warp - 4) * EPI_BYTES;
+    float* const scale = ctl.scale[warp - 4];
+    constexpr int PARTS = TOK / 64;   // of 32 tokens
+    // What a tile needs besides the accumulator: fetched a tile ahead, behind the wait for the one in front.
+    struct Ahead {
+      Tile tile;
+      float sw, bias, token[PARTS];   // scale and bias of the lane's channel, scales of the lane's tokens
+    };
+    auto fetch = [&](int t) {
+      Ahead f;
+      f.tile = tile_of<TOK>(t, p, seg, ctl.by);
+      const int n = f.tile.channel + q * 32 + lane;
+      const int64_t c = (int64_t)f.tile.expert * p.t.N + n;
+      f.sw = n < p.t.N ? p.t.ws[c] : 0.f;
+      f.bias = n < p.t.N && p.t.bias ? __bfloat162float(p.t.bias[c]) : 0.f;
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i) {
+        const int j = half * 32 + i * 64 + lane;
+        f.token[i] = j < f.tile.rows ? p.xs[f.tile.row + j] : 0.f;
+      }
+      return f;
+    };
     int ab = 0;
     uint32_t aph = 0;
+    chain_wait();
+    Ahead next;
+    if ((int)blockIdx.x < total) next = fetch(blockIdx.x);
     for (int t = blockIdx.x; t < total; t += gridDim.x) {
-      const Tile tile = tile_of<TOK>(t, p.t.experts, p.n_tiles, seg, first);
-      const int n = tile.channel + q * 32 + lane;
-      const bool live = n < p.t.N;
-      const int64_t c = (int64_t)tile.expert * p.t.N + n;
-      const float sw = live ? p.t.ws[c] : 0.f, bias = live && p.t.bias ? __bfloat162float(p.t.bias[c]) : 0.f;
+      const Ahead now = next;
       if (!mbar_wait(smem_u32(&ctl.tfull[ab]), aph, abort_flag, p.max_polls)) break;
       tc_fence_after();
+      if (t + (int)gridDim.x < total) next = fetch(t + gridDim.x);
       const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + ab * TOK;
-      for (int j0 = half * 32; j0 < tile.rows; j0 += 64) {
-        const int left = tile.rows - j0;
-        const float mine = lane < left ? p.xs[tile.row + j0 + lane] : 0.f;
+      const int n = now.tile.channel + q * 32 + lane;
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i) {
+        const int j0 = half * 32 + i * 64, left = now.tile.rows - j0;
+        if (left <= 0) break;
         uint32_t r[32];
         tc_ld16(taddr + j0, r);
         tc_ld16(taddr + j0 + 16, r + 16);
+        scale[lane] = now.token[i];
+        __syncwarp();
         tc_ld_wait();
         float v[32];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          v[j] = __fmul_rn(__fmul_rn(__int2float_rn((int)r[j]), __shfl_sync(0xffffffffu, mine, j)), sw);
-          if (p.t.bias) v[j] = __fadd_rn(v[j], bias);
+        for (int j = 0; j < 32; j += 4) {
+          const float4 sx = *reinterpret_cast<const float4*>(scale + j);
+          v[j] = __fmul_rn(__fmul_rn(__int2float_rn((int)r[j]), sx.x), now.sw);
+          v[j + 1] = __fmul_rn(__fmul_rn(__int2float_rn((int)r[j + 1]), sx.y), now.sw);
+          v[j + 2] = __fmul_rn(__fmul_rn(__int2float_rn((int)r[j + 2]), sx.z), now.sw);
+          v[j + 3] = __fmul_rn(__fmul_rn(__int2float_rn((int)r[j + 3]), sx.w), now.sw);
         }
-        const int64_t row = tile.row + j0;
+        if (p.t.bias) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __fadd_rn(v[j], now.bias);
+        }
+        const int64_t row = now.tile.row + j0;
         if (p.t.out_f32) {
           float* y = static_cast<float*>(p.t.y) + row * p.t.N + n;
+          if (n < p.t.N) {
+            if (left >= 32) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (live && j < left) y[j * p.t.N] = v[j];
+              for (int j = 0; j < 32; ++j) y[j * p.t.N] = v[j];
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (j < left) y[j * p.t.N] = v[j];
+            }
+          }
+          __syncwarp();   // the scales have been read
         } else {
           __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(turn) + lane;
 #pragma unroll
           for (int j = 0; j < 32; ++j) to[j * 32] = __float2bfloat16_rn(v[j]);
           __syncwarp();
-          const int piece = lane & 3, n8 = tile.channel + q * 32 + piece * 8;
+          const int piece = lane & 3, n8 = now.tile.channel + q * 32 + piece * 8;
+          __nv_bfloat16* y = static_cast<__nv_bfloat16*>(p.t.y) + (row + (lane >> 2)) * p.t.N + n8;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int j = i * 8 + (lane >> 2);
+          for (int i8 = 0; i8 < 4; ++i8) {
+            const int j = i8 * 8 + (lane >> 2);
             if (j < left && n8 < p.t.N)
-              *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.t.y) + (row + j) * p.t.N + n8) = *reinterpret_cast<const uint4*>(turn + j * 64 + piece * 16);
+              *reinterpret_cast<uint4*>(y + i8 * 8 * p.t.N) = *reinterpret_cast<const uint4*>(turn + j * 64 + piece * 16);
           }
           __syncwarp();
         }
@@ -440,13 +517,41 @@ int few_rows(int64_t rows, int64_t K) {
   const int mt = rows == 1 ? 1 : rows == 2 ? 2 : rows <= 4 ? 4 : 8;
   return rows <= 8 && mt * K <= FEW_SMEM ? mt : 0;
 }
-template <int MT> int launch_few(const TokenArgs& a, cudaStream_t st) {
+template <int MT> int launch_few(const TokenArgs& a, const int8_t* xq, const float* xs, cudaStream_t st) {
   static std::atomic<int> allowed[MAX_SMEM_DEVICES];
   I8L_CUDA_OK(allow_smem(few_rows_kernel<MT>, allowed, FEW_SMEM));
   const int64_t segments = a.offsets ? (a.experts < a.rows ? a.experts : a.rows) : 1;
-  few_rows_kernel<MT><<<dim3((unsigned)((a.N + FEW_COLS - 1) / FEW_COLS), (unsigned)segments), FEW_THREADS, MT * a.K, st>>>(a);
-  I8L_CUDA_OK(cudaGetLastError());
+  I8L_CUDA_OK(launch(few_rows_kernel<MT>, dim3((unsigned)((a.N + FEW_COLS - 1) / FEW_COLS), (unsigned)segments), FEW_THREADS, (size_t)(MT * a.K), st,
+                     a, xq, xs));
   return I8L_OK;
+}
+
+// Tokens of a tile, from what the host knows: as if all rows belonged to experts, and to all alike.  A tile of s columns takes 0.4 + 0.6 *
+// s / 256 of a full one (less for the MMAs, as much for the weights and the rest), and up to three waves of tiles end with the
+// slowest.  us with 64, 128 and 256: dense 4096x4096 of 256 rows 12.6 / 13.3 / 16.0, 512 20.1 / 14.6 / 16.9, 1000 35 / 23 / 18.8;
+// 64 experts of 1408x4096 with 32 rows each 69 / 67 / 72, 100 102 / 87 / 91, 500 350 / 269 / 223.  Over 100 sizes the choice costs
+// 0.7 % against the best one, 9 % at most.
+int tile_tokens(const TokenArgs& a) {
+  const int64_t segments = a.experts < a.rows ? a.experts : a.rows, average = (a.rows + segments - 1) / segments;
+  const int64_t n_tiles = (a.N + CHANNELS - 1) / CHANNELS;
+  const int sms = gemm_cta_budget();
+  int best = 0;
+  double least = 0;
+  for (int t = 64; t <= 256; t *= 2) {
+    double per = 1;   // tiles of a segment; uneven ones need half a tile more than their average
+    if (segments == 1) per = (double)((average + t - 1) / t);
+    else if (average * 4 > t * 3) per = (double)average / t + 0.5;
+    if (per < 1) per = 1;
+    int64_t share = ((average + (int64_t)per - 1) / (int64_t)per + 15) / 16 * 16;
+    if (share > t) share = t;
+    const double tiles = (double)segments * per * (double)n_tiles, waves = tiles / sms;
+    const double cost = (waves < 3 ? (double)(((int64_t)tiles + sms - 1) / sms) : waves + 0.5) * (0.4 + 0.6 * (double)share / 256);
+    if (!best || cost < least) {
+      best = t;
+      least = cost;
+    }
+  }
+  return best;
 }
 
 template <int TOK> int launch_group(const int8_t* xq, GroupArgs& p, cudaStream_t st) {
@@ -457,10 +562,11 @@ template <int TOK> int launch_group(const int8_t* xq, GroupArgs& p, cudaStream_t
   p.n_tiles = (int)((a.N + CHANNELS - 1) / CHANNELS);
   const int64_t most = (a.rows / TOK + (a.experts < a.rows ? a.experts : a.rows)) * p.n_tiles;   // tiles, whatever the offsets
   if (most >= (1ll << 31)) return fail(I8L_ERR_SHAPE, "i8l_token_linear: too large for 32-bit tile numbers");
-  CUtensorMap mw, mb, ms;
+  CUtensorMap mw;
+  TokenMaps mx;
   if (int e = make_tile_map_i8(&mw, a.wq, a.experts * a.N, a.K, CHANNELS)) return e;
-  if (int e = make_tile_map_i8(&mb, xq, a.rows, a.K, BIG_BOX)) return e;
-  if (int e = make_tile_map_i8(&ms, xq, a.rows, a.K, SMALL_BOX)) return e;
+  for (int i = 0; i < BOXES; ++i)
+    if (int e = make_tile_map_i8(&mx.box[i], xq, a.rows, a.K, 16 << i)) return e;
   const int budget = gemm_cta_budget();
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attrs[1];
@@ -469,7 +575,7 @@ template <int TOK> int launch_group(const int8_t* xq, GroupArgs& p, cudaStream_t
   cfg.dynamicSmemBytes = G::smem(a.experts);
   cfg.stream = st;
   chain_attribute(cfg, attrs);
-  I8L_CUDA_OK(cudaLaunchKernelEx(&cfg, group_kernel<TOK>, mw, mb, ms, p));
+  I8L_CUDA_OK(cudaLaunchKernelEx(&cfg, group_kernel<TOK>, mw, mx, p));
   return I8L_OK;
 }
 
@@ -479,7 +585,7 @@ template <int TOK> int launch_group(const int8_t* xq, GroupArgs& p, cudaStream_t
 using namespace i8l;
 
 extern "C" int64_t i8l_token_linear_workspace(int64_t rows, int64_t K) {
-  if (rows <= 0 || K <= 0 || rows >= (1ll << 31) || K > MAX_K || few_rows(rows, K)) return 0;
+  if (rows <= 0 || K <= 0 || rows >= (1ll << 31) || K > MAX_K) return 0;
   return (rows * K + 255) / 256 * 256 + (4 * rows + 255) / 256 * 256;
 }
 
@@ -505,24 +611,25 @@ extern "C" int i8l_token_linear(const void* x, const int8_t* w_q, const float* w
   a.bias = static_cast<const __nv_bfloat16*>(bias); a.y = y;
   a.rows = rows; a.N = N; a.K = K; a.experts = experts; a.out_f32 = (flags & I8L_GEMM_OUT_F32) ? 1 : 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int8_t* xq = static_cast<int8_t*>(workspace);
+  float* xs = reinterpret_cast<float*>(xq + (rows * K + 255) / 256 * 256);
+  const LaunchChain chain(st);
+  if (int e = quant_token_rows(x, rows, K, xq, xs, st)) return e;
+  (void)chain_first();
   switch (few_rows(rows, K)) {
-    case 1: return launch_few<1>(a, st);
-    case 2: return launch_few<2>(a, st);
-    case 4: return launch_few<4>(a, st);
-    case 8: return launch_few<8>(a, st);
+    case 1: return launch_few<1>(a, xq, xs, st);
+    case 2: return launch_few<2>(a, xq, xs, st);
+    case 4: return launch_few<4>(a, xq, xs, st);
+    case 8: return launch_few<8>(a, xq, xs, st);
   }
   GroupArgs p{};
   p.t = a;
-  int8_t* xq = static_cast<int8_t*>(workspace);
-  float* xs = reinterpret_cast<float*>(xq + (rows * K + 255) / 256 * 256);
   p.xs = xs;
   p.status = status;
   p.mirror = status ? mirror_of(status) : nullptr;
   p.max_polls = gemm_wait_limit();
   p.withhold = gemm_withhold();
-  const LaunchChain chain(st);
-  if (int e = quant_token_rows(x, rows, K, xq, xs, st)) return e;
-  (void)chain_first();
-  // Tiles of 256 tokens read the weights least often; with few rows an expert they only take ring space from the weights.
-  return rows / experts > 64 ? launch_group<256>(xq, p, st) : launch_group<64>(xq, p, st);
+  const int tok = tile_tokens(a);
+  if (tok == 128) return launch_group<128>(xq, p, st);
+  return tok == 256 ? launch_group<256>(xq, p, st) : launch_group<64>(xq, p, st);
 }
