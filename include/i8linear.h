@@ -333,7 +333,7 @@ I8L_API int i8l_test_set_wait_limit(uint32_t max_polls, int withhold_one_load);
  *   pos     int32 [tokens, k]: the row of a choice, -1 if dropped
  *   src     int32 [rows]: the choice of a row, -1 if it has none
  * rows >= tokens * k + min(experts, tokens * k) * (align - 1), rounded up to `align`.  The result depends on the inputs only (a
- * stable counting sort, no atomics on places).  experts <= 1024, k <= 64, tokens * k <= 2^30, align <= 65536, any cols.
+ * stable counting sort, no atomics on places).  experts <= 1024, k <= 64, tokens * k <= 2^30, align <= 65536, cols from 1 to 2^28.
  * Pointers are aligned to their elements.  workspace: i8l_sort_workspace bytes, 4-byte aligned, may be NULL where that is 0.
  * No counterpart in the reference, which has no expert layers.
  */

@@ -40,43 +40,76 @@ template <typename T> __device__ __forceinline__ uint4 pack(const float* v) {
   return p;
 }
 
-// Rows that are no multiple of 16 bytes, or do not start on one, still move 16 bytes at a time: stores go to the aligned pieces of the
-// row that is written, and what belongs there is put together from the two aligned pieces that it lies across in the row that is
-// read.  Element by element a row of 1405 fp16 took 2 bytes an access: sort of 4099 tokens 41 us, its gradient 38.
-// Only pieces that the row itself has bytes in are read (memory comes in whole ones); of a piece at the row's ends the
-// elements that belong to the row are written.
-// Aligned piece q of a row written at `to` begins at this byte of the row, negative for the first one of a row that starts inside it.
-__device__ __forceinline__ int64_t piece_begin(const void* to, int64_t q) { return 16 * q - (int64_t)(reinterpret_cast<uintptr_t>(to) & 15); }
-__device__ __forceinline__ int64_t pieces_of(const void* to, int64_t bytes) { return (bytes + (int64_t)(reinterpret_cast<uintptr_t>(to) & 15) + 15) / 16; }
-__device__ __forceinline__ uint4 load_across(const char* row, int64_t bytes, int64_t at) {   // 16 bytes from byte `at` of the row on
-  const char* p = row + at;
-  const int off = (int)(reinterpret_cast<uintptr_t>(p) & 15);
-  p -= off;
-  uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-  if (p + 16 > row && p < row + bytes) lo = *reinterpret_cast<const uint4*>(p);
-  if (off && p + 32 > row && p + 16 < row + bytes) hi = *reinterpret_cast<const uint4*>(p + 16);
-  uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-  for (int i = 0; i < 6; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
-#pragma unroll
-  for (int i = 0; i < 5; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
-  const int bits = (off & 3) * 8;
-  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+// Rows that are no multiple of 16 bytes, or do not start on one ("odd"), still move 16 bytes at a time: whole aligned pieces of the row
+// that is written, each put together from the two aligned pieces that it lies across in the row that is read, and the elements at
+// the ends one by one.  Both of those pieces hold bytes of the piece that is wanted, so nothing is read that the row has no part in
+// (memory comes in whole ones).
+struct Cut {          // of a row that is written
+  int head, pieces;   // bytes in front of its whole pieces, their number
+};
+__device__ __forceinline__ Cut cut_of(const void* row, int bytes) {
+  const int head = (int)(-reinterpret_cast<uintptr_t>(row) & 15);
+  return head < bytes ? Cut{head, (bytes - head) / 16} : Cut{bytes, 0};
 }
-template <typename T> __device__ __forceinline__ void store_piece(char* row, int64_t bytes, int64_t at, const uint4& v) {   // an aligned one
-  if (at >= 0 && at + 16 <= bytes) {
-    *reinterpret_cast<uint4*>(row + at) = v;
+// Element i of those at the ends, or a negative number: their bytes in the row.
+template <typename T> __device__ __forceinline__ int end_element(const Cut& c, int bytes, int i) {
+  const int heads = c.head / (int)sizeof(T);
+  const int at = i < heads ? i * (int)sizeof(T) : c.head + 16 * c.pieces + (i - heads) * (int)sizeof(T);
+  return at < bytes ? at : -1;
+}
+template <typename T> constexpr int MOST_ENDS = 2 * (PER_PIECE<T> - 1);   // elements at both ends
+struct Across {       // a row that is read at the pieces of another one
+  const uint4* piece;   // the aligned one in which the first wanted piece begins
+  int off;              // where in it
+};
+__device__ __forceinline__ Across across(const char* row, const Cut& c) {
+  const uintptr_t p = reinterpret_cast<uintptr_t>(row + c.head);
+  return Across{reinterpret_cast<const uint4*>(p & ~(uintptr_t)15), (int)(p & 15)};
+}
+struct Pair {
+  uint4 lo, hi;
+};
+__device__ __forceinline__ Pair load_pair(const Across& r, int q) {
+  Pair v;
+  v.lo = r.piece[q];
+  if (r.off) v.hi = r.piece[q + 1];
+  return v;
+}
+// off is the same for a whole row: the branches are uniform.
+__device__ __forceinline__ uint4 joined(const Pair& v, int off) {
+  const int bits = (off & 3) * 8;
+  const uint4 &a = v.lo, &b = v.hi;
+  if (!off) return a;
+  switch (off >> 2) {
+    case 0: return make_uint4(__funnelshift_r(a.x, a.y, bits), __funnelshift_r(a.y, a.z, bits), __funnelshift_r(a.z, a.w, bits), __funnelshift_r(a.w, b.x, bits));
+    case 1: return make_uint4(__funnelshift_r(a.y, a.z, bits), __funnelshift_r(a.z, a.w, bits), __funnelshift_r(a.w, b.x, bits), __funnelshift_r(b.x, b.y, bits));
+    case 2: return make_uint4(__funnelshift_r(a.z, a.w, bits), __funnelshift_r(a.w, b.x, bits), __funnelshift_r(b.x, b.y, bits), __funnelshift_r(b.y, b.z, bits));
+    default: return make_uint4(__funnelshift_r(a.w, b.x, bits), __funnelshift_r(b.x, b.y, bits), __funnelshift_r(b.y, b.z, bits), __funnelshift_r(b.z, b.w, bits));
+  }
+}
+// An odd row, from another one or from nothing, by threads l, l + lanes, ...
+template <typename T> __device__ __forceinline__ void copy_odd(char* to, const char* from, int bytes, int l, int lanes) {
+  constexpr int U = 4;
+  const Cut c = cut_of(to, bytes);
+  for (int i = l; i < MOST_ENDS<T>; i += lanes) {
+    const int at = end_element<T>(c, bytes, i);
+    if (at >= 0) *reinterpret_cast<T*>(to + at) = from ? *reinterpret_cast<const T*>(from + at) : T{};
+  }
+  uint4* out = reinterpret_cast<uint4*>(to + c.head);
+  if (!from) {
+    for (int q = l; q < c.pieces; q += lanes) out[q] = make_uint4(0, 0, 0, 0);
     return;
   }
-  const T* e = reinterpret_cast<const T*>(&v);
+  const Across r = across(from, c);
+  for (int q0 = l; q0 < c.pieces; q0 += U * lanes) {
+    Pair v[U];
 #pragma unroll
-  for (int i = 0; i < PER_PIECE<T>; ++i)
-    if (at + i * (int)sizeof(T) >= 0 && at + i * (int)sizeof(T) < bytes) *reinterpret_cast<T*>(row + at + i * (int)sizeof(T)) = e[i];
-}
-// Zeros a row, a warp's work.
-template <typename T> __device__ __forceinline__ void clear_row(void* rows, int64_t bytes, int64_t r, int lane) {
-  char* row = static_cast<char*>(rows) + r * bytes;
-  for (int64_t q = lane; q < pieces_of(row, bytes); q += 32) store_piece<T>(row, bytes, piece_begin(row, q), make_uint4(0, 0, 0, 0));
+    for (int u = 0; u < U; ++u)
+      if (q0 + u * lanes < c.pieces) v[u] = load_pair(r, q0 + u * lanes);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (q0 + u * lanes < c.pieces) out[q0 + u * lanes] = joined(v[u], r.off);
+  }
 }
 
 __device__ __forceinline__ int64_t load_id(const void* ids, int wide, int64_t i) {
@@ -95,7 +128,8 @@ struct SortArgs {
   void* rows;
   int32_t *offsets, *pos, *src;
   int32_t* hist;        // [blocks, experts]: choices of each expert in each chunk
-  int64_t tokens, bytes;   // bytes of a row
+  int64_t tokens;
+  int bytes;   // of a row
   int n, k, experts, align, n_rows, ids64;
   int chunk, blocks;    // choices of a block in the counting and placing kernels
   int lanes;            // threads of a token in the copying kernels, a power of two
@@ -121,31 +155,19 @@ __device__ __forceinline__ void scan_offsets(const int* count, int* offsets, int
   }
 }
 
-// Copies the row of token t to the rows of its choices, `lanes` threads a token, four pieces in flight each.  ODD: see load_across.
+// Copies the row of token t to the rows of its choices, `lanes` threads a token, four pieces in flight each.
 template <typename T, bool ODD>
 __device__ __forceinline__ void copy_row(const SortArgs& a, int64_t t, int l, const int32_t* pos) {
   constexpr int U = 4;
   const char* from = static_cast<const char*>(a.x) + t * a.bytes;
+  char* const rows = static_cast<char*>(a.rows);
   if (ODD) {
-    for (int j = 0; j < a.k; ++j) {
-      const int r = pos[j];
-      if (r < 0) continue;
-      char* to = static_cast<char*>(a.rows) + (int64_t)r * a.bytes;
-      const int64_t pieces = pieces_of(to, a.bytes);
-      for (int64_t q0 = l; q0 < pieces; q0 += U * a.lanes) {
-        uint4 v[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (q0 + u * a.lanes < pieces) v[u] = load_across(from, a.bytes, piece_begin(to, q0 + u * a.lanes));
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (q0 + u * a.lanes < pieces) store_piece<T>(to, a.bytes, piece_begin(to, q0 + u * a.lanes), v[u]);
-      }
-    }
+    for (int j = 0; j < a.k; ++j)
+      if (pos[j] >= 0) copy_odd<T>(rows + (int64_t)pos[j] * a.bytes, from, a.bytes, l, a.lanes);
     return;
   }
-  const int64_t pieces = a.bytes / 16;
-  for (int64_t c0 = l; c0 < pieces; c0 += U * a.lanes) {
+  const int pieces = a.bytes / 16;
+  for (int c0 = l; c0 < pieces; c0 += U * a.lanes) {
     uint4 v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -153,7 +175,7 @@ __device__ __forceinline__ void copy_row(const SortArgs& a, int64_t t, int l, co
     for (int j = 0; j < a.k; ++j) {
       const int r = pos[j];
       if (r < 0) continue;
-      uint4* to = reinterpret_cast<uint4*>(static_cast<char*>(a.rows) + (int64_t)r * a.bytes);
+      uint4* to = reinterpret_cast<uint4*>(rows + (int64_t)r * a.bytes);
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (c0 + u * a.lanes < pieces) to[c0 + u * a.lanes] = v[u];
@@ -175,7 +197,7 @@ __global__ void __launch_bounds__(THREADS) sort_small_kernel(const SortArgs a) {
   for (int i = tid; i < a.n; i += THREADS) {
     const int e = expert_of(a.ids, a.ids64, i, a.experts);
     expert[i] = (int16_t)e;
-    if (e >= 0) atomicAdd(&count[e], 1);   // integers: the order of the additions does not show
+    if (e >= 0) atomicAdd(&count[e], 1);
   }
   __syncthreads();
   scan_offsets(count, offsets, a.experts, a.align);
@@ -214,7 +236,7 @@ __global__ void __launch_bounds__(THREADS) sort_small_kernel(const SortArgs a) {
       }
     if (lo < a.experts && r - offsets[lo] < count[lo]) continue;
     if (lane == 0) a.src[r] = -1;
-    clear_row<T>(a.rows, a.bytes, r, lane);
+    copy_odd<T>(static_cast<char*>(a.rows) + r * a.bytes, nullptr, a.bytes, lane, 32);
   }
 }
 
@@ -246,12 +268,20 @@ __global__ void __launch_bounds__(THREADS) sort_place_kernel(const SortArgs a) {
   chain_wait();
   chain_trigger();
   __syncthreads();
-  for (int i = tid; i < a.blocks * a.experts; i += THREADS) {
-    const int b = i / a.experts, e = i - b * a.experts, c = a.hist[i];
-    if (c) {
-      atomicAdd(&total[e], c);
-      if (b < (int)blockIdx.x) atomicAdd(&before[e], c);
+  // All blocks' counts added up: a thread takes every `stride`th block's of one expert, so that its loads are in flight together.
+  int wide = 32;
+  while (wide < a.experts && wide < THREADS) wide *= 2;
+  const int stride = THREADS / wide;
+  for (int e = tid & (wide - 1); e < a.experts; e += wide) {
+    int all = 0, front = 0;
+#pragma unroll 4
+    for (int b = tid / wide; b < a.blocks; b += stride) {
+      const int c = a.hist[(int64_t)b * a.experts + e];
+      all += c;
+      front += b < (int)blockIdx.x ? c : 0;
     }
+    if (all) atomicAdd(&total[e], all);   // integers: the order of the additions does not show
+    if (front) atomicAdd(&before[e], front);
   }
   const int run = (a.chunk + WARPS - 1) / WARPS;
   const int end = min((int)(blockIdx.x + 1) * a.chunk, a.n), first = min((int)blockIdx.x * a.chunk + warp * run, end), last = min(first + run, end);
@@ -297,29 +327,21 @@ __global__ void __launch_bounds__(THREADS) sort_copy_kernel(const SortArgs a) {
   if (t < a.tokens) copy_row<uint32_t, false>(a, t, threadIdx.x & (a.lanes - 1), a.pos + t * a.k);
   const int lane = threadIdx.x & 31;
   for (int64_t r = (int64_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5); r < a.n_rows; r += (int64_t)gridDim.x * (THREADS / 32))
-    if (a.src[r] < 0) clear_row<uint32_t>(a.rows, a.bytes, r, lane);
+    if (a.src[r] < 0) copy_odd<uint32_t>(static_cast<char*>(a.rows) + r * a.bytes, nullptr, a.bytes, lane, 32);
 }
-// Odd rows are put together for each place anyway: row by row, the rows of no choice among them, which are all alike much work.
+// Odd rows are put together for each place anyway: row by row, those of no choice among them, all of them alike much work.  Blocks go
+// on to further rows and know where from before they get there (a block a few rows 26 us for 4099 x 1405 fp16, 6 choices).
 template <typename T>
 __global__ void __launch_bounds__(THREADS) sort_copy_odd_kernel(const SortArgs a) {
-  constexpr int U = 4;
   chain_wait();
-  const int64_t r = (int64_t)blockIdx.x * (THREADS / a.lanes) + threadIdx.x / a.lanes;
-  if (r >= a.n_rows) return;
-  const int i = a.src[r];
-  const char* from = static_cast<const char*>(a.x) + (i < 0 ? 0 : i / a.k) * a.bytes;
-  char* to = static_cast<char*>(a.rows) + r * a.bytes;
-  const int64_t pieces = pieces_of(to, a.bytes);
-  for (int64_t q0 = threadIdx.x & (a.lanes - 1); q0 < pieces; q0 += U * a.lanes) {
-    uint4 v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      v[u] = make_uint4(0, 0, 0, 0);
-      if (i >= 0 && q0 + u * a.lanes < pieces) v[u] = load_across(from, a.bytes, piece_begin(to, q0 + u * a.lanes));
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (q0 + u * a.lanes < pieces) store_piece<T>(to, a.bytes, piece_begin(to, q0 + u * a.lanes), v[u]);
+  const int64_t step = (int64_t)gridDim.x * (THREADS / a.lanes);
+  int64_t r = (int64_t)blockIdx.x * (THREADS / a.lanes) + threadIdx.x / a.lanes;
+  int i = r < a.n_rows ? a.src[r] : -1;
+  for (; r < a.n_rows; r += step) {
+    const int next = r + step < a.n_rows ? a.src[r + step] : -1;
+    copy_odd<T>(static_cast<char*>(a.rows) + r * a.bytes, i < 0 ? nullptr : static_cast<const char*>(a.x) + (int64_t)(i / a.k) * a.bytes, a.bytes,
+                threadIdx.x & (a.lanes - 1), a.lanes);
+    i = next;
   }
 }
 
@@ -329,8 +351,8 @@ struct CombineArgs {
   const int32_t *pos, *src;
   const void* dy;
   void *y, *drows, *dweights;
-  int64_t tokens, bytes, n_rows;   // bytes of a row
-  int k, lanes;
+  int64_t tokens, n_rows;
+  int bytes, k, lanes;   // bytes of a row
 };
 
 template <typename W> __device__ __forceinline__ float weight_of(const void* w, int64_t i) { return w ? to_float(static_cast<const W*>(w)[i]) : 1.f; }
@@ -339,9 +361,8 @@ __device__ __forceinline__ int row_of(const CombineArgs& a, int64_t i) {
   const int r = a.pos[i];
   return r >= 0 && r < a.n_rows ? r : -1;
 }
-template <bool ODD> __device__ __forceinline__ uint4 load_piece(const char* row, int64_t bytes, int64_t at) {
-  return ODD ? load_across(row, bytes, at) : *reinterpret_cast<const uint4*>(row + at);
-}
+__device__ __forceinline__ const char* row_at(const void* rows, int64_t r, int bytes) { return static_cast<const char*>(rows) + r * bytes; }
+__device__ __forceinline__ char* row_at(void* rows, int64_t r, int bytes) { return static_cast<char*>(rows) + r * bytes; }
 
 // y[t] = sum over j of w[t, j] * rows[pos[t, j]], in the order of j, in 32 bits and rounded once.  J choices at a time and U
 // pieces of their rows, so that J * U loads are in flight together.
@@ -349,51 +370,80 @@ template <typename T, typename W, bool ODD, int J, int U>
 __global__ void __launch_bounds__(THREADS) combine_kernel(const CombineArgs a) {
   constexpr int N = PER_PIECE<T>;
   const int64_t t = (int64_t)blockIdx.x * (THREADS / a.lanes) + threadIdx.x / a.lanes;
+  const int l = threadIdx.x & (a.lanes - 1);
   if (t >= a.tokens) return;
-  char* y = static_cast<char*>(a.y) + t * a.bytes;
-  const int64_t pieces = pieces_of(y, a.bytes);
-  for (int64_t q0 = threadIdx.x & (a.lanes - 1); q0 < pieces; q0 += U * a.lanes) {
+  char* y = row_at(a.y, t, a.bytes);
+  const Cut cut = ODD ? cut_of(y, a.bytes) : Cut{0, a.bytes / 16};
+  uint4* out = reinterpret_cast<uint4*>(y + cut.head);
+  for (int q0 = l; q0 < cut.pieces; q0 += U * a.lanes) {
     float acc[U][N];
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < N; ++i) acc[u][i] = 0.f;
+    int later_r[J];
+    float later_w[J];
+    auto choices = [&](int j0) {   // loaded while the rows of those in front are on their way
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const bool some = j0 + j < a.k;
+        later_r[j] = some ? row_of(a, t * a.k + j0 + j) : -1;
+        later_w[j] = some ? weight_of<W>(a.weights, t * a.k + j0 + j) : 0.f;
+      }
+    };
+    choices(0);
     for (int j0 = 0; j0 < a.k; j0 += J) {
-      uint4 v[J][U];
+      Pair v[J][U];
+      Across from[J];
       float w[J];
       int r[J];
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        r[j] = j0 + j < a.k ? row_of(a, t * a.k + j0 + j) : -1;
-        w[j] = r[j] >= 0 ? weight_of<W>(a.weights, t * a.k + j0 + j) : 0.f;
+        r[j] = later_r[j];
+        w[j] = later_w[j];
       }
 #pragma unroll
-      for (int j = 0; j < J; ++j)
+      for (int j = 0; j < J; ++j) {
+        if (r[j] < 0) continue;
+        const char* row = row_at(a.rows, r[j], a.bytes);
+        from[j] = ODD ? across(row, cut) : Across{reinterpret_cast<const uint4*>(row), 0};
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (r[j] >= 0 && q0 + u * a.lanes < pieces)
-            v[j][u] = load_piece<ODD>(static_cast<const char*>(a.rows) + (int64_t)r[j] * a.bytes, a.bytes, piece_begin(y, q0 + u * a.lanes));
+          if (q0 + u * a.lanes < cut.pieces) v[j][u] = load_pair(from[j], q0 + u * a.lanes);
+      }
+      choices(j0 + J);
 #pragma unroll
-      for (int j = 0; j < J; ++j)
-        if (r[j] >= 0) {
+      for (int j = 0; j < J; ++j) {
+        if (r[j] < 0) continue;
 #pragma unroll
-          for (int u = 0; u < U; ++u) {
-            float f[N];
-            unpack<T>(v[j][u], f);
+        for (int u = 0; u < U; ++u) {
+          float f[N];
+          unpack<T>(joined(v[j][u], ODD ? from[j].off : 0), f);
 #pragma unroll
-            for (int i = 0; i < N; ++i) acc[u][i] = fmaf(w[j], f[i], acc[u][i]);
-          }
+          for (int i = 0; i < N; ++i) acc[u][i] = fmaf(w[j], f[i], acc[u][i]);
         }
+      }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (q0 + u * a.lanes < pieces) store_piece<T>(y, a.bytes, piece_begin(y, q0 + u * a.lanes), pack<T>(acc[u]));
+      if (q0 + u * a.lanes < cut.pieces) out[q0 + u * a.lanes] = pack<T>(acc[u]);
   }
+  if (ODD)
+    for (int i = l; i < MOST_ENDS<T>; i += a.lanes) {
+      const int at = end_element<T>(cut, a.bytes, i);
+      if (at < 0) continue;
+      float sum = 0.f;
+      for (int j = 0; j < a.k; ++j) {
+        const int r = row_of(a, t * a.k + j);
+        if (r >= 0) sum = fmaf(weight_of<W>(a.weights, t * a.k + j), to_float(*reinterpret_cast<const T*>(row_at(a.rows, r, a.bytes) + at)), sum);
+      }
+      *reinterpret_cast<T*>(y + at) = from_float<T>(sum);
+    }
 }
 
 // drows[pos[t, j]] = w[t, j] * dy[t], rows of no choice zero; dw[t, j] = the sum of dy[t] * rows[pos[t, j]], added in an order that
 // depends on the sizes and the alignment only.  A row is written by the choice that src names, so that rows are written once whatever pos
-// holds.  J choices at a time share the loads of dy; of ODD rows each has pieces of its own, so those come one by one.
+// holds.  J choices at a time share the loads of dy; of odd rows each has pieces of its own, so those come one by one.
 template <typename T, typename W, bool ODD, int J, int U>
 __global__ void __launch_bounds__(THREADS) combine_backward_kernel(const CombineArgs a) {
   static_assert(!ODD || J == 1, "one choice at a time");
@@ -402,7 +452,7 @@ __global__ void __launch_bounds__(THREADS) combine_backward_kernel(const Combine
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = threadIdx.x & (a.lanes - 1);
   const int64_t t = (int64_t)blockIdx.x * (THREADS / a.lanes) + threadIdx.x / a.lanes;
   const bool live = t < a.tokens;
-  const char* dy = static_cast<const char*>(a.dy) + t * a.bytes;
+  const char* dy = row_at(a.dy, t, a.bytes);
   for (int j0 = 0; j0 < a.k; j0 += J) {
     float w[J], dot[J];
     const char* from[J];   // the choice's row, null: nothing to read, or to write
@@ -412,43 +462,56 @@ __global__ void __launch_bounds__(THREADS) combine_backward_kernel(const Combine
       const int64_t i = t * a.k + j0 + j;
       const int r = live && j0 + j < a.k ? row_of(a, i) : -1;
       w[j] = r >= 0 ? weight_of<W>(a.weights, i) : 0.f;
-      from[j] = r >= 0 && a.dweights ? static_cast<const char*>(a.rows) + (int64_t)r * a.bytes : nullptr;
-      to[j] = r >= 0 && a.drows && a.src[r] == (int32_t)i ? static_cast<char*>(a.drows) + (int64_t)r * a.bytes : nullptr;
+      from[j] = r >= 0 && a.dweights ? row_at(a.rows, r, a.bytes) : nullptr;
+      to[j] = r >= 0 && a.drows && a.src[r] == (int32_t)i ? row_at(a.drows, r, a.bytes) : nullptr;
       dot[j] = 0.f;
     }
     // pieces of the row written; without one, of the row read
-    const void* grid = ODD ? (to[0] ? to[0] : from[0]) : nullptr;
-    const int64_t pieces = live && (!ODD || grid) ? pieces_of(grid, a.bytes) : 0;
-    for (int64_t q0 = l; q0 < pieces; q0 += U * a.lanes) {
-      uint4 g[U], v[J][U];
+    Cut cut{0, live ? a.bytes / 16 : 0};
+    Across g_from{reinterpret_cast<const uint4*>(dy), 0}, v_from{nullptr, 0};
+    if (ODD) {
+      const char* grid = to[0] ? to[0] : from[0];
+      cut = grid ? cut_of(grid, a.bytes) : Cut{0, 0};
+      if (grid) g_from = across(dy, cut);
+      if (from[0]) v_from = across(from[0], cut);
+      if (grid)
+        for (int i = l; i < MOST_ENDS<T>; i += a.lanes) {
+          const int at = end_element<T>(cut, a.bytes, i);
+          if (at < 0) continue;
+          const float d = to_float(*reinterpret_cast<const T*>(dy + at));
+          if (from[0]) dot[0] = fmaf(d, to_float(*reinterpret_cast<const T*>(from[0] + at)), dot[0]);
+          if (to[0]) *reinterpret_cast<T*>(to[0] + at) = from_float<T>(d * w[0]);
+        }
+    }
+    for (int q0 = l; q0 < cut.pieces; q0 += U * a.lanes) {
+      Pair g[U], v[J][U];
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (q0 + u * a.lanes < pieces) g[u] = load_piece<ODD>(dy, a.bytes, piece_begin(grid, q0 + u * a.lanes));
+        if (q0 + u * a.lanes < cut.pieces) g[u] = load_pair(g_from, q0 + u * a.lanes);
 #pragma unroll
       for (int j = 0; j < J; ++j)
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (from[j] && q0 + u * a.lanes < pieces) v[j][u] = load_piece<ODD>(from[j], a.bytes, piece_begin(grid, q0 + u * a.lanes));
+          if (from[j] && q0 + u * a.lanes < cut.pieces)
+            v[j][u] = load_pair(ODD ? v_from : Across{reinterpret_cast<const uint4*>(from[j]), 0}, q0 + u * a.lanes);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (q0 + u * a.lanes >= pieces) break;
-        const int64_t at = piece_begin(grid, q0 + u * a.lanes);
+        if (q0 + u * a.lanes >= cut.pieces) break;
         float d[N];
-        unpack<T>(g[u], d);
+        unpack<T>(joined(g[u], ODD ? g_from.off : 0), d);
 #pragma unroll
         for (int j = 0; j < J; ++j) {
           if (from[j]) {
             float f[N];
-            unpack<T>(v[j][u], f);
+            unpack<T>(joined(v[j][u], ODD ? v_from.off : 0), f);
 #pragma unroll
-            for (int q = 0; q < N; ++q)
-              if (!ODD || (at + q * (int)sizeof(T) >= 0 && at + q * (int)sizeof(T) < a.bytes)) dot[j] = fmaf(d[q], f[q], dot[j]);   // what lies around the row is others'
+            for (int q = 0; q < N; ++q) dot[j] = fmaf(d[q], f[q], dot[j]);
           }
           if (to[j]) {
             float f[N];
 #pragma unroll
             for (int q = 0; q < N; ++q) f[q] = d[q] * w[j];
-            store_piece<T>(to[j], a.bytes, at, pack<T>(f));
+            reinterpret_cast<uint4*>(to[j] + cut.head)[q0 + u * a.lanes] = pack<T>(f);
           }
         }
       }
@@ -479,7 +542,7 @@ __global__ void __launch_bounds__(THREADS) combine_backward_kernel(const Combine
   }
   if (a.drows)
     for (int64_t r = (int64_t)blockIdx.x * (THREADS / 32) + warp; r < a.n_rows; r += (int64_t)gridDim.x * (THREADS / 32))
-      if (a.src[r] < 0) clear_row<T>(a.drows, a.bytes, r, lane);
+      if (a.src[r] < 0) copy_odd<T>(row_at(a.drows, r, a.bytes), nullptr, a.bytes, lane, 32);
 }
 
 // The same two for many tokens with rows of whole 16 bytes.  What bounds them is how many bytes are in flight: with loads into registers
@@ -639,7 +702,7 @@ __global__ void __launch_bounds__(RING_THREADS) combine_ring_kernel(const Combin
   asm volatile("cp.async.wait_all;" ::: "memory");
   if (BACKWARD && a.drows)
     for (int64_t r = me; r < a.n_rows; r += warps)
-      if (a.src[r] < 0) clear_row<T>(a.drows, a.bytes, r, lane);
+      if (a.src[r] < 0) copy_odd<T>(row_at(a.drows, r, a.bytes), nullptr, a.bytes, lane, 32);
 }
 
 // ------------------------------------------------------------------------------------------ host
@@ -670,7 +733,7 @@ int check_rows(const char* name, int64_t tokens, int64_t cols, int64_t rows, int
   if (dtype != I8L_DTYPE_BF16 && dtype != I8L_DTYPE_F16 && dtype != I8L_DTYPE_F32) return fail(I8L_ERR_ARG, "%s: unknown dtype %d", name, dtype);
   if (wdtype != I8L_DTYPE_F32 && wdtype != dtype) return fail(I8L_ERR_ARG, "%s: weights are fp32 or of the rows' type", name);
   if (k < 1 || k > MAX_CHOICES) return fail(I8L_ERR_SHAPE, "%s: %d choices a token, 1 to %d are possible", name, k, MAX_CHOICES);
-  if (tokens < 0 || cols < 1 || rows < 0 || tokens > (1ll << 30) / k || rows >= (1ll << 31) || cols >= (1ll << 31))
+  if (tokens < 0 || cols < 1 || rows < 0 || tokens > (1ll << 30) / k || rows >= (1ll << 31) || cols > (1ll << 28))
     return fail(I8L_ERR_SHAPE, "%s: tokens=%lld cols=%lld rows=%lld out of range", name, (long long)tokens, (long long)cols, (long long)rows);
   return I8L_OK;
 }
@@ -697,7 +760,7 @@ int launch_combine(const CombineArgs& a, bool backward, bool odd, cudaStream_t s
     else if (a.k <= 2) combine_backward_kernel<T, W, false, 2, 2><<<grid, THREADS, 0, st>>>(a);
     else combine_backward_kernel<T, W, false, 4, 2><<<grid, THREADS, 0, st>>>(a);
   } else {
-    if (odd) combine_kernel<T, W, true, 4, 2><<<grid, THREADS, 0, st>>>(a);
+    if (odd) combine_kernel<T, W, true, 2, 1><<<grid, THREADS, 0, st>>>(a);
     else if (one) combine_kernel<T, W, false, 4, 1><<<grid, THREADS, 0, st>>>(a);
     else if (a.k <= 2) combine_kernel<T, W, false, 2, 4><<<grid, THREADS, 0, st>>>(a);
     else combine_kernel<T, W, false, 4, 2><<<grid, THREADS, 0, st>>>(a);
@@ -710,7 +773,7 @@ int launch_combine(const CombineArgs& a, int wdtype, bool backward, bool odd, cu
   return wdtype == I8L_DTYPE_F32 ? launch_combine<T, float>(a, backward, odd, st) : launch_combine<T, T>(a, backward, odd, st);
 }
 int run_combine(CombineArgs a, int64_t cols, int dtype, int wdtype, bool backward, cudaStream_t st) {
-  a.bytes = cols * elem_size(dtype);
+  a.bytes = (int)(cols * elem_size(dtype));
   a.lanes = lanes_for(a.bytes, a.tokens);
   const bool odd = a.bytes % 16 || !aligned16(a.rows) || !aligned16(a.y) || !aligned16(a.dy) || !aligned16(a.drows);
   if (dtype == I8L_DTYPE_F32) return launch_combine<float, float>(a, backward, odd, st);
@@ -750,7 +813,7 @@ extern "C" int i8l_sort_tokens(const void* x, const void* ids, int ids64, int64_
   SortArgs a{};
   a.x = x; a.ids = ids; a.rows = out; a.offsets = offsets; a.pos = pos; a.src = src;
   a.hist = static_cast<int32_t*>(workspace);
-  a.tokens = tokens; a.bytes = cols * size;
+  a.tokens = tokens; a.bytes = (int)(cols * size);
   a.n = (int)n; a.k = k; a.experts = experts; a.align = (int)align; a.n_rows = (int)rows; a.ids64 = ids64 ? 1 : 0;
   a.lanes = lanes_for(a.bytes, tokens);
   const unsigned copies = (unsigned)((tokens + THREADS / a.lanes - 1) / (THREADS / a.lanes));
@@ -769,7 +832,8 @@ extern "C" int i8l_sort_tokens(const void* x, const void* ids, int ids64, int64_
   I8L_CUDA_OK(launch(sort_count_kernel, dim3(a.blocks), THREADS, 0, st, a));
   I8L_CUDA_OK(launch(sort_place_kernel, dim3(a.blocks), THREADS, THREADS / 32 * experts * sizeof(int), st, a));
   if (odd) a.lanes = lanes_for(a.bytes, rows);
-  const dim3 by_row((unsigned)((rows + THREADS / a.lanes - 1) / (THREADS / a.lanes)));
+  const int64_t row_blocks = (rows + THREADS / a.lanes - 1) / (THREADS / a.lanes), resident = 4 * sm_count();
+  const dim3 by_row((unsigned)(row_blocks < resident ? row_blocks : resident));
   I8L_CUDA_OK(!odd        ? launch(sort_copy_kernel, dim3(grid), THREADS, 0, st, a)
               : size == 4 ? launch(sort_copy_odd_kernel<uint32_t>, by_row, THREADS, 0, st, a)
                           : launch(sort_copy_odd_kernel<uint16_t>, by_row, THREADS, 0, st, a));
