@@ -86,7 +86,9 @@ def test_workspace_sizes(lib):
     assert lib.i8l_sort_workspace(512, 2, 8) == 0                      # few choices need none
     assert lib.i8l_sort_workspace(513, 2, 8) == 5 * 8 * 4              # chunks of 256 choices
     assert lib.i8l_sort_workspace(1 << 20, 8, 1024) == 16 * 1024 * 4
-    assert lib.i8l_token_linear_workspace(3, 48) == 256 + 256
+    assert lib.i8l_token_linear_workspace(9, 48) == 512 + 256
+    assert lib.i8l_token_linear_workspace(8, 48) == 0                  # few rows: one launch
+    assert lib.i8l_token_linear_workspace(1, 131072) == 131072 + 256   # but long ones
     assert lib.i8l_token_linear_workspace(0, 48) == 0
 
 

@@ -43,116 +43,181 @@ __device__ __forceinline__ uint4 load_weights(const int8_t* p) {   // read once:
 }
 
 // ------------------------------------------------------------------------------------------ few rows
-// Up to eight rows: a warp multiplies two channels' weights with the rows of their expert by dp4a, 512 bytes of K a step.  Bound by
-// the weights' bytes, so it is the loads that matter: a warp has eight of 16 bytes a lane in flight ahead of those it works on, and
-// the first go out before the rows have been quantized (the weights and offsets were there before the chain).  The rows then come
-// to shared memory; a piece of them read there serves two loads of weights.
-constexpr int FEW_THREADS = 256, FEW_WARP_COLS = 2, FEW_COLS = FEW_THREADS / 32 * FEW_WARP_COLS, FEW_STEPS = 4, FEW_BATCH = FEW_STEPS * 512;
+// Up to eight rows in one launch: every block quantizes them into its shared memory, then its warps go through the channels of the
+// experts that have rows, two at a time, and multiply the weights by dp4a.  Bound by the weights' bytes, so it is the loads that
+// matter: while a warp works on a batch (2 KB of each of its two channels, eight loads of 16 bytes a lane) the next one is in flight,
+// across channels and experts, and the first goes out ahead of the quantization.
+constexpr int FEW_THREADS = 256, FEW_WARPS = FEW_THREADS / 32, FEW_COLS = 2, FEW_STEPS = 4, FEW_BATCH = FEW_STEPS * 512, FEW_ROWS = 8;
+
+struct FewSegment {
+  int expert, row, rows;
+};
+struct Batch {
+  uint4 w[FEW_COLS][FEW_STEPS];
+};
+template <int MT, int CT>
+__device__ __forceinline__ void multiply_batch(int (&acc)[FEW_COLS][MT], const Batch& w, const int8_t* rows, int count, int K, int limit, int k0) {
+  int at[CT];   // of a row: CT may be above their number, and what is multiplied with the first one once more is not used
+#pragma unroll
+  for (int t = 0; t < CT; ++t) at[t] = t < count ? t * K : 0;
+#pragma unroll
+  for (int s = 0; s < FEW_STEPS; ++s) {
+    const int k = k0 + s * 512;
+    if (k >= limit) break;
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+      const uint4 v = *reinterpret_cast<const uint4*>(rows + at[t] + k);
+#pragma unroll
+      for (int j = 0; j < FEW_COLS; ++j) {
+        acc[j][t] = __dp4a((int)w.w[j][s].x, (int)v.x, acc[j][t]);
+        acc[j][t] = __dp4a((int)w.w[j][s].y, (int)v.y, acc[j][t]);
+        acc[j][t] = __dp4a((int)w.w[j][s].z, (int)v.z, acc[j][t]);
+        acc[j][t] = __dp4a((int)w.w[j][s].w, (int)v.w, acc[j][t]);
+      }
+    }
+  }
+}
 
 template <int MT>
-__global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const TokenArgs a, const int8_t* xq, const float* xs) {
-  extern __shared__ __align__(16) int8_t rows[];   // [MT, K]
-  __shared__ int s_expert;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int K = (int)a.K;
-  int64_t begin, end;
-  int e = 0;
-  if (a.offsets) {   // the blockIdx.y-th expert that has rows
+__global__ void __launch_bounds__(FEW_THREADS, 2) few_rows_kernel(const TokenArgs a) {
+  extern __shared__ __align__(16) int8_t xq[];   // [MT, K]
+  __shared__ float xs[MT], red[FEW_WARPS];
+  __shared__ FewSegment s_seg[FEW_ROWS];
+  __shared__ int s_segments;
+  constexpr int LANES = FEW_THREADS / MT;        // threads that quantize a row
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = (int)a.K;
+  if (a.offsets) {   // the experts that have rows, at most as many as rows
     if (warp == 0) {
-      int found = -1, left = blockIdx.y;
-      for (int e0 = 0; e0 < a.experts && found < 0; e0 += 32) {
-        bool some = false;
-        if (e0 + lane < a.experts) {
-          segment(a, e0 + lane, begin, end);
-          some = end > begin;
-        }
-        const unsigned set = __ballot_sync(0xffffffffu, some);
-        if (left < __popc(set)) found = e0 + (int)__fns(set, 0, left + 1);
-        else left -= __popc(set);
+      int count = 0;
+      for (int e0 = 0; e0 < a.experts; e0 += 32) {
+        int64_t begin = 0, end = 0;
+        if (e0 + lane < a.experts) segment(a, e0 + lane, begin, end);
+        const unsigned set = __ballot_sync(0xffffffffu, end > begin);
+        const int at = count + __popc(set & ((1u << lane) - 1));
+        if (end > begin && at < FEW_ROWS) s_seg[at] = FewSegment{e0 + lane, (int)begin, (int)(end - begin)};
+        count += __popc(set);
       }
-      if (lane == 0) s_expert = found;
+      if (lane == 0) s_segments = count < FEW_ROWS ? count : FEW_ROWS;   // more only where offsets decrease
     }
-    __syncthreads();
-    e = s_expert;
+  } else if (tid == 0) {
+    s_seg[0] = FewSegment{0, 0, (int)a.rows};
+    s_segments = 1;
   }
-  const int64_t n0 = (int64_t)blockIdx.x * FEW_COLS + warp * FEW_WARP_COLS;
-  const int8_t* w = a.wq + ((int64_t)(e < 0 ? 0 : e) * a.N + n0) * a.K + lane * 16;
-  const bool live = e >= 0 && n0 < a.N;   // N is a multiple of 8: both channels or none
-  uint4 now[FEW_WARP_COLS][FEW_STEPS], next[FEW_WARP_COLS][FEW_STEPS];
-  auto load = [&](uint4 (&to)[FEW_WARP_COLS][FEW_STEPS], int k0) {
+  __syncthreads();
+
+  // Where a warp is: channels n and n + 1 of segment `seg`, K from k on.
+  const int64_t step = (int64_t)gridDim.x * FEW_WARPS * FEW_COLS;
+  struct Place {
+    int seg, k;
+    int64_t n;
+  };
+  const int segments = s_segments;
+  auto settle = [&](Place& p) {   // into the segment that its channels belong to
+    while (p.seg < segments && p.n >= a.N) {
+      p.n -= a.N;
+      ++p.seg;
+    }
+  };
+  auto load = [&](Batch& b, const Place& p) {
+    if (p.seg >= segments) return;
+    const int8_t* w = a.wq + ((int64_t)s_seg[p.seg].expert * a.N + p.n) * a.K + lane * 16;
 #pragma unroll
     for (int s = 0; s < FEW_STEPS; ++s)
 #pragma unroll
-      for (int j = 0; j < FEW_WARP_COLS; ++j)
-        if (live && k0 + s * 512 + lane * 16 < K) to[j][s] = load_weights(w + (int64_t)j * K + k0 + s * 512);
+      for (int j = 0; j < FEW_COLS; ++j)
+        if (p.k + s * 512 + lane * 16 < K) b.w[j][s] = load_weights(w + (int64_t)j * K + p.k + s * 512);
   };
-  load(now, 0);
-  chain_wait();
-  if (a.offsets && blockIdx.y == 0) {   // rows of no expert
-    int64_t b, n, last_b, last_n;
-    segment(a, 0, b, n);
-    segment(a, a.experts - 1, last_b, last_n);
-    const int64_t dead = b + (a.rows - last_n);
-    for (int64_t i = tid; i < dead * FEW_COLS; i += FEW_THREADS) {
-      const int64_t r = i / FEW_COLS, c = (int64_t)blockIdx.x * FEW_COLS + i % FEW_COLS;
-      const int64_t at = (r < b ? r : last_n + r - b) * a.N + c;
-      if (c < a.N) {
-        if (a.out_f32) static_cast<float*>(a.y)[at] = 0.f;
-        else static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(0.f);
-      }
-    }
-  }
-  if (e < 0) return;
-  segment(a, e, begin, end);
-  const int count = (int)(end - begin);
-  for (int i = tid; i < MT * K / 16; i += FEW_THREADS)
-    reinterpret_cast<uint4*>(rows)[i] = i < count * K / 16 ? reinterpret_cast<const uint4*>(xq + begin * K)[i] : make_uint4(0, 0, 0, 0);
-  __syncthreads();
-  if (!live) return;
-  int acc[FEW_WARP_COLS][MT];
+  Place now{0, 0, ((int64_t)warp * gridDim.x + blockIdx.x) * FEW_COLS};
+  settle(now);
+  Batch even, odd;
+  load(even, now);
+
+  {   // the rows in int8, a scale each
+    const int t = tid / LANES, l = tid & (LANES - 1);
+    const bool live = t < a.rows;
+    const uint4* row = reinterpret_cast<const uint4*>(a.x + t * a.K);
+    float m = 0.f;
+    if (live)
+#pragma unroll 4
+      for (int c = l; c < K / 8; c += LANES) {
+        float v[8];
+        unpack8(row[c], v);
 #pragma unroll
-  for (int j = 0; j < FEW_WARP_COLS; ++j)
+        for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[i]));
+      }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) red[warp] = m;
+    __syncthreads();
+    m = red[t * (LANES / 32)];
+#pragma unroll
+    for (int i = 1; i < LANES / 32; ++i) m = fmaxf(m, red[t * (LANES / 32) + i]);
+    float s, stored;
+    make_scale<I8L_QMODE_ROWRCP>(m, s, stored);
+    if (l == 0) xs[t] = stored;
+    uint2* q = reinterpret_cast<uint2*>(xq + t * K);
+#pragma unroll 4
+    for (int c = l; c < K / 8; c += LANES) q[c] = live ? quant_piece<I8L_QMODE_ROWRCP>(row[c], s) : make_uint2(0, 0);
+    __syncthreads();
+  }
+
+  int acc[FEW_COLS][MT];
+#pragma unroll
+  for (int j = 0; j < FEW_COLS; ++j)
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[j][t] = 0;
-  auto multiply = [&](const uint4 (&u)[FEW_WARP_COLS][FEW_STEPS], int k0) {
+  auto work = [&](Batch& mine, Batch& ahead) {
+    Place next = now;
+    next.k += FEW_BATCH;
+    const bool last = next.k >= K;
+    if (last) {
+      next.k = 0;
+      next.n += step;
+      settle(next);
+    }
+    load(ahead, next);
+    const FewSegment seg = s_seg[now.seg];
+    const int8_t* rows = xq + (int64_t)seg.row * K + lane * 16;
+    const int limit = K - lane * 16;   // of k, so that the lane's 16 bytes are inside the row
+    if (MT == 1 || seg.rows == 1) multiply_batch<MT, 1>(acc, mine, rows, seg.rows, K, limit, now.k);
+    else if (MT == 2 || seg.rows == 2) multiply_batch<MT, MT < 2 ? MT : 2>(acc, mine, rows, seg.rows, K, limit, now.k);
+    else if (MT == 4 || seg.rows <= 4) multiply_batch<MT, MT < 4 ? MT : 4>(acc, mine, rows, seg.rows, K, limit, now.k);
+    else multiply_batch<MT, MT>(acc, mine, rows, seg.rows, K, limit, now.k);
+    if (last) {
+      int sum = 0;   // lane j * MT + t has that of channel j and row t
 #pragma unroll
-    for (int s = 0; s < FEW_STEPS; ++s) {
-      const int k = k0 + s * 512 + lane * 16;
-      if (k >= K) break;
+      for (int j = 0; j < FEW_COLS; ++j)
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        const uint4 v = *reinterpret_cast<const uint4*>(rows + t * K + k);
-#pragma unroll
-        for (int j = 0; j < FEW_WARP_COLS; ++j) {
-          acc[j][t] = __dp4a((int)u[j][s].x, (int)v.x, acc[j][t]);
-          acc[j][t] = __dp4a((int)u[j][s].y, (int)v.y, acc[j][t]);
-          acc[j][t] = __dp4a((int)u[j][s].z, (int)v.z, acc[j][t]);
-          acc[j][t] = __dp4a((int)u[j][s].w, (int)v.w, acc[j][t]);
+        for (int t = 0; t < MT; ++t) {
+          const int all = __reduce_add_sync(0xffffffffu, acc[j][t]);
+          if (lane == j * MT + t) sum = all;
+          acc[j][t] = 0;
         }
+      const int j = lane / MT, t = lane % MT;
+      if (j < FEW_COLS && t < seg.rows) {
+        const int64_t c = (int64_t)seg.expert * a.N + now.n + j, at = (int64_t)(seg.row + t) * a.N + now.n + j;
+        float v = __fmul_rn(__fmul_rn(__int2float_rn(sum), xs[seg.row + t]), a.ws[c]);
+        if (a.bias) v = __fadd_rn(v, __bfloat162float(a.bias[c]));
+        if (a.out_f32) static_cast<float*>(a.y)[at] = v;
+        else static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(v);
       }
     }
+    now = next;
   };
-  for (int k0 = 0; k0 < K; k0 += 2 * FEW_BATCH) {
-    load(next, k0 + FEW_BATCH);
-    multiply(now, k0);
-    load(now, k0 + 2 * FEW_BATCH);
-    multiply(next, k0 + FEW_BATCH);
+  while (now.seg < segments) {
+    work(even, odd);
+    if (now.seg >= segments) break;
+    work(odd, even);
   }
-  int mine = 0;   // lane j * MT + t has the sum of channel j and row t
-#pragma unroll
-  for (int j = 0; j < FEW_WARP_COLS; ++j)
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      const int sum = __reduce_add_sync(0xffffffffu, acc[j][t]);
-      if (lane == j * MT + t) mine = sum;
+  if (a.offsets) {   // rows of no expert
+    const int64_t pieces = a.N * (a.out_f32 ? 4 : 2) / 16;
+    for (int64_t r = 0; r < a.rows; ++r) {
+      bool some = false;
+      for (int i = 0; i < segments; ++i) some |= r >= s_seg[i].row && r < s_seg[i].row + s_seg[i].rows;
+      if (some) continue;
+      for (int64_t c = (int64_t)blockIdx.x * FEW_THREADS + tid; c < pieces; c += (int64_t)gridDim.x * FEW_THREADS)
+        static_cast<uint4*>(a.y)[r * pieces + c] = make_uint4(0, 0, 0, 0);
     }
-  const int j = lane / MT, t = lane % MT;
-  if (j < FEW_WARP_COLS && t < count) {
-    const int64_t n = n0 + j, c = (int64_t)e * a.N + n, at = (begin + t) * a.N + n;
-    float v = __fmul_rn(__fmul_rn(__int2float_rn(mine), xs[begin + t]), a.ws[c]);
-    if (a.bias) v = __fadd_rn(v, __bfloat162float(a.bias[c]));
-    if (a.out_f32) static_cast<float*>(a.y)[at] = v;
-    else static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(v);
   }
 }
 
@@ -515,14 +580,15 @@ group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
 constexpr int FEW_SMEM = 64 * 1024;
 int few_rows(int64_t rows, int64_t K) {
   const int mt = rows == 1 ? 1 : rows == 2 ? 2 : rows <= 4 ? 4 : 8;
-  return rows <= 8 && mt * K <= FEW_SMEM ? mt : 0;
+  return rows <= FEW_ROWS && mt * K <= FEW_SMEM ? mt : 0;
 }
-template <int MT> int launch_few(const TokenArgs& a, const int8_t* xq, const float* xs, cudaStream_t st) {
+template <int MT> int launch_few(const TokenArgs& a, cudaStream_t st) {
   static std::atomic<int> allowed[MAX_SMEM_DEVICES];
   I8L_CUDA_OK(allow_smem(few_rows_kernel<MT>, allowed, FEW_SMEM));
-  const int64_t segments = a.offsets ? (a.experts < a.rows ? a.experts : a.rows) : 1;
-  I8L_CUDA_OK(launch(few_rows_kernel<MT>, dim3((unsigned)((a.N + FEW_COLS - 1) / FEW_COLS), (unsigned)segments), FEW_THREADS, (size_t)(MT * a.K), st,
-                     a, xq, xs));
+  const int64_t segments = a.experts < a.rows ? a.experts : a.rows;
+  const int64_t blocks = (segments * a.N / FEW_COLS + FEW_WARPS - 1) / FEW_WARPS, resident = 2 * sm_count();
+  few_rows_kernel<MT><<<(unsigned)(blocks < resident ? blocks : resident), FEW_THREADS, MT * a.K, st>>>(a);
+  I8L_CUDA_OK(cudaGetLastError());
   return I8L_OK;
 }
 
@@ -585,7 +651,7 @@ template <int TOK> int launch_group(const int8_t* xq, GroupArgs& p, cudaStream_t
 using namespace i8l;
 
 extern "C" int64_t i8l_token_linear_workspace(int64_t rows, int64_t K) {
-  if (rows <= 0 || K <= 0 || rows >= (1ll << 31) || K > MAX_K) return 0;
+  if (rows <= 0 || K <= 0 || rows >= (1ll << 31) || K > MAX_K || few_rows(rows, K)) return 0;
   return (rows * K + 255) / 256 * 256 + (4 * rows + 255) / 256 * 256;
 }
 
@@ -611,17 +677,17 @@ extern "C" int i8l_token_linear(const void* x, const int8_t* w_q, const float* w
   a.bias = static_cast<const __nv_bfloat16*>(bias); a.y = y;
   a.rows = rows; a.N = N; a.K = K; a.experts = experts; a.out_f32 = (flags & I8L_GEMM_OUT_F32) ? 1 : 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (few_rows(rows, K)) {
+    case 1: return launch_few<1>(a, st);
+    case 2: return launch_few<2>(a, st);
+    case 4: return launch_few<4>(a, st);
+    case 8: return launch_few<8>(a, st);
+  }
   int8_t* xq = static_cast<int8_t*>(workspace);
   float* xs = reinterpret_cast<float*>(xq + (rows * K + 255) / 256 * 256);
   const LaunchChain chain(st);
   if (int e = quant_token_rows(x, rows, K, xq, xs, st)) return e;
   (void)chain_first();
-  switch (few_rows(rows, K)) {
-    case 1: return launch_few<1>(a, xq, xs, st);
-    case 2: return launch_few<2>(a, xq, xs, st);
-    case 4: return launch_few<4>(a, xq, xs, st);
-    case 8: return launch_few<8>(a, xq, xs, st);
-  }
   GroupArgs p{};
   p.t = a;
   p.xs = xs;
