@@ -368,7 +368,7 @@ I8L_API int i8l_combine_backward(const void* rows, const void* weights, const in
  * 16-byte aligned.  workspace: i8l_token_linear_workspace bytes, 256-byte aligned, may be NULL where that is 0.
  * The row and channel scales are those of the reference's double_channel variant (triton/double-channle_fwd32.py:295-311).
  */
-I8L_API int64_t i8l_token_linear_workspace(int64_t rows, int64_t K);
+I8L_API int64_t i8l_token_linear_workspace(int64_t rows, int experts, int64_t N, int64_t K);
 I8L_API int i8l_token_linear(const void* x, const int8_t* w_q, const float* w_scale, const int32_t* offsets, const void* bias,
                    void* y, int64_t rows, int experts, int64_t N, int64_t K, int flags, void* workspace,
                    int64_t workspace_bytes, int32_t* status, void* stream);

@@ -86,10 +86,11 @@ def test_workspace_sizes(lib):
     assert lib.i8l_sort_workspace(512, 2, 8) == 0                      # few choices need none
     assert lib.i8l_sort_workspace(513, 2, 8) == 5 * 8 * 4              # chunks of 256 choices
     assert lib.i8l_sort_workspace(1 << 20, 8, 1024) == 16 * 1024 * 4
-    assert lib.i8l_token_linear_workspace(9, 48) == 512 + 256
-    assert lib.i8l_token_linear_workspace(8, 48) == 0                  # few rows: one launch
-    assert lib.i8l_token_linear_workspace(1, 131072) == 131072 + 256   # but long ones
-    assert lib.i8l_token_linear_workspace(0, 48) == 0
+    assert lib.i8l_token_linear_workspace(9, 1, 8, 48) == 512 + 256
+    assert lib.i8l_token_linear_workspace(8, 1, 8, 48) == 0                     # few rows: one launch
+    assert lib.i8l_token_linear_workspace(1, 1, 8, 131072) == 131072 + 256      # but long ones
+    assert lib.i8l_token_linear_workspace(8, 1, 11008, 4096) == 32768 + 256     # and more than four on many weights
+    assert lib.i8l_token_linear_workspace(0, 1, 8, 48) == 0
 
 
 def test_wrappers_refuse_what_the_kernels_do_not_take():

@@ -38,6 +38,7 @@ DENSE = [   # rows, N, K: one row to many, sizes that fill no tile
     (1, 8, 16), (1, 4096, 4096), (2, 1000, 2048), (3, 40, 48), (5, 136, 4112), (8, 256, 11008), (9, 264, 144), (16, 128, 128), (17, 1408, 1040),
     (33, 128, 112), (63, 520, 512), (64, 64, 64), (65, 72, 2064), (127, 384, 256), (128, 128, 128), (129, 136, 144), (255, 1000, 272), (257, 264, 400),
     (300, 128, 16), (1000, 2176, 1408), (2048, 512, 1024), (1, 64, 131072), (4, 72, 81936), (40, 72, 40976),
+    (20, 200, 2064), (50, 1288, 2304), (100, 3016, 3200), (64, 1024, 4096), (65, 1024, 4096), (129, 2048, 3088),   # K shared by a cluster
 ]
 
 
@@ -56,7 +57,7 @@ def test_dense(R, N, Kd, with_bias):
 GROUPED = [   # rows of each expert, rows behind the last one, N, K
     ([1], 0, 64, 128), ([0, 1, 0, 1], 0, 4096, 1024), ([0, 0, 0], 3, 64, 48), ([2, 0, 5, 1], 2, 136, 208), ([8], 1, 96, 256), ([9, 0, 7], 0, 128, 144),
     ([64, 1, 0, 65, 16], 5, 264, 400), ([100] * 12, 0, 72, 128), ([0, 0, 700], 130, 128, 256), ([255, 256, 257, 1], 0, 320, 384),
-    ([128, 384, 0, 128], 128, 256, 512), ([513, 31, 2000], 77, 1000, 272), ([1] * 60, 4, 40, 64), ([0] * 1000 + [3, 0, 40] + [0] * 21, 1, 24, 112),
+    ([128, 384, 0, 128], 128, 256, 512), ([513, 31, 2000], 77, 1000, 272), ([1] * 60, 4, 40, 64), ([5, 0, 30, 1], 2, 136, 2080), ([9, 64, 0, 70], 3, 264, 4112), ([0, 33], 0, 3000, 3200), ([0] * 1000 + [3, 0, 40] + [0] * 21, 1, 24, 112),
 ]
 
 
@@ -208,7 +209,8 @@ def test_elements_beyond_32_bits():
     assert y.numel() > 2 ** 31 and torch.equal(y[pick].cpu(), _plain(x[pick], wq, ws, None).to(BF16))
 
 
-@pytest.mark.parametrize("R,E,N,Kd", [(200, 1, 2048, 512), (3000, 4, 1000, 272), (3000, 4, 20000, 272)])
+@pytest.mark.parametrize("R,E,N,Kd", [(200, 1, 2048, 512), (3000, 4, 1000, 272), (3000, 4, 20000, 272), (20, 1, 200, 2064), (50, 1, 1288, 2304),
+                                      (100, 2, 1504, 3200), (60, 2, 40, 9008)])
 def test_wait_that_runs_out_and_the_next_call(R, E, N, Kd):
     """A withheld load: the kernel returns, the status word says so, the next call is right (see test_timeout_gpu.py)."""
     from triton_int8_b200 import _lib as L

@@ -53,7 +53,7 @@ SIGNATURES = {
     "i8l_sort_tokens": [_P, _P, _I, _I64, _I64, _I, _I, _I64, _I, _I64, _P, _P, _P, _P, _P, _I64, _P],
     "i8l_combine": [_P, _P, _P, _I64, _I64, _I64, _I, _I, _I, _P, _P],
     "i8l_combine_backward": [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I, _I, _I, _P, _P, _P],
-    "i8l_token_linear_workspace": [_I64, _I64],
+    "i8l_token_linear_workspace": [_I64, _I, _I64, _I64],
     "i8l_token_linear": [_P, _P, _P, _P, _P, _P, _I64, _I, _I64, _I64, _I, _P, _I64, _P, _P],
 }
 

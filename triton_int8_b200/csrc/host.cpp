@@ -384,7 +384,7 @@ Tensor token_linear(const Tensor& x, const Tensor& wq, const Tensor& ws, const T
   auto shape = x.sizes().vec();
   shape.back() = N;
   Tensor y = at::empty(shape, x.options().dtype(f32 ? at::kFloat : at::kBFloat16));
-  const int64_t size = lib_token_workspace(R, K);
+  const int64_t size = lib_token_workspace(R, (int)E, N, K);
   const Tensor work = size ? bytes(size, x) : Tensor();
   check("i8l_token_linear",
         lib_token_linear(x.data_ptr(), at_of<int8_t>(wq), at_of<float>(ws), offsets.defined() ? at_of<int32_t>(offsets) : nullptr,

@@ -43,32 +43,126 @@ __device__ __forceinline__ uint4 load_weights(const int8_t* p) {   // read once:
 }
 
 // ------------------------------------------------------------------------------------------ few rows
-// Up to eight rows in one launch: every block quantizes them into its shared memory, then its warps go through the channels of the
-// experts that have rows, two at a time, and multiply the weights by dp4a.  Bound by the weights' bytes, so it is the loads that
-// matter: while a warp works on a batch (2 KB of each of its two channels, eight loads of 16 bytes a lane) the next one is in flight,
-// across channels and experts, and the first goes out ahead of the quantization.
-constexpr int FEW_THREADS = 256, FEW_WARPS = FEW_THREADS / 32, FEW_COLS = 2, FEW_STEPS = 4, FEW_BATCH = FEW_STEPS * 512, FEW_ROWS = 8;
-
+// Up to eight rows in one launch, bound by the weights' bytes.  Two kernels share the frame: every block quantizes the rows into its shared
+// memory and then goes through channels of the experts that have rows, resident blocks over all of them, with loads from memory
+// straight into registers, the next batch in flight while one is multiplied and the next channels on their way into L2; the first
+// batch goes out ahead of the quantization.  (Set-up and drain of tcgen05 take longer than these products.)
+constexpr int FEW_THREADS = 256, FEW_WARPS = FEW_THREADS / 32, FEW_ROWS = 8;
 struct FewSegment {
   int expert, row, rows;
 };
-struct Batch {
-  uint4 w[FEW_COLS][FEW_STEPS];
+struct FewShared {
+  float scale[FEW_ROWS], red[FEW_WARPS];
+  FewSegment seg[FEW_ROWS];
+  int segments;
+};
+
+// The experts that have rows, at most as many as rows.
+__device__ __forceinline__ void few_segments(const TokenArgs& a, FewShared& sh) {
+  const int lane = threadIdx.x & 31;
+  if (!a.offsets) {
+    if (threadIdx.x == 0) {
+      sh.seg[0] = FewSegment{0, 0, (int)a.rows};
+      sh.segments = 1;
+    }
+  } else if (threadIdx.x < 32) {
+    int count = 0;
+    for (int e0 = 0; e0 < a.experts; e0 += 32) {
+      int64_t begin = 0, end = 0;
+      if (e0 + lane < a.experts) segment(a, e0 + lane, begin, end);
+      const unsigned set = __ballot_sync(0xffffffffu, end > begin);
+      const int at = count + __popc(set & ((1u << lane) - 1));
+      if (end > begin && at < FEW_ROWS) sh.seg[at] = FewSegment{e0 + lane, (int)begin, (int)(end - begin)};
+      count += __popc(set);
+    }
+    if (lane == 0) sh.segments = count < FEW_ROWS ? count : FEW_ROWS;   // more only where offsets decrease
+  }
+  __syncthreads();
+}
+// All rows in int8, `stride` bytes apart, zeros behind K, and a scale each; as many threads a row as there are for a power of two rows.
+__device__ __forceinline__ void few_quantize(const TokenArgs& a, FewShared& sh, int8_t* xq, int stride) {
+  const int rows = (int)a.rows, pieces = (int)a.K / 8, lanes = rows == 1 ? 256 : rows == 2 ? 128 : rows <= 4 ? 64 : 32;
+  const int t = threadIdx.x / lanes, l = threadIdx.x & (lanes - 1);
+  const bool live = t < rows;
+  const uint4* row = reinterpret_cast<const uint4*>(a.x + t * a.K);
+  float m = 0.f;
+  if (live)
+#pragma unroll 4
+    for (int c = l; c < pieces; c += lanes) {
+      float v[8];
+      unpack8(row[c], v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[i]));
+    }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((threadIdx.x & 31) == 0) sh.red[threadIdx.x >> 5] = m;
+  __syncthreads();
+  for (int i = 0; i < lanes / 32; ++i) m = fmaxf(m, sh.red[t * (lanes / 32) + i]);
+  float s, stored;
+  make_scale<I8L_QMODE_ROWRCP>(m, s, stored);
+  if (live && l == 0) sh.scale[t] = stored;
+  uint2* q = reinterpret_cast<uint2*>(xq + t * stride);
+  if (live)
+#pragma unroll 4
+    for (int c = l; c < stride / 8; c += lanes) q[c] = c < pieces ? quant_piece<I8L_QMODE_ROWRCP>(row[c], s) : make_uint2(0, 0);
+  __syncthreads();
+}
+__device__ __forceinline__ void few_store(const TokenArgs& a, const FewShared& sh, const FewSegment& seg, int r, int64_t n, int sum) {
+  const int64_t c = (int64_t)seg.expert * a.N + n, at = (int64_t)(seg.row + r) * a.N + n;
+  float v = __fmul_rn(__fmul_rn(__int2float_rn(sum), sh.scale[seg.row + r]), a.ws[c]);
+  if (a.bias) v = __fadd_rn(v, __bfloat162float(a.bias[c]));
+  if (a.out_f32) static_cast<float*>(a.y)[at] = v;
+  else static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(v);
+}
+__device__ __forceinline__ void few_clear(const TokenArgs& a, const FewShared& sh) {   // rows of no expert
+  const int64_t pieces = a.N * (a.out_f32 ? 4 : 2) / 16;
+  for (int64_t r = 0; a.offsets && r < a.rows; ++r) {
+    bool some = false;
+    for (int i = 0; i < sh.segments; ++i) some |= r >= sh.seg[i].row && r < sh.seg[i].row + sh.seg[i].rows;
+    if (some) continue;
+    for (int64_t c = (int64_t)blockIdx.x * FEW_THREADS + threadIdx.x; c < pieces; c += (int64_t)gridDim.x * FEW_THREADS)
+      static_cast<uint4*>(a.y)[r * pieces + c] = make_uint4(0, 0, 0, 0);
+  }
+}
+// Where a warp is: channels from n on of segment `seg`, of K from `k` on.
+struct FewPlace {
+  int seg, k;
+  int64_t n;
+};
+__device__ __forceinline__ void few_settle(FewPlace& p, int segments, int64_t channels) {   // into the segment that n belongs to
+  while (p.seg < segments && p.n >= channels) {
+    p.n -= channels;
+    ++p.seg;
+  }
+}
+__device__ __forceinline__ void fetch_l2(const TokenArgs& a, const FewShared& sh, const FewPlace& p, int channels) {   // by one thread
+  const int64_t some = a.N - p.n < channels ? a.N - p.n : channels;
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a.wq + ((int64_t)sh.seg[p.seg].expert * a.N + p.n) * a.K), "r"((uint32_t)(some * a.K))
+               : "memory");
+}
+
+// Up to four rows: a warp takes two channels at a time over all of K, 512 bytes of each a load, and multiplies by dp4a; a batch is 2 KB of
+// each.  11008x4096: one row 9.3 us, two 9.8, four 12.2 (without the fetch into L2 11.5, 12.1, 13.8); 4096x4096 4.4, 5.0, 6.7;
+// one token x 2 of 8 experts of 11008x4096 17.9 (14 of bytes).
+constexpr int DP_CHANNELS = 2, DP_STEPS = 4, DP_BATCH = DP_STEPS * 512;
+struct DpBatch {
+  uint4 w[DP_CHANNELS][DP_STEPS];
 };
 template <int MT, int CT>
-__device__ __forceinline__ void multiply_batch(int (&acc)[FEW_COLS][MT], const Batch& w, const int8_t* rows, int count, int K, int limit, int k0) {
+__device__ __forceinline__ void dp_multiply(int (&acc)[DP_CHANNELS][MT], const DpBatch& w, const int8_t* rows, int count, int K, int limit, int k0) {
   int at[CT];   // of a row: CT may be above their number, and what is multiplied with the first one once more is not used
 #pragma unroll
   for (int t = 0; t < CT; ++t) at[t] = t < count ? t * K : 0;
 #pragma unroll
-  for (int s = 0; s < FEW_STEPS; ++s) {
+  for (int s = 0; s < DP_STEPS; ++s) {
     const int k = k0 + s * 512;
     if (k >= limit) break;
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
       const uint4 v = *reinterpret_cast<const uint4*>(rows + at[t] + k);
 #pragma unroll
-      for (int j = 0; j < FEW_COLS; ++j) {
+      for (int j = 0; j < DP_CHANNELS; ++j) {
         acc[j][t] = __dp4a((int)w.w[j][s].x, (int)v.x, acc[j][t]);
         acc[j][t] = __dp4a((int)w.w[j][s].y, (int)v.y, acc[j][t]);
         acc[j][t] = __dp4a((int)w.w[j][s].z, (int)v.z, acc[j][t]);
@@ -79,128 +173,72 @@ __device__ __forceinline__ void multiply_batch(int (&acc)[FEW_COLS][MT], const B
 }
 
 template <int MT>
-__global__ void __launch_bounds__(FEW_THREADS, 2) few_rows_kernel(const TokenArgs a) {
+__global__ void __launch_bounds__(FEW_THREADS, 2) few_dp_kernel(const TokenArgs a) {
   extern __shared__ __align__(16) int8_t xq[];   // [MT, K]
-  __shared__ float xs[MT], red[FEW_WARPS];
-  __shared__ FewSegment s_seg[FEW_ROWS];
-  __shared__ int s_segments;
-  constexpr int LANES = FEW_THREADS / MT;        // threads that quantize a row
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = (int)a.K;
-  if (a.offsets) {   // the experts that have rows, at most as many as rows
-    if (warp == 0) {
-      int count = 0;
-      for (int e0 = 0; e0 < a.experts; e0 += 32) {
-        int64_t begin = 0, end = 0;
-        if (e0 + lane < a.experts) segment(a, e0 + lane, begin, end);
-        const unsigned set = __ballot_sync(0xffffffffu, end > begin);
-        const int at = count + __popc(set & ((1u << lane) - 1));
-        if (end > begin && at < FEW_ROWS) s_seg[at] = FewSegment{e0 + lane, (int)begin, (int)(end - begin)};
-        count += __popc(set);
-      }
-      if (lane == 0) s_segments = count < FEW_ROWS ? count : FEW_ROWS;   // more only where offsets decrease
-    }
-  } else if (tid == 0) {
-    s_seg[0] = FewSegment{0, 0, (int)a.rows};
-    s_segments = 1;
-  }
-  __syncthreads();
-
-  // Where a warp is: channels n and n + 1 of segment `seg`, K from k on.
-  const int64_t step = (int64_t)gridDim.x * FEW_WARPS * FEW_COLS;
-  struct Place {
-    int seg, k;
-    int64_t n;
-  };
-  const int segments = s_segments;
-  auto settle = [&](Place& p) {   // into the segment that its channels belong to
-    while (p.seg < segments && p.n >= a.N) {
-      p.n -= a.N;
-      ++p.seg;
-    }
-  };
-  auto load = [&](Batch& b, const Place& p) {
+  __shared__ FewShared sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, K = (int)a.K;
+  chain_wait();   // launched ahead of its predecessor's end, as the first kernels of the other calls are
+  chain_trigger();
+  few_segments(a, sh);
+  const int segments = sh.segments;
+  const int64_t step = (int64_t)gridDim.x * FEW_WARPS * DP_CHANNELS;
+  auto load = [&](DpBatch& b, const FewPlace& p) {
     if (p.seg >= segments) return;
-    const int8_t* w = a.wq + ((int64_t)s_seg[p.seg].expert * a.N + p.n) * a.K + lane * 16;
+    const int8_t* w = a.wq + ((int64_t)sh.seg[p.seg].expert * a.N + p.n) * a.K + lane * 16;
 #pragma unroll
-    for (int s = 0; s < FEW_STEPS; ++s)
+    for (int s = 0; s < DP_STEPS; ++s)
 #pragma unroll
-      for (int j = 0; j < FEW_COLS; ++j)
+      for (int j = 0; j < DP_CHANNELS; ++j)   // N is a multiple of 8: both channels or none
         if (p.k + s * 512 + lane * 16 < K) b.w[j][s] = load_weights(w + (int64_t)j * K + p.k + s * 512);
   };
-  Place now{0, 0, ((int64_t)warp * gridDim.x + blockIdx.x) * FEW_COLS};
-  settle(now);
-  Batch even, odd;
+  auto after = [&](FewPlace p) {
+    p.n += step;
+    few_settle(p, segments, a.N);
+    return p;
+  };
+  FewPlace now{0, 0, ((int64_t)warp * gridDim.x + blockIdx.x) * DP_CHANNELS};
+  few_settle(now, segments, a.N);
+  DpBatch even, odd;
   load(even, now);
+  FewPlace fetched = now;
+  if (lane == 0 && fetched.seg < segments) fetch_l2(a, sh, fetched, DP_CHANNELS);   // the rest of these, and the next
+  fetched = after(fetched);
+  if (lane == 0 && fetched.seg < segments) fetch_l2(a, sh, fetched, DP_CHANNELS);
+  few_quantize(a, sh, xq, K);
 
-  {   // the rows in int8, a scale each
-    const int t = tid / LANES, l = tid & (LANES - 1);
-    const bool live = t < a.rows;
-    const uint4* row = reinterpret_cast<const uint4*>(a.x + t * a.K);
-    float m = 0.f;
-    if (live)
-#pragma unroll 4
-      for (int c = l; c < K / 8; c += LANES) {
-        float v[8];
-        unpack8(row[c], v);
+  int acc[DP_CHANNELS][MT];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[i]));
-      }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) red[warp] = m;
-    __syncthreads();
-    m = red[t * (LANES / 32)];
-#pragma unroll
-    for (int i = 1; i < LANES / 32; ++i) m = fmaxf(m, red[t * (LANES / 32) + i]);
-    float s, stored;
-    make_scale<I8L_QMODE_ROWRCP>(m, s, stored);
-    if (l == 0) xs[t] = stored;
-    uint2* q = reinterpret_cast<uint2*>(xq + t * K);
-#pragma unroll 4
-    for (int c = l; c < K / 8; c += LANES) q[c] = live ? quant_piece<I8L_QMODE_ROWRCP>(row[c], s) : make_uint2(0, 0);
-    __syncthreads();
-  }
-
-  int acc[FEW_COLS][MT];
-#pragma unroll
-  for (int j = 0; j < FEW_COLS; ++j)
+  for (int j = 0; j < DP_CHANNELS; ++j)
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[j][t] = 0;
-  auto work = [&](Batch& mine, Batch& ahead) {
-    Place next = now;
-    next.k += FEW_BATCH;
+  auto work = [&](const DpBatch& mine, DpBatch& ahead) {
+    FewPlace next = now;
+    next.k += DP_BATCH;
     const bool last = next.k >= K;
     if (last) {
+      next = after(now);
       next.k = 0;
-      next.n += step;
-      settle(next);
+      fetched = after(fetched);
+      if (lane == 0 && fetched.seg < segments) fetch_l2(a, sh, fetched, DP_CHANNELS);
     }
     load(ahead, next);
-    const FewSegment seg = s_seg[now.seg];
-    const int8_t* rows = xq + (int64_t)seg.row * K + lane * 16;
+    const FewSegment seg = sh.seg[now.seg];
+    const int8_t* rows = xq + seg.row * K + lane * 16;
     const int limit = K - lane * 16;   // of k, so that the lane's 16 bytes are inside the row
-    if (MT == 1 || seg.rows == 1) multiply_batch<MT, 1>(acc, mine, rows, seg.rows, K, limit, now.k);
-    else if (MT == 2 || seg.rows == 2) multiply_batch<MT, MT < 2 ? MT : 2>(acc, mine, rows, seg.rows, K, limit, now.k);
-    else if (MT == 4 || seg.rows <= 4) multiply_batch<MT, MT < 4 ? MT : 4>(acc, mine, rows, seg.rows, K, limit, now.k);
-    else multiply_batch<MT, MT>(acc, mine, rows, seg.rows, K, limit, now.k);
+    if (MT == 1 || seg.rows == 1) dp_multiply<MT, 1>(acc, mine, rows, seg.rows, K, limit, now.k);
+    else if (MT == 2 || seg.rows == 2) dp_multiply<MT, MT < 2 ? MT : 2>(acc, mine, rows, seg.rows, K, limit, now.k);
+    else dp_multiply<MT, MT>(acc, mine, rows, seg.rows, K, limit, now.k);
     if (last) {
       int sum = 0;   // lane j * MT + t has that of channel j and row t
 #pragma unroll
-      for (int j = 0; j < FEW_COLS; ++j)
+      for (int j = 0; j < DP_CHANNELS; ++j)
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
           const int all = __reduce_add_sync(0xffffffffu, acc[j][t]);
           if (lane == j * MT + t) sum = all;
           acc[j][t] = 0;
         }
-      const int j = lane / MT, t = lane % MT;
-      if (j < FEW_COLS && t < seg.rows) {
-        const int64_t c = (int64_t)seg.expert * a.N + now.n + j, at = (int64_t)(seg.row + t) * a.N + now.n + j;
-        float v = __fmul_rn(__fmul_rn(__int2float_rn(sum), xs[seg.row + t]), a.ws[c]);
-        if (a.bias) v = __fadd_rn(v, __bfloat162float(a.bias[c]));
-        if (a.out_f32) static_cast<float*>(a.y)[at] = v;
-        else static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(v);
-      }
+      if (lane < DP_CHANNELS * MT && lane % MT < seg.rows) few_store(a, sh, seg, lane % MT, now.n + lane / MT, sum);
     }
     now = next;
   };
@@ -209,16 +247,110 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_rows_kernel(const TokenArg
     if (now.seg >= segments) break;
     work(odd, even);
   }
-  if (a.offsets) {   // rows of no expert
-    const int64_t pieces = a.N * (a.out_f32 ? 4 : 2) / 16;
-    for (int64_t r = 0; r < a.rows; ++r) {
-      bool some = false;
-      for (int i = 0; i < segments; ++i) some |= r >= s_seg[i].row && r < s_seg[i].row + s_seg[i].rows;
-      if (some) continue;
-      for (int64_t c = (int64_t)blockIdx.x * FEW_THREADS + tid; c < pieces; c += (int64_t)gridDim.x * FEW_THREADS)
-        static_cast<uint4*>(a.y)[r * pieces + c] = make_uint4(0, 0, 0, 0);
+  few_clear(a, sh);
+}
+
+// Five to eight rows, which dp4a is too slow for: a block takes 16 channels at a time, its warps split K into pieces of 128 and multiply by
+// mma.sync m16n8k32, channels times rows.  The order of K inside a product does not matter, so a lane's 16 contiguous bytes serve
+// as its fragments as they are, for weights and rows alike.  8 rows x 11008x4096 13.8 us, 4096x4096 8.8, 1024x1024 3.8 (dp4a 17.9, 9.8,
+// 3.9; one row 10.8, 5.7, 3.3 against 9.3, 4.4, 2.8: lines of four rows a load and the sum over the warps cost more there).
+constexpr int MMA_CHANNELS = 16, MMA_K = 128, MMA_PIECES = 2;
+struct MmaBatch {
+  uint4 w[MMA_PIECES][2][2];   // piece of K, channel g or g + 8, half of the piece
+};
+__device__ __forceinline__ void mma_16x8x32(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__global__ void __launch_bounds__(FEW_THREADS, 2) few_mma_kernel(const TokenArgs a, int row_bytes) {
+  extern __shared__ __align__(16) int8_t xq[];   // [rows, row_bytes]: K rounded up to whole pieces
+  __shared__ FewShared sh;
+  __shared__ __align__(16) int part[2][FEW_WARPS][MMA_CHANNELS * FEW_ROWS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = (int)a.K, stride = FEW_WARPS * MMA_K;   // of a warp's pieces
+  const int g = lane >> 2, byte = (lane & 3) * 16;   // the lane's channel (and g + 8) or row, its bytes of half a piece
+  chain_wait();
+  chain_trigger();
+  few_segments(a, sh);
+  const int segments = sh.segments;
+  const int64_t step = (int64_t)gridDim.x * MMA_CHANNELS, width = (a.N + MMA_CHANNELS - 1) / MMA_CHANNELS * MMA_CHANNELS;
+  auto load = [&](MmaBatch& b, const FewPlace& p) {
+    if (p.seg >= segments) return;
+    const int8_t* w = a.wq + ((int64_t)sh.seg[p.seg].expert * a.N + p.n + g) * a.K;
+#pragma unroll
+    for (int i = 0; i < MMA_PIECES; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int k = p.k + warp * MMA_K + i * stride + c * 64 + byte;
+          b.w[i][h][c] = k < K && p.n + g + h * 8 < a.N ? load_weights(w + h * 8 * a.K + k) : make_uint4(0, 0, 0, 0);
+        }
+  };
+  auto after = [&](FewPlace p) {
+    p.n += step;
+    few_settle(p, segments, width);
+    return p;
+  };
+  FewPlace now{0, 0, (int64_t)blockIdx.x * MMA_CHANNELS};   // the same for all warps of the block
+  few_settle(now, segments, width);
+  MmaBatch even, odd;
+  load(even, now);
+  FewPlace fetched = now;
+  if (tid == 0 && fetched.seg < segments) fetch_l2(a, sh, fetched, MMA_CHANNELS);   // the rest of these, and the next
+  fetched = after(fetched);
+  if (tid == 0 && fetched.seg < segments) fetch_l2(a, sh, fetched, MMA_CHANNELS);
+  few_quantize(a, sh, xq, row_bytes);
+
+  int acc[4] = {0, 0, 0, 0}, turn = 0;
+  auto work = [&](const MmaBatch& mine, MmaBatch& ahead) {
+    FewPlace next = now;
+    next.k += MMA_PIECES * stride;
+    const bool last = next.k >= row_bytes;
+    if (last) {
+      next = after(now);
+      next.k = 0;
+      fetched = after(fetched);
+      if (tid == 0 && fetched.seg < segments) fetch_l2(a, sh, fetched, MMA_CHANNELS);
     }
+    load(ahead, next);
+    const FewSegment seg = sh.seg[now.seg];
+    const int8_t* row = xq + (seg.row + (g < seg.rows ? g : 0)) * row_bytes + byte;   // rows past the segment's: some row, not used
+#pragma unroll
+    for (int i = 0; i < MMA_PIECES; ++i) {
+      const int k = now.k + warp * MMA_K + i * stride;
+      if (k >= row_bytes) break;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const uint4 x = *reinterpret_cast<const uint4*>(row + k + c * 64), &u = mine.w[i][0][c], &v = mine.w[i][1][c];
+        mma_16x8x32(acc, u.x, v.x, u.y, v.y, x.x, x.y);
+        mma_16x8x32(acc, u.z, v.z, u.w, v.w, x.z, x.w);
+      }
+    }
+    if (last) {   // the warps' sums are added up; the other buffer is that of the channels before, whose readers may still be at it
+      *reinterpret_cast<int4*>(&part[turn][warp][lane * 4]) = make_int4(acc[0], acc[1], acc[2], acc[3]);
+      acc[0] = acc[1] = acc[2] = acc[3] = 0;
+      __syncthreads();
+      if (tid < MMA_CHANNELS * FEW_ROWS) {
+        int sum = 0;
+#pragma unroll
+        for (int w = 0; w < FEW_WARPS; ++w) sum += part[turn][w][tid];
+        // as mma.sync leaves them: lane l has channels l / 4 (and + 8 in the upper two), rows 2 * (l % 4) and the next one
+        const int from = tid >> 2, r = (from & 3) * 2 + (tid & 1);
+        const int64_t n = now.n + (from >> 2) + (tid & 2) * 4;
+        if (r < seg.rows && n < a.N) few_store(a, sh, seg, r, n, sum);
+      }
+      turn ^= 1;
+    }
+    now = next;
+  };
+  while (now.seg < segments) {
+    work(even, odd);
+    if (now.seg >= segments) break;
+    work(odd, even);
   }
+  few_clear(a, sh);
 }
 
 // ------------------------------------------------------------------------------------------ many rows
@@ -242,11 +374,11 @@ struct __align__(16) Segment {
   int share;       // tokens of each of its tiles
   int first;       // number of its first tile
 };
-template <int TOK> struct Grp {
-  static constexpr int STAGES = TOK == 256 ? 4 : TOK == 128 ? 6 : 8, BUFS = 512 / TOK < 4 ? 512 / TOK : 4, COLUMNS = BUFS * TOK;
+template <int TOK, int SPLIT> struct Grp {
+  static constexpr int STAGES = TOK == 256 ? 4 : TOK == 128 ? 6 : SPLIT > 1 ? 7 : 8, BUFS = 512 / TOK < 4 ? 512 / TOK : 4, COLUMNS = BUFS * TOK;
   static constexpr int B_BYTES = TOK * KBYTES;
   static constexpr int RING = STAGES * (A_BYTES + B_BYTES);
-  static constexpr int TABLE = RING + GRP_EPI_WARPS * EPI_BYTES;   // then experts + 1 segments
+  static constexpr int TABLE = RING + (SPLIT > 1 ? TOK * CHANNELS * 4 : GRP_EPI_WARPS * EPI_BYTES);   // then experts + 1 segments
   static int smem(int experts) { return TABLE + (experts + 1) * (int)sizeof(Segment) + 1024; }
 };
 
@@ -258,7 +390,7 @@ struct GroupArgs {
   int n_tiles, withhold;
 };
 struct __align__(16) GroupCtl {
-  uint64_t full[8], empty[8], tfull[4], tempty[4], done;
+  uint64_t full[8], empty[8], tfull[4], tempty[4], done, ready, freed;
   int abort_flag;
   uint32_t tmem_base, by[RASTER + 1];
   __align__(16) float scale[GRP_EPI_WARPS][32];   // of the tokens that a warp takes out, read four at a time
@@ -314,10 +446,35 @@ __device__ __forceinline__ Tile tile_of(int t, const GroupArgs& p, const Segment
   return r;
 }
 
-template <int TOK>
+// Waits for arrivals from the cluster's CTAs: what they wrote before them is visible behind it.  Bounded like the others; once the flag is
+// set it gives up after one poll.
+__device__ __forceinline__ void wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t max_polls) {
+  for (uint32_t i = 0; i < max_polls; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok || *abort_flag) return;
+  }
+  *abort_flag = 1;
+}
+__device__ __forceinline__ void store_remote(uint32_t at, int v) { asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
+__device__ __forceinline__ int4 load_remote(uint32_t at) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+
+// SPLIT > 1: the CTAs of a cluster share a tile, each takes its part of K; the int32 sums meet in shared memory (integers: their order does
+// not show), and each CTA finishes its share of the tokens.
+template <int TOK, int SPLIT>
 __global__ void __launch_bounds__(GRP_THREADS, 1)
 group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ TokenMaps map_x, const GroupArgs p) {
-  using G = Grp<TOK>;
+  using G = Grp<TOK, SPLIT>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ GroupCtl ctl;
   uint8_t* const smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -337,6 +494,8 @@ group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
       mbar_init(smem_u32(&ctl.tempty[b]), GRP_EPI_WARPS);
     }
     mbar_init(smem_u32(&ctl.done), 1);
+    mbar_init(smem_u32(&ctl.ready), SPLIT);
+    mbar_init(smem_u32(&ctl.freed), SPLIT);
     ctl.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -374,8 +533,11 @@ group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     }
   }
   __syncthreads();
+  if (SPLIT > 1) cluster_sync_all();   // the others' barriers are initialised before anything arrives on them
   const uint32_t tmem_base = ctl.tmem_base;
-  const int total = seg[p.t.experts].first, KB = (int)((p.t.K + KBYTES - 1) / KBYTES);
+  const int total = seg[p.t.experts].first, blocks = (int)((p.t.K + KBYTES - 1) / KBYTES);
+  const int rank = SPLIT > 1 ? (int)cluster_ctarank() : 0, unit = (int)blockIdx.x / SPLIT, units = (int)gridDim.x / SPLIT;
+  const int kb0 = rank * blocks / SPLIT, kb1 = (rank + 1) * blocks / SPLIT;   // this CTA's K blocks
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
@@ -384,31 +546,31 @@ group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     uint32_t ph = 0, issued = 0, issued_ph = 0;   // bit s: a load into stage s is (or was) in flight, with parity
     bool ok = true;
     int ahead = 0;   // K blocks of the first tile whose weights are on their way before the rows have been quantized
-    if ((int)blockIdx.x < total && !p.withhold) {
-      const Tile tile = tile_of<TOK>(blockIdx.x, p, seg, ctl.by);
-      ahead = KB < G::STAGES ? KB : G::STAGES;
+    if (unit < total && !p.withhold) {
+      const Tile tile = tile_of<TOK>(unit, p, seg, ctl.by);
+      ahead = kb1 - kb0 < G::STAGES ? kb1 - kb0 : G::STAGES;
       const uint32_t bytes = A_BYTES + boxes_of(tile.columns).tokens() * KBYTES;
       if (elected)
         for (int kb = 0; kb < ahead; ++kb) {
           mbar_expect_tx(smem_u32(&ctl.full[kb]), bytes);
-          tma_load_2d(smem_a + kb * A_BYTES, &map_w, smem_u32(&ctl.full[kb]), kb * KBYTES, (int)((int64_t)tile.expert * p.t.N) + tile.channel);
+          tma_load_2d(smem_a + kb * A_BYTES, &map_w, smem_u32(&ctl.full[kb]), (kb0 + kb) * KBYTES, (int)((int64_t)tile.expert * p.t.N) + tile.channel);
         }
     }
     chain_wait();
-    for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+    for (int t = unit; t < total && ok; t += units) {
       const Tile tile = tile_of<TOK>(t, p, seg, ctl.by);
       const int w_row = (int)((int64_t)tile.expert * p.t.N) + tile.channel;
       const Boxes box = boxes_of(tile.columns);
       const uint32_t bytes = A_BYTES + box.tokens() * KBYTES;
-      for (int kb = 0; kb < KB; ++kb) {
+      for (int kb = kb0; kb < kb1; ++kb) {
         if (!(ok = mbar_wait(smem_u32(&ctl.empty[s]), ph ^ 1u, abort_flag, p.max_polls))) break;
-        if (p.withhold && t == (int)blockIdx.x && kb == KB - 1) {   // test hook: the waits that depend on this stage run out
+        if (p.withhold && t == unit && kb == kb1 - 1) {   // test hook: the waits that depend on this stage run out
           if (++s == G::STAGES) { s = 0; ph ^= 1u; }
           continue;
         }
         if (elected) {
           const uint32_t bar = smem_u32(&ctl.full[s]);
-          if (t != (int)blockIdx.x || kb >= ahead) {
+          if (t != unit || kb - kb0 >= ahead) {
             mbar_expect_tx(bar, bytes);
             tma_load_2d(smem_a + s * A_BYTES, &map_w, bar, kb * KBYTES, w_row);
           }
@@ -434,18 +596,18 @@ group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     int s = 0, ab = 0;
     uint32_t ph = 0, aph = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+    for (int t = unit; t < total && ok; t += units) {
       const uint32_t idesc = mma_desc(tile_of<TOK>(t, p, seg, ctl.by).columns), d = tmem_base + ab * TOK;
       if (!(ok = mbar_wait(smem_u32(&ctl.tempty[ab]), aph ^ 1u, abort_flag, p.max_polls))) break;
-      for (int kb = 0; kb < KB; ++kb) {
+      for (int kb = kb0; kb < kb1; ++kb) {
         if (!(ok = mbar_wait(smem_u32(&ctl.full[s]), ph, abort_flag, p.max_polls))) break;
         tc_fence_after();
         if (elected) {
           const uint64_t da = smem_desc(smem_a + s * A_BYTES), db = smem_desc(smem_b + s * G::B_BYTES);
 #pragma unroll
-          for (int k4 = 0; k4 < KBYTES / 32; ++k4) tc_mma_i8(d, da + 2 * k4, db + 2 * k4, idesc, (k4 > 0 || kb > 0) ? 1u : 0u);
+          for (int k4 = 0; k4 < KBYTES / 32; ++k4) tc_mma_i8(d, da + 2 * k4, db + 2 * k4, idesc, (k4 > 0 || kb > kb0) ? 1u : 0u);
           tc_commit(smem_u32(&ctl.empty[s]));
-          if (kb == KB - 1) tc_commit(smem_u32(&ctl.tfull[ab]));
+          if (kb == kb1 - 1) tc_commit(smem_u32(&ctl.tfull[ab]));
         }
         __syncwarp();
         if (++s == G::STAGES) { s = 0; ph ^= 1u; }
@@ -468,8 +630,83 @@ group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     // ------------------------------------------------------------------ epilogue
     const int q = warp & 3, half = (warp - 4) >> 2;   // a quarter of the channels, every other 32 tokens
     uint8_t* const turn = smem + G::RING + (warp - 4) * EPI_BYTES;
-    float* const scale = ctl.scale[warp - 4];
     constexpr int PARTS = TOK / 64;   // of 32 tokens
+    if constexpr (SPLIT > 1) {
+      int* const part = reinterpret_cast<int*>(smem + G::RING);   // [tokens, channels]: this CTA's sums
+      const uint32_t part_at = smem_u32(part), ready = smem_u32(&ctl.ready), freed = smem_u32(&ctl.freed);
+      // Once all of this CTA's epilogue warps are here.  None of them leaves the loop early, so that they all come; a CTA that has given up a
+      // wait says so to the others, which store nothing from then on.
+      auto arrive_everywhere = [&](uint32_t bar) {
+        named_sync(1, GRP_EPI_WARPS * 32);
+        if (threadIdx.x - 128 < SPLIT) {
+          if (*abort_flag) store_remote(map_to_cta(smem_u32(&ctl.abort_flag), threadIdx.x - 128), 1);
+          mbar_arrive_cluster(map_to_cta(bar, threadIdx.x - 128));
+        }
+      };
+      int ab = 0;
+      uint32_t aph = 0, ph = 0;
+      chain_wait();
+      for (int t = unit; t < total; t += units, ph ^= 1u) {
+        const Tile tile = tile_of<TOK>(t, p, seg, ctl.by);
+        mbar_wait_or_flag(smem_u32(&ctl.tfull[ab]), aph, abort_flag, p.max_polls);
+        tc_fence_after();
+        wait_cluster(freed, ph ^ 1u, abort_flag, p.max_polls);   // the tile before has been read by all
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+          const int j0 = half * 32 + i * 64;
+          if (j0 >= tile.rows) break;
+          uint32_t r[32];
+          tc_ld16(tmem_base + ((uint32_t)(q * 32) << 16) + ab * TOK + j0, r);
+          tc_ld16(tmem_base + ((uint32_t)(q * 32) << 16) + ab * TOK + j0 + 16, r + 16);
+          tc_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) part[(j0 + j) * CHANNELS + q * 32 + lane] = (int)r[j];
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ctl.tempty[ab]));
+        if (++ab == G::BUFS) { ab = 0; aph ^= 1u; }
+        arrive_everywhere(ready);
+        wait_cluster(ready, ph, abort_flag, p.max_polls);
+        const int from = rank * tile.rows / SPLIT, to = (rank + 1) * tile.rows / SPLIT, n = tile.channel + lane * 4;
+        if (n < p.t.N && !*abort_flag) {   // N is a multiple of 8, n of 4
+          const int64_t c = (int64_t)tile.expert * p.t.N + n;
+          float sw[4], bias[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            sw[i] = p.t.ws[c + i];
+            bias[i] = p.t.bias ? __bfloat162float(p.t.bias[c + i]) : 0.f;
+          }
+          for (int j = from + warp - 4; j < to; j += GRP_EPI_WARPS) {
+            int sum[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int r = 0; r < SPLIT; ++r) {
+              const int4 v = load_remote(map_to_cta(part_at + (j * CHANNELS + lane * 4) * 4, r));
+              sum[0] += v.x;
+              sum[1] += v.y;
+              sum[2] += v.z;
+              sum[3] += v.w;
+            }
+            const float sx = p.xs[tile.row + j];
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              v[i] = __fmul_rn(__fmul_rn(__int2float_rn(sum[i]), sx), sw[i]);
+              if (p.t.bias) v[i] = __fadd_rn(v[i], bias[i]);
+            }
+            const int64_t at = (tile.row + j) * p.t.N + n;
+            if (p.t.out_f32) *reinterpret_cast<float4*>(static_cast<float*>(p.t.y) + at) = make_float4(v[0], v[1], v[2], v[3]);
+            else {
+              const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
+              *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.t.y) + at) =
+                  make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+            }
+          }
+        }
+        arrive_everywhere(freed);
+      }
+    } else {
+    float* const scale = ctl.scale[warp - 4];
     // What a tile needs besides the accumulator: fetched a tile ahead, behind the wait for the one in front.
     struct Ahead {
       Tile tile;
@@ -493,12 +730,12 @@ group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     uint32_t aph = 0;
     chain_wait();
     Ahead next;
-    if ((int)blockIdx.x < total) next = fetch(blockIdx.x);
-    for (int t = blockIdx.x; t < total; t += gridDim.x) {
+    if (unit < total) next = fetch(unit);
+    for (int t = unit; t < total; t += units) {
       const Ahead now = next;
       if (!mbar_wait(smem_u32(&ctl.tfull[ab]), aph, abort_flag, p.max_polls)) break;
       tc_fence_after();
-      if (t + (int)gridDim.x < total) next = fetch(t + gridDim.x);
+      if (t + units < total) next = fetch(t + units);
       const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + ab * TOK;
       const int n = now.tile.channel + q * 32 + lane;
 #pragma unroll
@@ -559,9 +796,11 @@ group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
       if (lane == 0) mbar_arrive(smem_u32(&ctl.tempty[ab]));
       if (++ab == G::BUFS) { ab = 0; aph ^= 1u; }
     }
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if (SPLIT > 1) cluster_sync_all();   // shared memory and barriers outlive the others' use of them
   if (threadIdx.x == 0 && ctl.abort_flag && p.status) {
     atomicExch(p.status, I8L_ERR_TIMEOUT);
     if (p.mirror) {
@@ -576,20 +815,32 @@ group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
 }
 
 // ------------------------------------------------------------------------------------------ host
-// The rows that the kernel for few of them takes at once, 0: too many, or too long for its shared memory.
-constexpr int FEW_SMEM = 64 * 1024;
-int few_rows(int64_t rows, int64_t K) {
-  const int mt = rows == 1 ? 1 : rows == 2 ? 2 : rows <= 4 ? 4 : 8;
-  return rows <= FEW_ROWS && mt * K <= FEW_SMEM ? mt : 0;
+// Whether the kernels for few rows take them: in the shared memory of which two blocks fit on an SM.
+constexpr int FEW_SMEM = 96 * 1024;
+int64_t few_row_bytes(int64_t rows, int64_t K) { return rows <= 4 ? K : (K + MMA_K - 1) / MMA_K * MMA_K; }
+// Above four rows only as long as the weights are few, 2^24 bytes if all rows belong to different experts: 8 rows x 4096x4096 8.9 us here and
+// 11.0 on the tensor cores, but 11008x4096 14.0 and 13.0, 8 of 8 experts of 1408x4096 17.8 and 14.2.
+bool few_rows(int64_t rows, int64_t K, int64_t experts, int64_t N) {
+  if (rows > FEW_ROWS || rows * few_row_bytes(rows, K) > FEW_SMEM) return false;
+  return rows <= 4 || (experts < rows ? experts : rows) * N * K <= 1 << 24;
 }
-template <int MT> int launch_few(const TokenArgs& a, cudaStream_t st) {
-  static std::atomic<int> allowed[MAX_SMEM_DEVICES];
-  I8L_CUDA_OK(allow_smem(few_rows_kernel<MT>, allowed, FEW_SMEM));
-  const int64_t segments = a.experts < a.rows ? a.experts : a.rows;
-  const int64_t blocks = (segments * a.N / FEW_COLS + FEW_WARPS - 1) / FEW_WARPS, resident = 2 * sm_count();
-  few_rows_kernel<MT><<<(unsigned)(blocks < resident ? blocks : resident), FEW_THREADS, MT * a.K, st>>>(a);
-  I8L_CUDA_OK(cudaGetLastError());
+template <typename Kernel, typename... Args>
+int launch_few(Kernel kernel, std::atomic<int>* allowed, const TokenArgs& a, int64_t channels, int warps, cudaStream_t st, Args... args) {
+  I8L_CUDA_OK(allow_smem(kernel, allowed, FEW_SMEM));
+  const int64_t segments = a.experts < a.rows ? a.experts : a.rows, units = segments * ((a.N + channels - 1) / channels);
+  const int64_t blocks = (units + warps - 1) / warps, resident = 2 * sm_count();
+  const LaunchChain chain(st);
+  (void)chain_first();   // it always waits
+  I8L_CUDA_OK(launch(kernel, dim3((unsigned)(blocks < resident ? blocks : resident)), FEW_THREADS, (size_t)(a.rows * few_row_bytes(a.rows, a.K)), st,
+                     a, args...));
   return I8L_OK;
+}
+int run_few(const TokenArgs& a, cudaStream_t st) {
+  static std::atomic<int> allowed[4][MAX_SMEM_DEVICES];
+  if (a.rows == 1) return launch_few(few_dp_kernel<1>, allowed[0], a, DP_CHANNELS, FEW_WARPS, st);
+  if (a.rows == 2) return launch_few(few_dp_kernel<2>, allowed[1], a, DP_CHANNELS, FEW_WARPS, st);
+  if (a.rows <= 4) return launch_few(few_dp_kernel<4>, allowed[2], a, DP_CHANNELS, FEW_WARPS, st);
+  return launch_few(few_mma_kernel, allowed[3], a, MMA_CHANNELS, 1, st, (int)few_row_bytes(a.rows, a.K));
 }
 
 // Tokens of a tile, from what the host knows: as if all rows belonged to experts, and to all alike.  A tile of s columns takes 0.4 + 0.6 *
@@ -620,11 +871,24 @@ int tile_tokens(const TokenArgs& a) {
   return best;
 }
 
-template <int TOK> int launch_group(const int8_t* xq, GroupArgs& p, cudaStream_t st) {
-  using G = Grp<TOK>;
+// CTAs that share a tile of 64 tokens, where there are few tiles and a long K: a share costs 2 us (the sums meet, clusters start later) and
+// saves its part of 0.18 us a K block; clusters of eight find few places.  us with 1, 2, 4 and 8: 9 rows x 512x8192 17.8 / 12.8 /
+// 9.6 / 8.0, 256 rows 18.8 / 14.7 / 11.6 / 17.3; 16 rows x 4096x11008 22.7 / 16.6 / 14.7 / 21.7, 128 rows 24.8 / 19.1 / 25.4 / 34;
+// 64 rows x 1000x2048 9.0 / 9.6 / 8.5 / 8.0, x 2176x1408 8.0 / 9.2 / 8.3 / 14.
+int k_split(const TokenArgs& a) {
+  const int64_t segments = a.experts < a.rows ? a.experts : a.rows, average = (a.rows + segments - 1) / segments;
+  const int64_t tiles = segments * ((average + 63) / 64) * ((a.N + CHANNELS - 1) / CHANNELS), blocks = (a.K + KBYTES - 1) / KBYTES;
+  if (gemm_cta_budget() < sm_count()) return 1;   // some SMs are kept free, and clusters need whole groups of them
+  if (blocks >= 16 && tiles <= 8) return 8;
+  if (blocks >= 16 && tiles <= 32) return 4;
+  return blocks >= 24 && tiles <= 64 ? 2 : 1;
+}
+
+template <int TOK, int SPLIT = 1> int launch_group(const int8_t* xq, GroupArgs& p, cudaStream_t st) {
+  using G = Grp<TOK, SPLIT>;
   static std::atomic<int> allowed[MAX_SMEM_DEVICES];
   const TokenArgs& a = p.t;
-  I8L_CUDA_OK(allow_smem(group_kernel<TOK>, allowed, G::smem(MAX_EXPERTS)));
+  I8L_CUDA_OK(allow_smem(group_kernel<TOK, SPLIT>, allowed, G::smem(MAX_EXPERTS)));
   p.n_tiles = (int)((a.N + CHANNELS - 1) / CHANNELS);
   const int64_t most = (a.rows / TOK + (a.experts < a.rows ? a.experts : a.rows)) * p.n_tiles;   // tiles, whatever the offsets
   if (most >= (1ll << 31)) return fail(I8L_ERR_SHAPE, "i8l_token_linear: too large for 32-bit tile numbers");
@@ -633,15 +897,22 @@ template <int TOK> int launch_group(const int8_t* xq, GroupArgs& p, cudaStream_t
   if (int e = make_tile_map_i8(&mw, a.wq, a.experts * a.N, a.K, CHANNELS)) return e;
   for (int i = 0; i < BOXES; ++i)
     if (int e = make_tile_map_i8(&mx.box[i], xq, a.rows, a.K, 16 << i)) return e;
-  const int budget = gemm_cta_budget();
+  const int64_t budget = gemm_cta_budget() / SPLIT > 0 ? gemm_cta_budget() / SPLIT : 1;
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attrs[1];
-  cfg.gridDim = dim3((unsigned)(most < budget ? most : budget), 1, 1);
+  cudaLaunchAttribute attrs[2];
+  cfg.gridDim = dim3((unsigned)((most < budget ? most : budget) * SPLIT), 1, 1);
   cfg.blockDim = dim3(GRP_THREADS, 1, 1);
   cfg.dynamicSmemBytes = G::smem(a.experts);
   cfg.stream = st;
+  if (SPLIT > 1) {
+    attrs[0].id = cudaLaunchAttributeClusterDimension;
+    attrs[0].val.clusterDim.x = SPLIT;
+    attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
+    cfg.attrs = attrs;
+    cfg.numAttrs = 1;
+  }
   chain_attribute(cfg, attrs);
-  I8L_CUDA_OK(cudaLaunchKernelEx(&cfg, group_kernel<TOK>, mw, mx, p));
+  I8L_CUDA_OK(cudaLaunchKernelEx(&cfg, group_kernel<TOK, SPLIT>, mw, mx, p));
   return I8L_OK;
 }
 
@@ -650,8 +921,8 @@ template <int TOK> int launch_group(const int8_t* xq, GroupArgs& p, cudaStream_t
 
 using namespace i8l;
 
-extern "C" int64_t i8l_token_linear_workspace(int64_t rows, int64_t K) {
-  if (rows <= 0 || K <= 0 || rows >= (1ll << 31) || K > MAX_K || few_rows(rows, K)) return 0;
+extern "C" int64_t i8l_token_linear_workspace(int64_t rows, int experts, int64_t N, int64_t K) {
+  if (rows <= 0 || K <= 0 || N <= 0 || experts <= 0 || rows >= (1ll << 31) || N >= (1ll << 31) || K > MAX_K || few_rows(rows, K, experts, N)) return 0;
   return (rows * K + 255) / 256 * 256 + (4 * rows + 255) / 256 * 256;
 }
 
@@ -667,7 +938,7 @@ extern "C" int i8l_token_linear(const void* x, const int8_t* w_q, const float* w
   if (!w_q || !w_scale || (rows && (!x || !y))) return fail(I8L_ERR_ARG, "i8l_token_linear: null pointer");
   if (!aligned16(x) || !aligned16(w_q) || !aligned16(y) || !aligned16(bias) || (reinterpret_cast<uintptr_t>(workspace) & 255))
     return fail(I8L_ERR_ALIGN, "i8l_token_linear: x, w_q, y and bias must be 16-byte aligned, the workspace 256-byte");
-  const int64_t need = i8l_token_linear_workspace(rows, K);
+  const int64_t need = i8l_token_linear_workspace(rows, experts, N, K);
   if (need && (!workspace || workspace_bytes < need))
     return fail(I8L_ERR_ARG, "i8l_token_linear: workspace of %lld bytes is too small", (long long)workspace_bytes);
   if (!rows) return I8L_OK;
@@ -677,12 +948,7 @@ extern "C" int i8l_token_linear(const void* x, const int8_t* w_q, const float* w
   a.bias = static_cast<const __nv_bfloat16*>(bias); a.y = y;
   a.rows = rows; a.N = N; a.K = K; a.experts = experts; a.out_f32 = (flags & I8L_GEMM_OUT_F32) ? 1 : 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  switch (few_rows(rows, K)) {
-    case 1: return launch_few<1>(a, st);
-    case 2: return launch_few<2>(a, st);
-    case 4: return launch_few<4>(a, st);
-    case 8: return launch_few<8>(a, st);
-  }
+  if (few_rows(rows, K, experts, N)) return run_few(a, st);
   int8_t* xq = static_cast<int8_t*>(workspace);
   float* xs = reinterpret_cast<float*>(xq + (rows * K + 255) / 256 * 256);
   const LaunchChain chain(st);
@@ -696,6 +962,11 @@ extern "C" int i8l_token_linear(const void* x, const int8_t* w_q, const float* w
   p.max_polls = gemm_wait_limit();
   p.withhold = gemm_withhold();
   const int tok = tile_tokens(a);
+  if (tok == 64) switch (k_split(a)) {
+      case 8: return launch_group<64, 8>(xq, p, st);
+      case 4: return launch_group<64, 4>(xq, p, st);
+      case 2: return launch_group<64, 2>(xq, p, st);
+    }
   if (tok == 128) return launch_group<128>(xq, p, st);
   return tok == 256 ? launch_group<256>(xq, p, st) : launch_group<64>(xq, p, st);
 }

@@ -519,7 +519,7 @@ def token_linear(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, offsets=No
         raise TypeError(f"out_dtype must be bfloat16 or float32, got {out_dtype}")
     x, wq, ws = _aligned(x), _aligned(wq), ws.contiguous()
     y = torch.empty((R, N), dtype=out_dtype, device=dev)
-    size = L.load().i8l_token_linear_workspace(R, Kd)
+    size = L.load().i8l_token_linear_workspace(R, E, N, Kd)
     work = torch.empty((size,), dtype=torch.int8, device=dev) if size else None
     if status is None:
         poll_status(dev)   # an earlier kernel that gave up a wait
