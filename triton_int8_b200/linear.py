@@ -224,6 +224,10 @@ class Int8Linear(nn.Module):
         m.load_state_dict({k: v.to(torch.bfloat16) for k, v in lin.state_dict().items()})
         return m
 
+    def freeze(self) -> "Int8FrozenLinear":
+        """The layer for serving: weights quantized once."""
+        return Int8FrozenLinear.from_linear(self)
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if not torch.compiler.is_compiling():   # plain tensors: the same calls and autograd node without the interpreter
             y = K.host().linear(x, self.weight, self.bias, *self.config.native)
@@ -233,3 +237,29 @@ class Int8Linear(nn.Module):
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, {self.config}"
+
+
+class Int8FrozenLinear(nn.Module):
+    """A linear layer for serving: int8 weights with one scale an output channel, kept; activations quantized per row (linear_w8a8).  Any
+    number of tokens, in_features a multiple of 16, out_features of 8.  Buffers weight_q, weight_scale and bias; no gradient."""
+
+    def __init__(self, weight_q: torch.Tensor, weight_scale: torch.Tensor, bias=None):
+        super().__init__()
+        self.out_features, self.in_features = weight_q.shape
+        self.register_buffer("weight_q", weight_q)
+        self.register_buffer("weight_scale", weight_scale)
+        self.register_buffer("bias", bias)
+
+    @classmethod
+    def from_linear(cls, lin: nn.Module) -> "Int8FrozenLinear":
+        """From Int8Linear or nn.Linear on a GPU, whose in_features are a multiple of 128."""
+        with torch.no_grad():
+            q, s = K.quant_row(lin.weight.to(torch.bfloat16), L.QMODE_ROWRCP)
+            bias = None if lin.bias is None else lin.bias.detach().to(torch.bfloat16).clone()
+        return cls(q, s, bias)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return linear_w8a8(x, self.weight_q, self.weight_scale, self.bias)
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"

@@ -4,15 +4,18 @@
     ...                                                        # any computation that keeps the rows in their places
     y = combine(rows, weights, pos, src)                       # y[t] = sum over j of weights[t, j] * rows[pos[t, j]]
 
-Both are differentiable and neither waits for the device: shapes depend on the sizes, not on the choices.  The reference has no
-expert layers.
+Both are differentiable and neither waits for the device: shapes depend on the sizes, not on the choices.  expert_linear multiplies the
+rows with their experts' kept int8 weights (serving); Int8MoE puts all of them together.  The reference has no expert layers.
 """
 from __future__ import annotations
 
 import torch
+import torch.nn.functional as F
+from torch import nn
 
 from . import _lib as L
 from . import kernels as K
+from .linear import DEFAULT, Int8Config, Int8Linear
 
 
 def _once(name: str, inputs, *results):
@@ -107,3 +110,72 @@ def expert_linear(rows: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, offset
     if offsets is None:
         raise ValueError("expert_linear: offsets are needed (linear_w8a8 takes one matrix for all rows)")
     return K.token_linear(rows, wq, ws, offsets, bias, out_dtype)
+
+
+class Int8MoE(nn.Module):
+    """Gated experts: y[t] = sum over the top_k experts e of token t of p_e * down_e(silu(gate_e(x)) * up_e(x)), p = softmax over the logits of
+    the chosen ones.  hidden and mlp are multiples of 128.
+
+    Training: the tokens are sorted with segments of whole blocks of 128 rows, and every expert's three linears are Int8Linear (or
+    what `linear(in, out)` builds) on its segment; the sizes of the segments are read from the device once a forward pass.
+    Serving: freeze() quantizes the weights once; forward passes without gradients then take expert_linear, any number of tokens from
+    one on, without waiting for the device.  It is a copy of the weights as they are then: train(), load_state_dict() and moving
+    the module drop it; after other changes to the weights freeze again."""
+
+    def __init__(self, hidden: int, mlp: int, experts: int, top_k: int, device=None, config: Int8Config = DEFAULT, linear=None):
+        super().__init__()
+        if not 1 <= top_k <= experts:
+            raise ValueError(f"top_k must be between 1 and the {experts} experts, got {top_k}")
+        if linear is None:
+            def linear(i, o):
+                return Int8Linear(i, o, bias=False, device=device, config=config)
+        self.experts, self.top_k = experts, top_k
+        self.router = nn.Linear(hidden, experts, bias=False, device=device, dtype=torch.bfloat16)
+        self.gate_proj = nn.ModuleList(linear(hidden, mlp) for _ in range(experts))
+        self.up_proj = nn.ModuleList(linear(hidden, mlp) for _ in range(experts))
+        self.down_proj = nn.ModuleList(linear(mlp, hidden) for _ in range(experts))
+        self._frozen = None
+        self.register_load_state_dict_post_hook(lambda module, keys: module._thaw())
+
+    def _thaw(self) -> None:
+        self._frozen = None
+
+    def _apply(self, fn, *args, **kwargs):   # to(), cuda(), half() and so on
+        self._thaw()
+        return super()._apply(fn, *args, **kwargs)
+
+    @torch.no_grad()
+    def freeze(self) -> "Int8MoE":
+        gate_up = torch.stack([torch.cat([g.weight, u.weight]) for g, u in zip(self.gate_proj, self.up_proj)])
+        down = torch.stack([d.weight for d in self.down_proj])
+        self._frozen = (*quantize_experts(gate_up), *quantize_experts(down))
+        return self
+
+    def train(self, mode: bool = True):
+        if mode:
+            self._thaw()
+        return super().train(mode)
+
+    def route(self, x: torch.Tensor):
+        """x [T, hidden] -> (ids int64 [T, top_k], weights fp32 [T, top_k])."""
+        logits, ids = self.router(x).float().topk(self.top_k, dim=-1)
+        return ids, logits.softmax(-1)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        x2 = x.reshape(-1, x.shape[-1])
+        ids, weights = self.route(x2)
+        if self._frozen is not None and not torch.is_grad_enabled():
+            gate_up_q, gate_up_s, down_q, down_s = self._frozen
+            rows, offsets, pos, src = sort_tokens(x2, ids, self.experts)
+            gate, up = expert_linear(rows, gate_up_q, gate_up_s, offsets).chunk(2, -1)
+            rows = expert_linear(F.silu(gate) * up, down_q, down_s, offsets)
+        else:
+            rows, offsets, pos, src = sort_tokens(x2, ids, self.experts, align=128)
+            ends = offsets.tolist()
+            parts = []
+            for e, (a, b) in enumerate(zip(ends, ends[1:])):
+                if b > a:
+                    part = rows[a:b]
+                    parts.append(self.down_proj[e](F.silu(self.gate_proj[e](part)) * self.up_proj[e](part)))
+            rows = torch.cat([*parts, rows.new_zeros(rows.shape[0] - ends[-1], rows.shape[1])])
+        return combine(rows, weights, pos, src).view(x.shape)
