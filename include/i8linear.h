@@ -363,8 +363,9 @@ I8L_API int i8l_combine_backward(const void* rows, const void* weights, const in
  *   y = (float(acc) * x_scale[row]) * w_scale[e, n] + bias[e, n]
  * is rounded once to bf16 (fp32 with I8L_GEMM_OUT_F32).  w_scale fp32 [experts, N]; bias bf16 [experts, N] or NULL.
  *   offsets int32 [experts + 1] on the device, non-decreasing, or NULL: one matrix (experts = 1) for all rows.  Rows in front
- *   of offsets[0] and from offsets[experts] on come out zero.
- * N a multiple of 8, K of 16 and at most 131072 (the int32 sum cannot overflow), experts <= 1024, rows >= 0.  x, w_q, y, bias
+ *   of offsets[0] and from offsets[experts] on come out zero.  Offsets outside [0, rows] are cut off; if they decrease y is
+ *   undefined, but nothing outside of it is touched.
+ * N a multiple of 8, K of 16 and at most 131072 (the int32 sum cannot overflow), experts <= 1024, rows from 0 to 2^30.  x, w_q, y, bias
  * 16-byte aligned.  workspace: i8l_token_linear_workspace bytes, 256-byte aligned, may be NULL where that is 0.
  * The row and channel scales are those of the reference's double_channel variant (triton/double-channle_fwd32.py:295-311).
  */

@@ -310,3 +310,95 @@ def test_rows_beyond_32_bit_offsets():
     assert torch.equal(drows[T:][::997], 2 * x[::997])
     ref = (x[::997].double() ** 2).sum(-1)
     assert ((dweights[::997, 1].double() - ref).abs() <= (H + 16) * 2.0 ** -24 * ref).all()
+
+
+def test_transforms_are_refused():
+    """The kernels cannot see through a batched tensor: an error, not numbers."""
+    x, ids = torch.randn(6, 16, device=DEV).requires_grad_(), torch.randint(0, 3, (6, 2), device=DEV)
+    w = torch.rand(6, 2, device=DEV).requires_grad_()
+    rows, offsets, pos, src = moe.sort_tokens(x, ids, 3)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(rows, x, torch.randn(3, *rows.shape, device=DEV), is_grads_batched=True, retain_graph=True)
+    y = moe.combine(rows.detach().requires_grad_(), w, pos, src)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y, w, torch.randn(3, *y.shape, device=DEV), is_grads_batched=True)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda r: moe.combine(r, w.detach(), pos, src))(torch.randn(2, *rows.shape, device=DEV))
+
+
+def test_changed_inputs_and_a_second_pass_are_noticed(path):
+    x, ids = torch.randn(6, 16, device=DEV).requires_grad_(), torch.randint(0, 3, (6, 2), device=DEV)
+    w = torch.rand(6, 2, device=DEV).requires_grad_()
+    rows, offsets, pos, src = moe.sort_tokens(x, ids, 3)
+    rows.sum().backward(retain_graph=True)
+    rows.sum().backward()
+    assert torch.equal(x.grad, torch.full_like(x, 4.0))
+    r = rows.detach().requires_grad_()
+    y = moe.combine(r, w, pos, src)
+    with torch.no_grad():
+        r.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
+
+
+def test_calls_from_several_threads_on_streams_of_their_own():
+    import threading
+
+    from triton_int8_b200.moe import expert_linear
+    q, s = K.quant_row(torch.randn(8 * 256, 512, device=DEV).to(BF16), 3)
+    q, s, bad = q.view(8, 256, 512), s.view(8, 256), []
+
+    def work(seed):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            g = torch.Generator(device=DEV).manual_seed(seed)
+            for T in (3, 7, 40, 700) * 3:
+                x = torch.randn(T, 512, device=DEV, generator=g).to(BF16).requires_grad_()
+                offsets = torch.linspace(0, T, 9, device=DEV).int()
+                ids = torch.randint(0, 8, (T, 2), device=DEV, generator=g)
+                stream.synchronize()   # the weights, and what the generators made
+                same = torch.equal(expert_linear(x.detach(), q, s, offsets), expert_linear(x.detach(), q, s, offsets))
+                rows, _, pos, src = moe.sort_tokens(x, ids, 8)
+                y = moe.combine(rows, torch.ones(T, 2, device=DEV), pos, src)
+                (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+                if not same or not torch.equal(y, (2 * x.detach().float()).to(BF16)) or not torch.equal(dx, torch.full_like(dx, 2.0)):
+                    bad.append((seed, T))
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+    K.check_status(DEV)
+
+
+def test_capture_beside_a_living_eager_graph_does_not_end_the_process(tmp_path):
+    """torch cannot capture a backward pass whose leaves belong to an eager graph on another stream: an exception, in a child process here."""
+    import os
+    import subprocess
+    import sys
+    script = tmp_path / "child.py"
+    script.write_text("""
+import torch
+from triton_int8_b200 import moe
+x = torch.randn(900, 136, device="cuda").requires_grad_()
+w, ids = torch.rand(900, 2, device="cuda").requires_grad_(), torch.randint(0, 6, (900, 2), device="cuda")
+def forward():
+    rows, offsets, pos, src = moe.sort_tokens(x, ids, 6)
+    return moe.combine(rows, w, pos, src)
+eager, dy = forward(), torch.randn(900, 136, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+try:
+    with torch.cuda.graph(graph):
+        torch.autograd.grad(forward(), (x, w), dy)
+except RuntimeError as e:
+    print("raised", type(e).__name__)
+dx, dw = torch.autograd.grad(eager, (x, w), dy)   # the eager graph still is what it was
+assert torch.isfinite(dx).all() and torch.isfinite(dw).all()
+print("alive")
+""")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, str(script)], cwd=root, env=dict(os.environ, PYTHONPATH=root), capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "alive" in done.stdout, done.stdout + done.stderr[-2000:]

@@ -94,6 +94,21 @@ def test_rows_in_front_of_the_first_expert_and_offsets_out_of_range():
     K.check_status(DEV)
 
 
+@pytest.mark.parametrize("R", [5, 200, 1000])
+def test_offsets_that_decrease_touch_nothing_else(R):
+    """Overlapping segments: y is undefined, what lies around it is not touched, and the next call is right."""
+    g = torch.Generator().manual_seed(R)
+    E, N = 64, 136
+    x, (wq, ws) = _rows(g, R, 64), _weights(g, E, N, 64)
+    offsets = torch.tensor([0, R] * (E // 2) + [0], dtype=torch.int32, device=DEV)
+    y = moe.expert_linear(x, wq, ws, offsets)
+    torch.cuda.synchronize()
+    assert y.shape == (R, N)
+    offsets = torch.tensor([0] + [R] * E, dtype=torch.int32, device=DEV)
+    assert torch.equal(moe.expert_linear(x, wq, ws, offsets, out_dtype=F32).cpu(), _plain(x, wq[0], ws[0], None))
+    K.check_status(DEV)
+
+
 @pytest.mark.parametrize("M,N,Kd", [(128, 256, 384), (256, 128, 1024), (512, 640, 128)])
 def test_bit_equal_to_double_channel(M, N, Kd):
     g = torch.Generator().manual_seed(M)

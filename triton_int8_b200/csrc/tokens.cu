@@ -11,7 +11,8 @@ namespace i8l {
 namespace {
 
 constexpr int MAX_EXPERTS = 1024;
-constexpr int64_t MAX_K = 131072;   // 127 * 128 * K < 2^31
+constexpr int64_t MAX_K = 131072;      // 127 * 128 * K < 2^31
+constexpr int64_t MAX_ROWS = 1 << 30;   // row and tile numbers are int
 
 struct TokenArgs {
   const __nv_bfloat16* x;
@@ -388,6 +389,7 @@ struct GroupArgs {
   int32_t *status, *mirror;
   uint32_t max_polls;
   int n_tiles, withhold;
+  int most;   // tiles there can be
 };
 struct __align__(16) GroupCtl {
   uint64_t full[8], empty[8], tfull[4], tempty[4], done, ready, freed;
@@ -519,18 +521,20 @@ group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
   __syncthreads();
   tc_fence_after();
   if (warp == 0) {   // running sum of the tiles
-    int carry = 0;
+    int64_t carry = 0;
     if (lane == 0) seg[0].first = 0;
     for (int e0 = 0; e0 < p.t.experts; e0 += 32) {
-      int up = e0 + lane < p.t.experts ? seg[e0 + lane + 1].first : 0;
+      int64_t up = e0 + lane < p.t.experts ? seg[e0 + lane + 1].first : 0;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, up, d);
+        const int64_t v = __shfl_up_sync(0xffffffffu, up, d);
         if (lane >= d) up += v;
       }
-      if (e0 + lane < p.t.experts) seg[e0 + lane + 1].first = carry + up;
+      // More than there can be: offsets that decrease, whose segments overlap.  Nothing is computed then.
+      if (e0 + lane < p.t.experts) seg[e0 + lane + 1].first = carry + up <= p.most ? (int)(carry + up) : 0;
       carry += __shfl_sync(0xffffffffu, up, 31);
     }
+    if (lane == 0 && carry > p.most) seg[p.t.experts].first = 0;
   }
   __syncthreads();
   if (SPLIT > 1) cluster_sync_all();   // the others' barriers are initialised before anything arrives on them
@@ -892,6 +896,7 @@ template <int TOK, int SPLIT = 1> int launch_group(const int8_t* xq, GroupArgs& 
   p.n_tiles = (int)((a.N + CHANNELS - 1) / CHANNELS);
   const int64_t most = (a.rows / TOK + (a.experts < a.rows ? a.experts : a.rows)) * p.n_tiles;   // tiles, whatever the offsets
   if (most >= (1ll << 31)) return fail(I8L_ERR_SHAPE, "i8l_token_linear: too large for 32-bit tile numbers");
+  p.most = (int)most;
   CUtensorMap mw;
   TokenMaps mx;
   if (int e = make_tile_map_i8(&mw, a.wq, a.experts * a.N, a.K, CHANNELS)) return e;
@@ -922,14 +927,14 @@ template <int TOK, int SPLIT = 1> int launch_group(const int8_t* xq, GroupArgs& 
 using namespace i8l;
 
 extern "C" int64_t i8l_token_linear_workspace(int64_t rows, int experts, int64_t N, int64_t K) {
-  if (rows <= 0 || K <= 0 || N <= 0 || experts <= 0 || rows >= (1ll << 31) || N >= (1ll << 31) || K > MAX_K || few_rows(rows, K, experts, N)) return 0;
+  if (rows <= 0 || K <= 0 || N <= 0 || experts <= 0 || rows > MAX_ROWS || N >= (1ll << 31) || K > MAX_K || few_rows(rows, K, experts, N)) return 0;
   return (rows * K + 255) / 256 * 256 + (4 * rows + 255) / 256 * 256;
 }
 
 extern "C" int i8l_token_linear(const void* x, const int8_t* w_q, const float* w_scale, const int32_t* offsets, const void* bias, void* y,
                                 int64_t rows, int experts, int64_t N, int64_t K, int flags, void* workspace, int64_t workspace_bytes,
                                 int32_t* status, void* stream) {
-  if (rows < 0 || rows >= (1ll << 31) || N < 8 || N % 8 || K < 16 || K % 16 || K > MAX_K || N >= (1ll << 31))
+  if (rows < 0 || rows > MAX_ROWS || N < 8 || N % 8 || K < 16 || K % 16 || K > MAX_K || N >= (1ll << 31))
     return fail(I8L_ERR_SHAPE, "i8l_token_linear: rows=%lld N=%lld K=%lld: N a multiple of 8, K of 16 and at most %lld", (long long)rows,
                 (long long)N, (long long)K, (long long)MAX_K);
   if (experts < 1 || experts > MAX_EXPERTS || (!offsets && experts != 1) || experts * N >= (1ll << 31))
