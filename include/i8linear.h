@@ -348,7 +348,7 @@ I8L_API int i8l_sort_tokens(const void* x, const void* ids, int ids64, int64_t t
  * i8l_sort_tokens).  A choice whose pos is outside [0, n_rows) adds nothing, whatever its weight.
  * i8l_combine_backward: drows[pos[t, j]] = weights[t, j] * dy[t], rows whose src is negative zero, and dweights[t, j] = the sum of
  * dy[t] * rows[pos[t, j]] in fp32, zero for dropped choices; either may be NULL.  pos and src are inverse to one another, as
- * i8l_sort_tokens makes them: a row is written by the choice that src names, and not at all if that choice names another row.
+ * i8l_sort_tokens makes them; where they are not, the gradients are undefined, but nothing outside of them is touched.
  * No counterpart in the reference.
  */
 I8L_API int i8l_combine(const void* rows, const void* weights, const int32_t* pos, int64_t n_rows, int64_t tokens, int64_t cols,

@@ -442,11 +442,10 @@ __global__ void __launch_bounds__(THREADS) combine_kernel(const CombineArgs a) {
 }
 
 // drows[pos[t, j]] = w[t, j] * dy[t], rows of no choice zero; dw[t, j] = the sum of dy[t] * rows[pos[t, j]], added in an order that
-// depends on the sizes and the alignment only.  A row is written by the choice that src names, so that rows are written once whatever pos
-// holds.  J choices at a time share the loads of dy; of odd rows each has pieces of its own, so those come one by one.
-template <typename T, typename W, bool ODD, int J, int U>
+// depends on the sizes only.  A row is written by the choice that src names, so that rows are written once whatever pos holds.  J choices at
+// a time share the loads of dy.
+template <typename T, typename W, int J, int U>
 __global__ void __launch_bounds__(THREADS) combine_backward_kernel(const CombineArgs a) {
-  static_assert(!ODD || J == 1, "one choice at a time");
   constexpr int N = PER_PIECE<T>;
   __shared__ float part[THREADS / 32][MAX_CHOICES];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = threadIdx.x & (a.lanes - 1);
@@ -466,44 +465,27 @@ __global__ void __launch_bounds__(THREADS) combine_backward_kernel(const Combine
       to[j] = r >= 0 && a.drows && a.src[r] == (int32_t)i ? row_at(a.drows, r, a.bytes) : nullptr;
       dot[j] = 0.f;
     }
-    // pieces of the row written; without one, of the row read
-    Cut cut{0, live ? a.bytes / 16 : 0};
-    Across g_from{reinterpret_cast<const uint4*>(dy), 0}, v_from{nullptr, 0};
-    if (ODD) {
-      const char* grid = to[0] ? to[0] : from[0];
-      cut = grid ? cut_of(grid, a.bytes) : Cut{0, 0};
-      if (grid) g_from = across(dy, cut);
-      if (from[0]) v_from = across(from[0], cut);
-      if (grid)
-        for (int i = l; i < MOST_ENDS<T>; i += a.lanes) {
-          const int at = end_element<T>(cut, a.bytes, i);
-          if (at < 0) continue;
-          const float d = to_float(*reinterpret_cast<const T*>(dy + at));
-          if (from[0]) dot[0] = fmaf(d, to_float(*reinterpret_cast<const T*>(from[0] + at)), dot[0]);
-          if (to[0]) *reinterpret_cast<T*>(to[0] + at) = from_float<T>(d * w[0]);
-        }
-    }
-    for (int q0 = l; q0 < cut.pieces; q0 += U * a.lanes) {
-      Pair g[U], v[J][U];
+    const int pieces = live ? a.bytes / 16 : 0;
+    for (int q0 = l; q0 < pieces; q0 += U * a.lanes) {
+      uint4 g[U], v[J][U];
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (q0 + u * a.lanes < cut.pieces) g[u] = load_pair(g_from, q0 + u * a.lanes);
+        if (q0 + u * a.lanes < pieces) g[u] = reinterpret_cast<const uint4*>(dy)[q0 + u * a.lanes];
 #pragma unroll
       for (int j = 0; j < J; ++j)
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (from[j] && q0 + u * a.lanes < cut.pieces)
-            v[j][u] = load_pair(ODD ? v_from : Across{reinterpret_cast<const uint4*>(from[j]), 0}, q0 + u * a.lanes);
+          if (from[j] && q0 + u * a.lanes < pieces) v[j][u] = reinterpret_cast<const uint4*>(from[j])[q0 + u * a.lanes];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (q0 + u * a.lanes >= cut.pieces) break;
+        if (q0 + u * a.lanes >= pieces) break;
         float d[N];
-        unpack<T>(joined(g[u], ODD ? g_from.off : 0), d);
+        unpack<T>(g[u], d);
 #pragma unroll
         for (int j = 0; j < J; ++j) {
           if (from[j]) {
             float f[N];
-            unpack<T>(joined(v[j][u], ODD ? v_from.off : 0), f);
+            unpack<T>(v[j][u], f);
 #pragma unroll
             for (int q = 0; q < N; ++q) dot[j] = fmaf(d[q], f[q], dot[j]);
           }
@@ -511,7 +493,7 @@ __global__ void __launch_bounds__(THREADS) combine_backward_kernel(const Combine
             float f[N];
 #pragma unroll
             for (int q = 0; q < N; ++q) f[q] = d[q] * w[j];
-            reinterpret_cast<uint4*>(to[j] + cut.head)[q0 + u * a.lanes] = pack<T>(f);
+            reinterpret_cast<uint4*>(to[j])[q0 + u * a.lanes] = pack<T>(f);
           }
         }
       }
@@ -543,6 +525,75 @@ __global__ void __launch_bounds__(THREADS) combine_backward_kernel(const Combine
   if (a.drows)
     for (int64_t r = (int64_t)blockIdx.x * (THREADS / 32) + warp; r < a.n_rows; r += (int64_t)gridDim.x * (THREADS / 32))
       if (a.src[r] < 0) copy_odd<T>(row_at(a.drows, r, a.bytes), nullptr, a.bytes, lane, 32);
+}
+
+// Odd rows, a warp each: the choice that src names has its whole dot product there and its gradient's row to write.  Pieces are those of
+// the row that is written, so dy is put together anew for each of them.  Choice by choice of a token 165 us for 9460 x 658 bf16 with 8
+// choices.
+template <typename T, typename W>
+__global__ void __launch_bounds__(THREADS) combine_backward_odd_kernel(const CombineArgs a) {
+  constexpr int N = PER_PIECE<T>, U = 2;
+  const int lane = threadIdx.x & 31;
+  const int64_t warps = (int64_t)gridDim.x * (THREADS / 32), me = (int64_t)(threadIdx.x >> 5) * gridDim.x + blockIdx.x, choices = a.tokens * a.k;
+  int next = me < a.n_rows ? a.src[me] : -1;
+  for (int64_t r = me; r < a.n_rows; r += warps) {
+    const int i = next;
+    next = r + warps < a.n_rows ? a.src[r + warps] : -1;
+    char* to = a.drows ? row_at(a.drows, r, a.bytes) : nullptr;
+    if (i < 0 || i >= choices) {
+      if (to) copy_odd<T>(to, nullptr, a.bytes, lane, 32);
+      continue;
+    }
+    const float w = weight_of<W>(a.weights, i);
+    const char *dy = row_at(a.dy, i / a.k, a.bytes), *row = row_at(a.rows, r, a.bytes);
+    const Cut cut = cut_of(to ? to : row, a.bytes);
+    const Across g_from = across(dy, cut), v_from = across(row, cut);
+    float dot = 0.f;
+    if (lane < MOST_ENDS<T>) {
+      const int at = end_element<T>(cut, a.bytes, lane);
+      if (at >= 0) {
+        const float d = to_float(*reinterpret_cast<const T*>(dy + at));
+        if (a.dweights) dot = d * to_float(*reinterpret_cast<const T*>(row + at));
+        if (to) *reinterpret_cast<T*>(to + at) = from_float<T>(d * w);
+      }
+    }
+    for (int q0 = lane; q0 < cut.pieces; q0 += U * 32) {
+      Pair g[U], v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (q0 + u * 32 < cut.pieces) {
+          g[u] = load_pair(g_from, q0 + u * 32);
+          if (a.dweights) v[u] = load_pair(v_from, q0 + u * 32);
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (q0 + u * 32 >= cut.pieces) break;
+        float d[N];
+        unpack<T>(joined(g[u], g_from.off), d);
+        if (a.dweights) {
+          float f[N];
+          unpack<T>(joined(v[u], v_from.off), f);
+#pragma unroll
+          for (int q = 0; q < N; ++q) dot = fmaf(d[q], f[q], dot);
+        }
+        if (to) {
+#pragma unroll
+          for (int q = 0; q < N; ++q) d[q] *= w;
+          reinterpret_cast<uint4*>(to + cut.head)[q0 + u * 32] = pack<T>(d);
+        }
+      }
+    }
+    if (a.dweights) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+      if (lane == 0) static_cast<W*>(a.dweights)[i] = from_float<W>(dot);
+    }
+  }
+  if (a.dweights)   // choices without a row
+    for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < choices; i += (int64_t)gridDim.x * THREADS) {
+      const int r = row_of(a, i);
+      if (r < 0 || a.src[r] != (int32_t)i) static_cast<W*>(a.dweights)[i] = from_float<W>(0.f);
+    }
 }
 
 // The same two for many tokens with rows of whole 16 bytes.  What bounds them is how many bytes are in flight: with loads into registers
@@ -720,6 +771,14 @@ int lanes_for(int64_t bytes, int64_t tokens) {
   while (lanes < THREADS && lanes * 16 < bytes && (lanes < 32 || lanes * 64 < bytes || tokens * lanes < few)) lanes *= 2;
   return lanes;
 }
+// Blocks for all tokens, and for the rows of no choice, of which there may be many more (padding behind a few tokens): a warp a row.
+unsigned blocks_for(int64_t tokens, int lanes, int64_t rows) {
+  const int64_t copies = (tokens + THREADS / lanes - 1) / (THREADS / lanes), resident = 4ll * sm_count();
+  int64_t clears = (rows + THREADS / 32 - 1) / (THREADS / 32);
+  if (clears > resident) clears = resident;
+  const int64_t blocks = copies > clears ? copies : clears;
+  return (unsigned)(blocks ? blocks : 1);
+}
 // Choices of a block that counts and places them: one a thread, more where all blocks' counts, which every block adds up, would be
 // over 16384.
 int64_t sort_chunk(int64_t n, int64_t experts) {
@@ -751,14 +810,13 @@ int launch_ring(const CombineArgs& a, cudaStream_t st) {
 template <typename T, typename W>
 int launch_combine(const CombineArgs& a, bool backward, bool odd, cudaStream_t st) {
   if (!odd && ring_fits(a, backward)) return backward ? launch_ring<T, W, true>(a, st) : launch_ring<T, W, false>(a, st);
-  const unsigned tokens = (unsigned)((a.tokens + THREADS / a.lanes - 1) / (THREADS / a.lanes));
-  const unsigned grid = tokens ? tokens : 1;   // without tokens there still are gradients of rows to clear
+  const unsigned grid = blocks_for(a.tokens, a.lanes, backward && a.drows ? a.n_rows : 0);
   const bool one = a.bytes <= 16 * a.lanes;    // a piece a thread: fewer registers, more blocks on an SM
   if (backward) {
-    if (odd) combine_backward_kernel<T, W, true, 1, 2><<<grid, THREADS, 0, st>>>(a);
-    else if (one) combine_backward_kernel<T, W, false, 2, 1><<<grid, THREADS, 0, st>>>(a);
-    else if (a.k <= 2) combine_backward_kernel<T, W, false, 2, 2><<<grid, THREADS, 0, st>>>(a);
-    else combine_backward_kernel<T, W, false, 4, 2><<<grid, THREADS, 0, st>>>(a);
+    if (odd) combine_backward_odd_kernel<T, W><<<blocks_for(0, 32, a.n_rows), THREADS, 0, st>>>(a);
+    else if (one) combine_backward_kernel<T, W, 2, 1><<<grid, THREADS, 0, st>>>(a);
+    else if (a.k <= 2) combine_backward_kernel<T, W, 2, 2><<<grid, THREADS, 0, st>>>(a);
+    else combine_backward_kernel<T, W, 4, 2><<<grid, THREADS, 0, st>>>(a);
   } else {
     if (odd) combine_kernel<T, W, true, 2, 1><<<grid, THREADS, 0, st>>>(a);
     else if (one) combine_kernel<T, W, false, 4, 1><<<grid, THREADS, 0, st>>>(a);
@@ -816,8 +874,7 @@ extern "C" int i8l_sort_tokens(const void* x, const void* ids, int ids64, int64_
   a.tokens = tokens; a.bytes = (int)(cols * size);
   a.n = (int)n; a.k = k; a.experts = experts; a.align = (int)align; a.n_rows = (int)rows; a.ids64 = ids64 ? 1 : 0;
   a.lanes = lanes_for(a.bytes, tokens);
-  const unsigned copies = (unsigned)((tokens + THREADS / a.lanes - 1) / (THREADS / a.lanes));
-  const unsigned grid = copies ? copies : 1;
+  const unsigned grid = blocks_for(tokens, a.lanes, rows);
   if (n <= SMALL_SORT) {
     if (!odd) sort_small_kernel<uint32_t, false><<<grid, THREADS, 0, st>>>(a);
     else if (size == 4) sort_small_kernel<uint32_t, true><<<grid, THREADS, 0, st>>>(a);

@@ -1263,18 +1263,29 @@ extern "C" int i8l_quant_tile(const void* x, int64_t batch, int64_t rows, int64_
 }
 
 namespace i8l {
-// The rows of a product for serving: the kernels below take any multiple of 8 columns where nothing is rotated.
-int quant_token_rows(const void* x, int64_t rows, int64_t cols, int8_t* q, float* scale, cudaStream_t st) {
+// The rows of a product for serving: any multiple of 8 columns, and none of the rows from *limit on, which belong to nobody.
+template <int T>
+__global__ void __launch_bounds__(256)
+quant_token_kernel(const __nv_bfloat16* __restrict__ x, int64_t rows, int64_t cols, int8_t* __restrict__ q, float* __restrict__ scale,
+                   const int32_t* limit, int first) {
+  chain_start(first);
+  if (limit) {
+    const int64_t end = *limit;
+    rows = end < rows ? end : rows;
+    if ((int64_t)blockIdx.x * (256 / T) >= rows) return;
+  }
+  quant_row_cached_body<I8L_QMODE_ROWRCP, T>(blockIdx.x, x, rows, cols, q, scale, 0);
+}
+int quant_token_rows(const void* x, int64_t rows, int64_t cols, int8_t* q, float* scale, const int32_t* limit, cudaStream_t st) {
   const __nv_bfloat16* xp = static_cast<const __nv_bfloat16*>(x);
-  constexpr int MODE = I8L_QMODE_ROWRCP;
   auto cached = [&](auto kernel, int per_block) {
-    return launch(kernel, dim3((unsigned)((rows + per_block - 1) / per_block)), 256, 0, st, xp, rows, cols, q, scale, chain_first());
+    return launch(kernel, dim3((unsigned)((rows + per_block - 1) / per_block)), 256, 0, st, xp, rows, cols, q, scale, limit, chain_first());
   };
-  I8L_CUDA_OK(cols <= 2048    ? cached(quant_row_cached_kernel<MODE, 32>, 8)
-              : cols <= 4096  ? cached(quant_row_cached_kernel<MODE, 64>, 4)
-              : cols <= 8192  ? cached(quant_row_cached_kernel<MODE, 128>, 2)
-              : cols <= 16384 ? cached(quant_row_cached_kernel<MODE, 256>, 1)
-                              : launch(quant_row_kernel<MODE, false>, dim3((unsigned)rows), 256, 0, st, xp, cols, q, scale, chain_first()));
+  I8L_CUDA_OK(cols <= 2048    ? cached(quant_token_kernel<32>, 8)
+              : cols <= 4096  ? cached(quant_token_kernel<64>, 4)
+              : cols <= 8192  ? cached(quant_token_kernel<128>, 2)
+              : cols <= 16384 ? cached(quant_token_kernel<256>, 1)
+                              : launch(quant_row_kernel<I8L_QMODE_ROWRCP, false>, dim3((unsigned)rows), 256, 0, st, xp, cols, q, scale, chain_first()));
   return I8L_OK;
 }
 }  // namespace i8l

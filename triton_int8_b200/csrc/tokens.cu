@@ -359,15 +359,16 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_mma_kernel(const TokenArgs
 // number is the instruction's N and may be any multiple of 16.  A segment of 17 rows costs 32 columns that way, where tokens as
 // MMA rows would cost 128, and the weights, which bound the product until a segment has some hundred rows, are read once.
 //
-// Persistent, a CTA per SM, 384 threads: warp 0 brings K blocks of 128 bytes by TMA (128 weight rows and the tokens of the tile) into a
-// ring, warp 1 issues tcgen05.mma kind::i8 into one of several accumulators in tensor memory, warps 4 to 11 take a finished one
-// out: a lane is a channel there, a register a token, so a bf16 tile is turned in shared memory and leaves 16 bytes a lane.
-// Warps 2 and 3 clear the rows of no expert.  Tiles come from the offsets in device memory: nothing waits for the host.
+// Persistent, a CTA per SM, 640 threads: warp 0 brings K blocks of 128 bytes by TMA (128 weight rows and the tokens of the tile) into a
+// ring, warp 1 issues tcgen05.mma kind::i8 into one of several accumulators in tensor memory, warps 4 to 19 take a finished one
+// out: a lane is a channel there, a register a token, so a bf16 tile is turned in shared memory, two tokens a word, and leaves 16 bytes a
+// lane.  Warps 2 and 3 clear the rows of no expert, the others too when their tiles are done.  Tiles come from the offsets in device memory: nothing waits for the host.
 // All waits are bounded, as in gemm.cu: on expiry every role leaves, the status word says so.
-constexpr int GRP_THREADS = 384, GRP_EPI_WARPS = 8, CHANNELS = 128, KBYTES = 128;
+constexpr int GRP_THREADS = 640, GRP_EPI_WARPS = 16, CHANNELS = 128, KBYTES = 128;
 constexpr int A_BYTES = CHANNELS * KBYTES;
 constexpr int BOXES = 5;   // maps of 16, 32, 64, 128 and 256 tokens
-constexpr int EPI_BYTES = 32 * 32 * 2;        // 32 tokens x 32 channels in bf16
+constexpr int EPI_TOKENS = 16, EPI_BYTES = EPI_TOKENS * 32 * 2;   // tokens that a warp takes out at a time, x 32 channels in bf16
+constexpr int CLEAR_WARPS = 2 + GRP_EPI_WARPS;
 constexpr int RASTER = 16;                    // token tiles whose rows should stay in L2 while the channels are gone through
 
 struct __align__(16) Segment {
@@ -395,7 +396,7 @@ struct __align__(16) GroupCtl {
   uint64_t full[8], empty[8], tfull[4], tempty[4], done, ready, freed;
   int abort_flag;
   uint32_t tmem_base, by[RASTER + 1];
-  __align__(16) float scale[GRP_EPI_WARPS][32];   // of the tokens that a warp takes out, read four at a time
+  __align__(16) float scale[GRP_EPI_WARPS][EPI_TOKENS];   // of the tokens that a warp takes out, read four at a time
 };
 static_assert(offsetof(GroupCtl, scale) % 16 == 0, "vector reads");
 struct TokenMaps {
@@ -543,6 +544,19 @@ group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
   const int rank = SPLIT > 1 ? (int)cluster_ctarank() : 0, unit = (int)blockIdx.x / SPLIT, units = (int)gridDim.x / SPLIT;
   const int kb0 = rank * blocks / SPLIT, kb1 = (rank + 1) * blocks / SPLIT;   // this CTA's K blocks
 
+  // Rows of no expert, a warp's share at a time: pieces of 4 KB go round the CTAs and their warps.
+  auto clear_dead = [&](int w) {
+    const int64_t before = seg[0].row, behind = (int64_t)seg[p.t.experts - 1].row + seg[p.t.experts - 1].rows, dead = before + p.t.rows - behind;
+    const int64_t pieces = p.t.N * (p.t.out_f32 ? 4 : 2) / 16, front = before * pieces, all = dead * pieces, skip = (behind - before) * pieces;
+    uint4* y = static_cast<uint4*>(p.t.y);
+    for (int64_t i0 = ((int64_t)w * gridDim.x + blockIdx.x) * 256; i0 < all; i0 += (int64_t)gridDim.x * CLEAR_WARPS * 256)
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int64_t i = i0 + u * 32 + lane;
+        if (i < all) y[i < front ? i : i + skip] = make_uint4(0, 0, 0, 0);
+      }
+  };
+
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     const bool elected = elect_one();
@@ -623,18 +637,12 @@ group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     int dummy = 0;
     mbar_wait(smem_u32(&ctl.done), 0, &dummy);
   } else if (warp < 4) {
-    // ------------------------------------------------------------------ rows of no expert
-    const int64_t before = seg[0].row, behind = (int64_t)seg[p.t.experts - 1].row + seg[p.t.experts - 1].rows, dead = before + p.t.rows - behind;
-    const int64_t pieces = p.t.N * (p.t.out_f32 ? 4 : 2) / 16;
-    for (int64_t i = (int64_t)blockIdx.x * 64 + threadIdx.x - 64; i < dead * pieces; i += (int64_t)gridDim.x * 64) {
-      const int64_t r = i / pieces;
-      static_cast<uint4*>(p.t.y)[(r < before ? r : behind + r - before) * pieces + i - r * pieces] = make_uint4(0, 0, 0, 0);
-    }
+    clear_dead(warp - 2);
   } else {
     // ------------------------------------------------------------------ epilogue
-    const int q = warp & 3, half = (warp - 4) >> 2;   // a quarter of the channels, every other 32 tokens
+    const int q = warp & 3, group = (warp - 4) >> 2;   // a quarter of the channels, 16 of every 64 tokens
     uint8_t* const turn = smem + G::RING + (warp - 4) * EPI_BYTES;
-    constexpr int PARTS = TOK / 64;   // of 32 tokens
+    constexpr int PARTS = TOK / 64;   // of 16 tokens
     if constexpr (SPLIT > 1) {
       int* const part = reinterpret_cast<int*>(smem + G::RING);   // [tokens, channels]: this CTA's sums
       const uint32_t part_at = smem_u32(part), ready = smem_u32(&ctl.ready), freed = smem_u32(&ctl.freed);
@@ -657,14 +665,13 @@ group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         wait_cluster(freed, ph ^ 1u, abort_flag, p.max_polls);   // the tile before has been read by all
 #pragma unroll
         for (int i = 0; i < PARTS; ++i) {
-          const int j0 = half * 32 + i * 64;
+          const int j0 = group * EPI_TOKENS + i * 64;
           if (j0 >= tile.rows) break;
-          uint32_t r[32];
+          uint32_t r[EPI_TOKENS];
           tc_ld16(tmem_base + ((uint32_t)(q * 32) << 16) + ab * TOK + j0, r);
-          tc_ld16(tmem_base + ((uint32_t)(q * 32) << 16) + ab * TOK + j0 + 16, r + 16);
           tc_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) part[(j0 + j) * CHANNELS + q * 32 + lane] = (int)r[j];
+          for (int j = 0; j < EPI_TOKENS; ++j) part[(j0 + j) * CHANNELS + q * 32 + lane] = (int)r[j];
         }
         tc_fence_before();
         __syncwarp();
@@ -725,8 +732,8 @@ group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
       f.bias = n < p.t.N && p.t.bias ? __bfloat162float(p.t.bias[c]) : 0.f;
 #pragma unroll
       for (int i = 0; i < PARTS; ++i) {
-        const int j = half * 32 + i * 64 + lane;
-        f.token[i] = j < f.tile.rows ? p.xs[f.tile.row + j] : 0.f;
+        const int j = group * EPI_TOKENS + i * 64 + lane;
+        f.token[i] = lane < EPI_TOKENS && j < f.tile.rows ? p.xs[f.tile.row + j] : 0.f;
       }
       return f;
     };
@@ -742,55 +749,54 @@ group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
       if (t + units < total) next = fetch(t + units);
       const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + ab * TOK;
       const int n = now.tile.channel + q * 32 + lane;
+      const float2 sw2 = make_float2(now.sw, now.sw), bias2 = make_float2(now.bias, now.bias);
 #pragma unroll
       for (int i = 0; i < PARTS; ++i) {
-        const int j0 = half * 32 + i * 64, left = now.tile.rows - j0;
+        const int j0 = group * EPI_TOKENS + i * 64, left = now.tile.rows - j0;
         if (left <= 0) break;
-        uint32_t r[32];
+        uint32_t r[EPI_TOKENS];
         tc_ld16(taddr + j0, r);
-        tc_ld16(taddr + j0 + 16, r + 16);
-        scale[lane] = now.token[i];
+        if (lane < EPI_TOKENS) scale[lane] = now.token[i];
         __syncwarp();
         tc_ld_wait();
-        float v[32];
+        float2 v[EPI_TOKENS / 2];   // two tokens each
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          const float4 sx = *reinterpret_cast<const float4*>(scale + j);
-          v[j] = __fmul_rn(__fmul_rn(__int2float_rn((int)r[j]), sx.x), now.sw);
-          v[j + 1] = __fmul_rn(__fmul_rn(__int2float_rn((int)r[j + 1]), sx.y), now.sw);
-          v[j + 2] = __fmul_rn(__fmul_rn(__int2float_rn((int)r[j + 2]), sx.z), now.sw);
-          v[j + 3] = __fmul_rn(__fmul_rn(__int2float_rn((int)r[j + 3]), sx.w), now.sw);
+        for (int j = 0; j < EPI_TOKENS / 2; j += 2) {
+          const float4 sx = *reinterpret_cast<const float4*>(scale + 2 * j);
+          v[j] = __fmul2_rn(__fmul2_rn(make_float2(__int2float_rn((int)r[2 * j]), __int2float_rn((int)r[2 * j + 1])), make_float2(sx.x, sx.y)), sw2);
+          v[j + 1] = __fmul2_rn(__fmul2_rn(make_float2(__int2float_rn((int)r[2 * j + 2]), __int2float_rn((int)r[2 * j + 3])), make_float2(sx.z, sx.w)), sw2);
         }
         if (p.t.bias) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __fadd_rn(v[j], now.bias);
+          for (int j = 0; j < EPI_TOKENS / 2; ++j) v[j] = make_float2(__fadd_rn(v[j].x, bias2.x), __fadd_rn(v[j].y, bias2.y));
         }
         const int64_t row = now.tile.row + j0;
         if (p.t.out_f32) {
           float* y = static_cast<float*>(p.t.y) + row * p.t.N + n;
           if (n < p.t.N) {
-            if (left >= 32) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) y[j * p.t.N] = v[j];
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (j < left) y[j * p.t.N] = v[j];
+            for (int j = 0; j < EPI_TOKENS / 2; ++j) {
+              if (2 * j < left) y[2 * j * p.t.N] = v[j].x;
+              if (2 * j + 1 < left) y[(2 * j + 1) * p.t.N] = v[j].y;
             }
           }
           __syncwarp();   // the scales have been read
         } else {
-          __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(turn) + lane;
+          uint32_t* words = reinterpret_cast<uint32_t*>(turn);   // [pairs of tokens, channels]
 #pragma unroll
-          for (int j = 0; j < 32; ++j) to[j * 32] = __float2bfloat16_rn(v[j]);
+          for (int j = 0; j < EPI_TOKENS / 2; ++j) {
+            const __nv_bfloat162 w = __floats2bfloat162_rn(v[j].x, v[j].y);
+            words[j * 32 + lane] = *reinterpret_cast<const uint32_t*>(&w);
+          }
           __syncwarp();
-          const int piece = lane & 3, n8 = now.tile.channel + q * 32 + piece * 8;
-          __nv_bfloat16* y = static_cast<__nv_bfloat16*>(p.t.y) + (row + (lane >> 2)) * p.t.N + n8;
-#pragma unroll
-          for (int i8 = 0; i8 < 4; ++i8) {
-            const int j = i8 * 8 + (lane >> 2);
-            if (j < left && n8 < p.t.N)
-              *reinterpret_cast<uint4*>(y + i8 * 8 * p.t.N) = *reinterpret_cast<const uint4*>(turn + j * 64 + piece * 16);
+          const int pair = lane >> 2, piece = lane & 3, n8 = now.tile.channel + q * 32 + piece * 8;
+          const uint4 lo = *reinterpret_cast<const uint4*>(words + pair * 32 + piece * 8), hi = *reinterpret_cast<const uint4*>(words + pair * 32 + piece * 8 + 4);
+          __nv_bfloat16* y = static_cast<__nv_bfloat16*>(p.t.y) + (row + 2 * pair) * p.t.N + n8;
+          if (n8 < p.t.N) {
+            if (2 * pair < left)
+              *reinterpret_cast<uint4*>(y) = make_uint4(__byte_perm(lo.x, lo.y, 0x5410), __byte_perm(lo.z, lo.w, 0x5410), __byte_perm(hi.x, hi.y, 0x5410), __byte_perm(hi.z, hi.w, 0x5410));
+            if (2 * pair + 1 < left)
+              *reinterpret_cast<uint4*>(y + p.t.N) = make_uint4(__byte_perm(lo.x, lo.y, 0x7632), __byte_perm(lo.z, lo.w, 0x7632), __byte_perm(hi.x, hi.y, 0x7632), __byte_perm(hi.z, hi.w, 0x7632));
           }
           __syncwarp();
         }
@@ -801,6 +807,7 @@ group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
       if (++ab == G::BUFS) { ab = 0; aph ^= 1u; }
     }
     }
+    clear_dead(warp - 2);
   }
   tc_fence_before();
   __syncthreads();
@@ -957,7 +964,7 @@ extern "C" int i8l_token_linear(const void* x, const int8_t* w_q, const float* w
   int8_t* xq = static_cast<int8_t*>(workspace);
   float* xs = reinterpret_cast<float*>(xq + (rows * K + 255) / 256 * 256);
   const LaunchChain chain(st);
-  if (int e = quant_token_rows(x, rows, K, xq, xs, st)) return e;
+  if (int e = quant_token_rows(x, rows, K, xq, xs, offsets ? offsets + experts : nullptr, st)) return e;
   (void)chain_first();
   GroupArgs p{};
   p.t = a;
