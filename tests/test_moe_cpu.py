@@ -86,7 +86,7 @@ def test_workspace_sizes(lib):
     assert lib.i8l_sort_workspace(512, 2, 8) == 0                      # few choices need none
     assert lib.i8l_sort_workspace(513, 2, 8) == 5 * 8 * 4              # chunks of 256 choices
     assert lib.i8l_sort_workspace(1 << 20, 8, 1024) == 16 * 1024 * 4
-    assert lib.i8l_token_linear_workspace(9, 1, 8, 48) == 512 + 256
+    assert lib.i8l_token_linear_workspace(9, 1, 8, 48) == 1280 + 256                 # rows 128 bytes apart
     assert lib.i8l_token_linear_workspace(8, 1, 8, 48) == 0                     # few rows: one launch
     assert lib.i8l_token_linear_workspace(1, 1, 8, 131072) == 131072 + 256      # but long ones
     assert lib.i8l_token_linear_workspace(8, 1, 11008, 4096) == 32768 + 256     # and more than four on many weights

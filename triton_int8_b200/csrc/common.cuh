@@ -30,8 +30,9 @@ int quant_pair(const void* a, int64_t a_batch, int64_t a_rows, int a_gran, int8_
                int64_t b_batch, int64_t b_rows, int b_gran, int8_t* bq, float* bs, int64_t cols, int qmode, int hadamard,
                cudaStream_t st);
 // x bf16 [rows, cols], cols a multiple of 8 and at most 2^20: int8 rows with one scale each, I8L_QMODE_ROWRCP without rotation.
-// limit: null, or a number in device memory from which on rows may be left out.
-int quant_token_rows(const void* x, int64_t rows, int64_t cols, int8_t* q, float* scale, const int32_t* limit, cudaStream_t st);
+// stride: bytes between rows of q (cols above 16384 columns).  limit: null, or a number in device memory from which on rows may be left out.
+int quant_token_rows(const void* x, int64_t rows, int64_t cols, int8_t* q, int64_t stride, float* scale, const int32_t* limit,
+                     cudaStream_t st);
 // i8l_col_sum; in a chain it runs beside its neighbours.
 int col_sum(const void* x, int64_t rows, int64_t cols, void* out, cudaStream_t st);
 // Clears n floats; in a chain the next kernel waits for it before anything else.

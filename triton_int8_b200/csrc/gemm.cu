@@ -1107,11 +1107,11 @@ int make_tile_map_bf16(CUtensorMap* map, const void* ptr, int64_t rows, int64_t 
   return I8L_OK;
 }
 
-int make_tile_map_i8(CUtensorMap* map, const void* ptr, int64_t rows, int64_t K, int box_rows) {
+int make_tile_map_i8(CUtensorMap* map, const void* ptr, int64_t rows, int64_t K, int64_t stride, int box_rows) {
   EncodeTiledFn enc = get_encode();
   if (!enc) return fail(I8L_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   cuuint64_t gdim[2] = {(cuuint64_t)K, (cuuint64_t)rows};
-  cuuint64_t gstr[1] = {(cuuint64_t)K};
+  cuuint64_t gstr[1] = {(cuuint64_t)stride};
   cuuint32_t box[2] = {(cuuint32_t)BK, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), gdim, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,

@@ -9,9 +9,9 @@ namespace i8l {
 // Host: tensor map of a bf16 [rows, K] matrix in boxes of 128 x 128 elements, unswizzled (defined with the
 // other tensor-map code next to the GEMM launcher).
 int make_tile_map_bf16(CUtensorMap* map, const void* ptr, int64_t rows, int64_t K);
-// The same of an int8 [rows, K] matrix in boxes of box_rows x 128 bytes, 128-byte swizzle; K a multiple of 16.  What a box reaches over
-// the matrix reads as zero.
-int make_tile_map_i8(CUtensorMap* map, const void* ptr, int64_t rows, int64_t K, int box_rows);
+// The same of an int8 [rows, K] matrix, rows `stride` bytes apart (a multiple of 16), in boxes of box_rows x 128 bytes, 128-byte swizzle.  What
+// a box reaches over the matrix reads as zero.
+int make_tile_map_i8(CUtensorMap* map, const void* ptr, int64_t rows, int64_t K, int64_t stride, int box_rows);
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 

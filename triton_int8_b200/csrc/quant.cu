@@ -748,7 +748,7 @@ quant_row_kernel(const __nv_bfloat16* __restrict__ x, int64_t cols, int8_t* __re
 template <int MODE, int T>
 __device__ __forceinline__ void
 quant_row_cached_body(unsigned block, const __nv_bfloat16* __restrict__ x, int64_t rows, int64_t cols, int8_t* __restrict__ q,
-                        float* __restrict__ scale, int first) {
+                        float* __restrict__ scale, int first, int64_t stride = 0) {
   __shared__ float s_red[8];
   const int tid = threadIdx.x, l = tid & 31, t = tid & (T - 1);
   const int64_t row = (int64_t)block * (256 / T) + tid / T;
@@ -775,7 +775,7 @@ quant_row_cached_body(unsigned block, const __nv_bfloat16* __restrict__ x, int64
     m = hmax_of(hm);
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  for (int o = (T < 32 ? T : 32) / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (T > 32) {
     if (l == 0) s_red[tid >> 5] = m;
     __syncthreads();
@@ -787,7 +787,7 @@ quant_row_cached_body(unsigned block, const __nv_bfloat16* __restrict__ x, int64
   float s, stored;
   make_scale<MODE>(m, s, stored);
   if (live && t == 0) scale[row] = stored;
-  uint2* qr = reinterpret_cast<uint2*>(q + row * cols);
+  uint2* qr = reinterpret_cast<uint2*>(q + row * (stride ? stride : cols));
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     if (i * T + t < nchunks) qr[i * T + t] = finite ? quant_piece_finite<MODE>(cache[i], s) : quant_piece<MODE>(cache[i], s);
@@ -1266,22 +1266,25 @@ namespace i8l {
 // The rows of a product for serving: any multiple of 8 columns, and none of the rows from *limit on, which belong to nobody.
 template <int T>
 __global__ void __launch_bounds__(256)
-quant_token_kernel(const __nv_bfloat16* __restrict__ x, int64_t rows, int64_t cols, int8_t* __restrict__ q, float* __restrict__ scale,
-                   const int32_t* limit, int first) {
+quant_token_kernel(const __nv_bfloat16* __restrict__ x, int64_t rows, int64_t cols, int8_t* __restrict__ q, int64_t stride,
+                   float* __restrict__ scale, const int32_t* limit, int first) {
   chain_start(first);
   if (limit) {
     const int64_t end = *limit;
     rows = end < rows ? end : rows;
     if ((int64_t)blockIdx.x * (256 / T) >= rows) return;
   }
-  quant_row_cached_body<I8L_QMODE_ROWRCP, T>(blockIdx.x, x, rows, cols, q, scale, 0);
+  quant_row_cached_body<I8L_QMODE_ROWRCP, T>(blockIdx.x, x, rows, cols, q, scale, 0, stride);
 }
-int quant_token_rows(const void* x, int64_t rows, int64_t cols, int8_t* q, float* scale, const int32_t* limit, cudaStream_t st) {
+int quant_token_rows(const void* x, int64_t rows, int64_t cols, int8_t* q, int64_t stride, float* scale, const int32_t* limit,
+                     cudaStream_t st) {
   const __nv_bfloat16* xp = static_cast<const __nv_bfloat16*>(x);
   auto cached = [&](auto kernel, int per_block) {
-    return launch(kernel, dim3((unsigned)((rows + per_block - 1) / per_block)), 256, 0, st, xp, rows, cols, q, scale, limit, chain_first());
+    return launch(kernel, dim3((unsigned)((rows + per_block - 1) / per_block)), 256, 0, st, xp, rows, cols, q, stride, scale, limit, chain_first());
   };
-  I8L_CUDA_OK(cols <= 2048    ? cached(quant_token_kernel<32>, 8)
+  I8L_CUDA_OK(cols <= 512     ? cached(quant_token_kernel<8>, 32)   // short rows: no lanes without a piece
+              : cols <= 1024  ? cached(quant_token_kernel<16>, 16)
+              : cols <= 2048  ? cached(quant_token_kernel<32>, 8)
               : cols <= 4096  ? cached(quant_token_kernel<64>, 4)
               : cols <= 8192  ? cached(quant_token_kernel<128>, 2)
               : cols <= 16384 ? cached(quant_token_kernel<256>, 1)
