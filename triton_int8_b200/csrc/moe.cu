@@ -89,7 +89,6 @@ __device__ __forceinline__ uint4 joined(const Pair& v, int off) {
 }
 // An odd row, from another one or from nothing, by threads l, l + lanes, ...
 template <typename T> __device__ __forceinline__ void copy_odd(char* to, const char* from, int bytes, int l, int lanes) {
-  constexpr int U = 4;
   const Cut c = cut_of(to, bytes);
   for (int i = l; i < MOST_ENDS<T>; i += lanes) {
     const int at = end_element<T>(c, bytes, i);
@@ -101,15 +100,7 @@ template <typename T> __device__ __forceinline__ void copy_odd(char* to, const c
     return;
   }
   const Across r = across(from, c);
-  for (int q0 = l; q0 < c.pieces; q0 += U * lanes) {
-    Pair v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (q0 + u * lanes < c.pieces) v[u] = load_pair(r, q0 + u * lanes);
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (q0 + u * lanes < c.pieces) out[q0 + u * lanes] = joined(v[u], r.off);
-  }
+  for (int q = l; q < c.pieces; q += lanes) out[q] = joined(load_pair(r, q), r.off);
 }
 
 __device__ __forceinline__ int64_t load_id(const void* ids, int wide, int64_t i) {
@@ -330,9 +321,10 @@ __global__ void __launch_bounds__(THREADS) sort_copy_kernel(const SortArgs a) {
     if (a.src[r] < 0) copy_odd<uint32_t>(static_cast<char*>(a.rows) + r * a.bytes, nullptr, a.bytes, lane, 32);
 }
 // Odd rows are put together for each place anyway: row by row, those of no choice among them, all of them alike much work.  Blocks go
-// on to further rows and know where from before they get there (a block a few rows 26 us for 4099 x 1405 fp16, 6 choices).
+// on to further rows and know where from before they get there, and there are many of them: 13554 x 780 fp16 with 6 choices 53 us (four
+// pieces a lane and half the blocks 60).
 template <typename T>
-__global__ void __launch_bounds__(THREADS) sort_copy_odd_kernel(const SortArgs a) {
+__global__ void __launch_bounds__(THREADS, 8) sort_copy_odd_kernel(const SortArgs a) {
   chain_wait();
   const int64_t step = (int64_t)gridDim.x * (THREADS / a.lanes);
   int64_t r = (int64_t)blockIdx.x * (THREADS / a.lanes) + threadIdx.x / a.lanes;
@@ -365,9 +357,10 @@ __device__ __forceinline__ const char* row_at(const void* rows, int64_t r, int b
 __device__ __forceinline__ char* row_at(void* rows, int64_t r, int bytes) { return static_cast<char*>(rows) + r * bytes; }
 
 // y[t] = sum over j of w[t, j] * rows[pos[t, j]], in the order of j, in 32 bits and rounded once.  J choices at a time and U
-// pieces of their rows, so that J * U loads are in flight together.
+// pieces of their rows, so that J * U loads are in flight together; odd rows, of which a piece is two loads and more registers, one at a
+// time in more warps (9460 x 658 bf16 with 8 choices 37 us, two choices at a time 48).
 template <typename T, typename W, bool ODD, int J, int U>
-__global__ void __launch_bounds__(THREADS) combine_kernel(const CombineArgs a) {
+__global__ void __launch_bounds__(THREADS, ODD ? 6 : 1) combine_kernel(const CombineArgs a) {
   constexpr int N = PER_PIECE<T>;
   const int64_t t = (int64_t)blockIdx.x * (THREADS / a.lanes) + threadIdx.x / a.lanes;
   const int l = threadIdx.x & (a.lanes - 1);
@@ -528,11 +521,11 @@ __global__ void __launch_bounds__(THREADS) combine_backward_kernel(const Combine
 }
 
 // Odd rows, a warp each: the choice that src names has its whole dot product there and its gradient's row to write.  Pieces are those of
-// the row that is written, so dy is put together anew for each of them.  Choice by choice of a token 165 us for 9460 x 658 bf16 with 8
-// choices.
+// the row that is written, so dy is put together anew for each of them.  Latency bounds it, so many warps beat many loads a warp: 9460 x
+// 658 bf16 with 8 choices 56 us (two pieces a lane and three blocks an SM 69, choice by choice of a token 165).
 template <typename T, typename W>
-__global__ void __launch_bounds__(THREADS) combine_backward_odd_kernel(const CombineArgs a) {
-  constexpr int N = PER_PIECE<T>, U = 2;
+__global__ void __launch_bounds__(THREADS, 5) combine_backward_odd_kernel(const CombineArgs a) {
+  constexpr int N = PER_PIECE<T>, U = 1;
   const int lane = threadIdx.x & 31;
   const int64_t warps = (int64_t)gridDim.x * (THREADS / 32), me = (int64_t)(threadIdx.x >> 5) * gridDim.x + blockIdx.x, choices = a.tokens * a.k;
   int next = me < a.n_rows ? a.src[me] : -1;
@@ -813,12 +806,12 @@ int launch_combine(const CombineArgs& a, bool backward, bool odd, cudaStream_t s
   const unsigned grid = blocks_for(a.tokens, a.lanes, backward && a.drows ? a.n_rows : 0);
   const bool one = a.bytes <= 16 * a.lanes;    // a piece a thread: fewer registers, more blocks on an SM
   if (backward) {
-    if (odd) combine_backward_odd_kernel<T, W><<<blocks_for(0, 32, a.n_rows), THREADS, 0, st>>>(a);
+    if (odd) combine_backward_odd_kernel<T, W><<<10 * sm_count(), THREADS, 0, st>>>(a);
     else if (one) combine_backward_kernel<T, W, 2, 1><<<grid, THREADS, 0, st>>>(a);
     else if (a.k <= 2) combine_backward_kernel<T, W, 2, 2><<<grid, THREADS, 0, st>>>(a);
     else combine_backward_kernel<T, W, 4, 2><<<grid, THREADS, 0, st>>>(a);
   } else {
-    if (odd) combine_kernel<T, W, true, 2, 1><<<grid, THREADS, 0, st>>>(a);
+    if (odd) combine_kernel<T, W, true, 1, 1><<<grid, THREADS, 0, st>>>(a);
     else if (one) combine_kernel<T, W, false, 4, 1><<<grid, THREADS, 0, st>>>(a);
     else if (a.k <= 2) combine_kernel<T, W, false, 2, 4><<<grid, THREADS, 0, st>>>(a);
     else combine_kernel<T, W, false, 4, 2><<<grid, THREADS, 0, st>>>(a);
@@ -889,7 +882,7 @@ extern "C" int i8l_sort_tokens(const void* x, const void* ids, int ids64, int64_
   I8L_CUDA_OK(launch(sort_count_kernel, dim3(a.blocks), THREADS, 0, st, a));
   I8L_CUDA_OK(launch(sort_place_kernel, dim3(a.blocks), THREADS, THREADS / 32 * experts * sizeof(int), st, a));
   if (odd) a.lanes = lanes_for(a.bytes, rows);
-  const int64_t row_blocks = (rows + THREADS / a.lanes - 1) / (THREADS / a.lanes), resident = 4 * sm_count();
+  const int64_t row_blocks = (rows + THREADS / a.lanes - 1) / (THREADS / a.lanes), resident = 16 * sm_count();
   const dim3 by_row((unsigned)(row_blocks < resident ? row_blocks : resident));
   I8L_CUDA_OK(!odd        ? launch(sort_copy_kernel, dim3(grid), THREADS, 0, st, a)
               : size == 4 ? launch(sort_copy_odd_kernel<uint32_t>, by_row, THREADS, 0, st, a)
