@@ -857,9 +857,9 @@ int run_few(const TokenArgs& a, cudaStream_t st) {
 
 // Tokens of a tile, from what the host knows: as if all rows belonged to experts, and to all alike.  A tile of s columns takes 0.4 + 0.6 *
 // s / 256 of a full one (less for the MMAs, as much for the weights and the rest), and up to three waves of tiles end with the
-// slowest.  us with 64, 128 and 256: dense 4096x4096 of 256 rows 12.6 / 13.3 / 16.0, 512 20.1 / 14.6 / 16.9, 1000 35 / 23 / 18.8;
-// 64 experts of 1408x4096 with 32 rows each 69 / 67 / 72, 100 102 / 87 / 91, 500 350 / 269 / 223.  Over 100 sizes the choice costs
-// 0.7 % against the best one, 9 % at most.
+// slowest.  us with 64, 128 and 256: dense 4096x4096 of 256 rows 13.3 / 13.9 / 16.0, 512 20.8 / 14.8 / 17.3, 1000 36 / 24 / 19.0;
+// 64 experts of 1408x4096 with 32 rows each 70 / 68 / 73, 100 100 / 88 / 92, 500 377 / 258 / 223.  Over 100 sizes the choice costs
+// 0.3 % against the best one, 8 % at most.
 int tile_tokens(const TokenArgs& a) {
   const int64_t segments = a.experts < a.rows ? a.experts : a.rows, average = (a.rows + segments - 1) / segments;
   const int64_t n_tiles = (a.N + CHANNELS - 1) / CHANNELS;
