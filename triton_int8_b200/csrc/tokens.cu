@@ -884,15 +884,17 @@ int tile_tokens(const TokenArgs& a) {
 }
 
 // CTAs that share a tile of 64 tokens, where there are few tiles and a long K: a share costs 2 us (the sums meet, clusters start later) and
-// saves its part of 0.18 us a K block; clusters of eight find few places.  us with 1, 2, 4 and 8: 9 rows x 512x8192 17.8 / 12.8 /
-// 9.6 / 8.0, 256 rows 18.8 / 14.7 / 11.6 / 17.3; 16 rows x 4096x11008 22.7 / 16.6 / 14.7 / 21.7, 128 rows 24.8 / 19.1 / 25.4 / 34;
-// 64 rows x 1000x2048 9.0 / 9.6 / 8.5 / 8.0, x 2176x1408 8.0 / 9.2 / 8.3 / 14.
+// saves its part of 0.17 us a K block; clusters of eight find few places, and 32 of four nearly all that there are.  us with 1, 2, 4
+// and 8: 9 rows x 512x8192 17.9 / 13.7 / 11.4 / 10.0, 256 rows 20.6 / 16.4 / 13.5 / 20.0; 16 rows x 4096x11008 23.6 / 17.8 / 16.0 /
+// 23.4, 128 rows 25.5 / 19.6 / 27.1 / 36.2; 64 rows x 4096x4096 13.9 / 13.5 / 14.7 / 20.6, x 4096x2048 10.5 / 11.4 / 13.1 / 19.2,
+// x 1000x2048 9.3 / 9.7 / 9.0 / 8.6, x 2176x1408 8.3 / 9.5 / 8.8 / 15.1.  9 rows x 4096x4096 lose by it: 12.7, and 11.8 with four.
 int k_split(const TokenArgs& a) {
   const int64_t segments = a.experts < a.rows ? a.experts : a.rows, average = (a.rows + segments - 1) / segments;
   const int64_t tiles = segments * ((average + 63) / 64) * ((a.N + CHANNELS - 1) / CHANNELS), blocks = (a.K + KBYTES - 1) / KBYTES;
   if (gemm_cta_budget() < sm_count()) return 1;   // some SMs are kept free, and clusters need whole groups of them
   if (blocks >= 16 && tiles <= 8) return 8;
-  if (blocks >= 16 && tiles <= 32) return 4;
+  if (blocks >= 16 && tiles <= 16) return 4;
+  if (blocks >= 64 && tiles <= 32) return 4;
   return blocks >= 24 && tiles <= 64 ? 2 : 1;
 }
 
