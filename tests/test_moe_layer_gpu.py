@@ -151,3 +151,26 @@ def test_decoder_layer_with_experts():
     plain = DecoderLayer(hidden=256, heads=4, mlp=384, device=DEV)
     assert len(plain.linears()) == 7 and plain(x.detach()).shape == x.shape
     K.check_status(DEV)
+
+
+@pytest.mark.parametrize("where", ["all", "up", "down"])
+def test_frozen_experts_keep_their_biases(where):
+    """Bit for bit what each expert's frozen linears give on its rows."""
+    built = []
+
+    def build(i, o):   # gates first, then ups, then downs
+        bias = where == "all" or where == ("gate", "up", "down")[len(built) // 5]
+        built.append(torch.nn.Linear(i, o, bias=bias, device=DEV, dtype=BF16))
+        return built[-1]
+
+    layer = _layer(7, linear=build).eval().freeze()
+    x = torch.randn(37, 256, device=DEV).to(BF16)
+    with torch.no_grad():
+        ids, weights = layer.route(x)
+        rows, offsets, pos, src = moe.sort_tokens(x, ids, 5)
+        ends, parts = offsets.tolist(), []
+        for e, (a, b) in enumerate(zip(ends, ends[1:])):
+            gate, up, down = (linear.Int8FrozenLinear.from_linear(m[e]) for m in (layer.gate_proj, layer.up_proj, layer.down_proj))
+            if b > a:
+                parts.append(down(F.silu(gate(rows[a:b])) * up(rows[a:b])))
+        assert torch.equal(layer(x), moe.combine(torch.cat(parts), weights, pos, src))

@@ -112,6 +112,13 @@ def expert_linear(rows: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, offset
     return K.token_linear(rows, wq, ws, offsets, bias, out_dtype)
 
 
+def _biases(linears):
+    """bf16 [len(linears), out_features], or None where no layer has one."""
+    if all(m.bias is None for m in linears):
+        return None
+    return torch.stack([m.weight.new_zeros(m.weight.shape[0]) if m.bias is None else m.bias for m in linears]).to(torch.bfloat16)
+
+
 class Int8MoE(nn.Module):
     """Gated experts: y[t] = sum over the top_k experts e of token t of p_e * down_e(silu(gate_e(x)) * up_e(x)), p = softmax over the logits of
     the chosen ones.  hidden and mlp are multiples of 128.
@@ -148,7 +155,10 @@ class Int8MoE(nn.Module):
     def freeze(self) -> "Int8MoE":
         gate_up = torch.stack([torch.cat([g.weight, u.weight]) for g, u in zip(self.gate_proj, self.up_proj)])
         down = torch.stack([d.weight for d in self.down_proj])
-        self._frozen = (*quantize_experts(gate_up), *quantize_experts(down))
+        bias = _biases([*self.gate_proj, *self.up_proj])
+        if bias is not None:   # an expert's gate in front of its up, as their weights are
+            bias = bias.view(2, self.experts, -1).transpose(0, 1).reshape(self.experts, -1)
+        self._frozen = (*quantize_experts(gate_up), bias, *quantize_experts(down), _biases(self.down_proj))
         return self
 
     def train(self, mode: bool = True):
@@ -165,10 +175,10 @@ class Int8MoE(nn.Module):
         x2 = x.reshape(-1, x.shape[-1])
         ids, weights = self.route(x2)
         if self._frozen is not None and not torch.is_grad_enabled():
-            gate_up_q, gate_up_s, down_q, down_s = self._frozen
+            gate_up_q, gate_up_s, gate_up_b, down_q, down_s, down_b = self._frozen
             rows, offsets, pos, src = sort_tokens(x2, ids, self.experts)
-            gate, up = expert_linear(rows, gate_up_q, gate_up_s, offsets).chunk(2, -1)
-            rows = expert_linear(F.silu(gate) * up, down_q, down_s, offsets)
+            gate, up = expert_linear(rows, gate_up_q, gate_up_s, offsets, gate_up_b).chunk(2, -1)
+            rows = expert_linear(F.silu(gate) * up, down_q, down_s, offsets, down_b)
         else:
             rows, offsets, pos, src = sort_tokens(x2, ids, self.experts, align=128)
             ends = offsets.tolist()
