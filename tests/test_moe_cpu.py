@@ -112,3 +112,11 @@ def test_wrappers_refuse_what_the_kernels_do_not_take():
             moe.expert_linear(tensor, wq[None], ws[None], None)
     with pytest.raises(RuntimeError, match="no gradient"):
         linear.linear_w8a8(x, wq, ws, torch.zeros(16, requires_grad=True))
+
+
+def test_frozen_linear_cast_leaves_the_scales():
+    from triton_int8_b200.linear import Int8FrozenLinear
+    scale = torch.rand(16)
+    frozen = Int8FrozenLinear(torch.zeros(16, 32, dtype=torch.int8), scale.clone(), torch.zeros(16)).to(torch.bfloat16)
+    assert torch.equal(frozen.weight_scale, scale) and frozen.bias.dtype == torch.bfloat16 and frozen.weight_q.dtype == torch.int8
+    assert torch.equal(frozen.state_dict()["weight_scale"], scale)

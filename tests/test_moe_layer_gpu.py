@@ -174,3 +174,11 @@ def test_frozen_experts_keep_their_biases(where):
             if b > a:
                 parts.append(down(F.silu(gate(rows[a:b])) * up(rows[a:b])))
         assert torch.equal(layer(x), moe.combine(torch.cat(parts), weights, pos, src))
+
+
+def test_frozen_linear_keeps_its_scales_when_it_is_cast():
+    torch.manual_seed(8)
+    frozen = linear.Int8Linear(256, 128, bias=True, device=DEV).freeze()
+    x = torch.randn(6, 256, device=DEV).to(BF16)
+    y = frozen(x)
+    assert torch.equal(frozen.to(BF16)(x), y) and frozen.weight_scale.dtype == torch.float32

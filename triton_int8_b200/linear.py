@@ -250,6 +250,13 @@ class Int8FrozenLinear(nn.Module):
         self.register_buffer("weight_scale", weight_scale)
         self.register_buffer("bias", bias)
 
+    def _apply(self, fn, *args, **kwargs):   # to(bfloat16) and the like leave the scales in 32 bits
+        scale = self.weight_scale
+        super()._apply(fn, *args, **kwargs)
+        if self.weight_scale.dtype != scale.dtype:
+            self.weight_scale = scale.to(self.weight_scale.device)
+        return self
+
     @classmethod
     def from_linear(cls, lin: nn.Module) -> "Int8FrozenLinear":
         """From Int8Linear or nn.Linear on a GPU, whose in_features are a multiple of 128."""
