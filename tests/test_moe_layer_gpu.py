@@ -182,3 +182,11 @@ def test_frozen_linear_keeps_its_scales_when_it_is_cast():
     x = torch.randn(6, 256, device=DEV).to(BF16)
     y = frozen(x)
     assert torch.equal(frozen.to(BF16)(x), y) and frozen.weight_scale.dtype == torch.float32
+
+
+def test_combine_checks_src_without_gradients_too():
+    rows, offsets, pos, src = moe.sort_tokens(torch.randn(9, 16, device=DEV), torch.zeros(9, 2, dtype=torch.int64, device=DEV), 3)
+    weights = torch.ones(9, 2, device=DEV)
+    for wrong, error in ((src[:-1], ValueError), (src.long(), TypeError), (src.cpu(), ValueError)):
+        with pytest.raises(error):
+            moe.combine(rows, weights, pos, wrong)

@@ -83,6 +83,9 @@ def combine(rows: torch.Tensor, weights: torch.Tensor, pos: torch.Tensor, src: t
         y = K.host().combine(rows, weights, pos, src)
         if y is not None:
             return y
+    K._check_ints(src, "src", tuple(rows.shape[:1]))   # also where no gradient will need it
+    if src.device != rows.device:
+        raise ValueError(f"rows are on {rows.device}, src on {src.device}")
     if torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
         return _CombineFn.apply(rows, weights, pos, src)
     return K.combine(rows, weights, pos)
