@@ -19,16 +19,16 @@ HEAD = r"""
 static uint32_t __umulhi(uint32_t a, uint32_t b) { return (uint32_t)((uint64_t)a * b >> 32); }
 static int __clz(int v) { return v ? __builtin_clz((unsigned)v) : 32; }
 struct TokenArgs { int experts; };
-struct GroupArgs { TokenArgs t; int n_tiles; };
+struct GroupArgs { TokenArgs t; int n_tiles, cap; uint32_t by_cap; };
 """
 TAIL = r"""
 static uint32_t by[RASTER + 1];
 static void init() { for (uint32_t w = 2; w <= RASTER; ++w) by[w] = 0xffffffffu / w + 1; }
-template <int TOK> static int cut(const int* rows, int experts, int n_tiles, Segment* seg) {
+static int cut(const GroupArgs& p, const int* rows, int experts, int n_tiles, Segment* seg) {
   init();
   int at = 0, first = 0;
   for (int e = 0; e < experts; ++e) {
-    const int count = rows[e], tiles = (count + TOK - 1) / TOK;
+    const int count = rows[e], tiles = tiles_of(count, p);
     seg[e].row = at; seg[e].rows = count;
     seg[e].share = tiles ? ((count + tiles - 1) / tiles + 15) & ~15 : 0;
     seg[e].first = first;
@@ -37,10 +37,10 @@ template <int TOK> static int cut(const int* rows, int experts, int n_tiles, Seg
   seg[experts].first = first;
   return first;
 }
-extern "C" int tiles(int tok, const int* rows, int experts, int n_tiles, int* out) {   // out: expert, channel, row, rows, columns, loaded
+extern "C" int tiles(int tok, int cap, const int* rows, int experts, int n_tiles, int* out) {   // out: expert, channel, row, rows, columns, loaded
   static Segment seg[2048];
-  const int total = tok == 64 ? cut<64>(rows, experts, n_tiles, seg) : tok == 128 ? cut<128>(rows, experts, n_tiles, seg) : cut<256>(rows, experts, n_tiles, seg);
-  GroupArgs p{{experts}, n_tiles};
+  const GroupArgs p{{experts}, n_tiles, cap / 16, 0xffffffffu / (cap / 16) + 1};
+  const int total = cut(p, rows, experts, n_tiles, seg);
   for (int t = 0; out && t < total; ++t, out += 6) {
     const Tile r = tok == 64 ? tile_of<64>(t, p, seg, by) : tok == 128 ? tile_of<128>(t, p, seg, by) : tile_of<256>(t, p, seg, by);
     out[0] = r.expert; out[1] = r.channel; out[2] = (int)r.row; out[3] = r.rows; out[4] = r.columns; out[5] = boxes_of(r.columns).tokens();
@@ -61,6 +61,7 @@ def lib(tmp_path_factory):
     parts = [_take(text, r"^constexpr int GRP_THREADS = [^;]*;"), _take(text, r"^constexpr int RASTER = [^;]*;"),
              _take(text, r"^struct __align__\(16\) Segment \{.*?^\};"), _take(text, r"^struct Tile \{.*?^\};"),
              _take(text, r"^struct Boxes \{.*?^\};"), _take(text, r"^__device__ __forceinline__ Boxes boxes_of.*?^\}"),
+             _take(text, r"^__device__ __forceinline__ int tiles_of.*?\}$"),
              _take(text, r"^template <int TOK>\n__device__ __forceinline__ Tile tile_of.*?^\}")]
     tmp = tmp_path_factory.mktemp("tiles")
     src, so = tmp / "tiles.cpp", tmp / "tiles.so"
@@ -69,23 +70,24 @@ def lib(tmp_path_factory):
     return ctypes.CDLL(str(so))
 
 
-@pytest.mark.parametrize("tok", [64, 128, 256])
-def test_every_token_and_channel_once(lib, tok):
-    rng = random.Random(tok)
-    cases = [[1], [16], [17], [63, 64, 65], [0, 0, 5, 0], [0], [255, 256, 257, 0, 1], [4096], [4097], [tok * 16], [tok * 16 + 1], [9000, 3], [1] * 300]
+@pytest.mark.parametrize("tok, cap", [(64, 64), (128, 128), (256, 256), (128, 80), (128, 96), (256, 144), (256, 240)])
+def test_every_token_and_channel_once(lib, tok, cap):
+    rng = random.Random(cap)
+    cases = [[1], [16], [17], [63, 64, 65], [0, 0, 5, 0], [0], [255, 256, 257, 0, 1], [4096], [4097], [cap * 16], [cap * 16 + 1], [9000, 3], [1] * 300]
     cases += [[rng.choice([0, 1, 7, rng.randrange(2000)]) for _ in range(rng.randrange(1, 40))] for _ in range(20)]
     for rows in cases:
         for n_tiles in (1, 3, 17):
             arr = (ctypes.c_int * len(rows))(*rows)
-            total = lib.tiles(tok, arr, len(rows), n_tiles, None)
-            assert total <= (sum(rows) // tok + sum(1 for r in rows if r)) * n_tiles   # what the host reckons with
+            total = lib.tiles(tok, cap, arr, len(rows), n_tiles, None)
+            assert total == sum(-(-r // cap) for r in rows) * n_tiles
+            assert total <= (sum(rows) // cap + sum(1 for r in rows if r)) * n_tiles   # what the host reckons with
             out = (ctypes.c_int * max(1, 6 * total))()
-            lib.tiles(tok, arr, len(rows), n_tiles, out)
+            lib.tiles(tok, cap, arr, len(rows), n_tiles, out)
             begin = [sum(rows[:e]) for e in range(len(rows))]
             seen = {}
             for t in range(total):
                 e, channel, row, count, columns, loaded = out[6 * t:6 * t + 6]
-                assert 0 < count <= columns <= tok and columns % 16 == 0 and columns - count < 16
+                assert 0 < count <= columns <= cap and columns % 16 == 0 and columns - count < 16
                 assert columns <= loaded <= tok and channel % 128 == 0 and 0 <= channel < 128 * n_tiles
                 assert begin[e] <= row and row + count <= begin[e] + rows[e]
                 seen.setdefault((e, channel), []).append((row, row + count))

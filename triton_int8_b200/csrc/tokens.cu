@@ -391,6 +391,8 @@ struct GroupArgs {
   uint32_t max_polls;
   int n_tiles, withhold;
   int most;   // tiles there can be
+  int cap;    // tokens of a tile at most, in sixteens: TOK or fewer
+  uint32_t by_cap;   // 2^32 / cap rounded up
   int64_t x_stride;
 };
 struct __align__(16) GroupCtl {
@@ -425,6 +427,8 @@ __device__ __forceinline__ Boxes boxes_of(int columns) {
   return Boxes{up - 1, rest <= 16 ? 0 : 32 - __clz((rest - 1) >> 4)};
 }
 
+__device__ __forceinline__ int tiles_of(int rows, const GroupArgs& p) { return (int)__umulhi((uint32_t)(((rows + 15) >> 4) + p.cap - 1), p.by_cap); }
+
 // Divisions by numbers that are not known at compile time cost a tile some 500 cycles, which every role goes through: the quotient
 // that the rows of a segment need is in the table, more than one group of token tiles makes a tile long enough, and the last one is a
 // multiplication.  by[w]: 2^32 / w rounded up, exact for numbers below 2^28 (16 * channels / 128) and w up to 16.
@@ -437,7 +441,7 @@ __device__ __forceinline__ Tile tile_of(int t, const GroupArgs& p, const Segment
     else hi = mid;
   }
   const Segment s = seg[lo];
-  const int tiles = (s.rows + TOK - 1) / TOK, local = t - s.first, per_group = RASTER * p.n_tiles;
+  const int tiles = tiles_of(s.rows, p), local = t - s.first, per_group = RASTER * p.n_tiles;
   const int group = tiles <= RASTER ? 0 : local / per_group, g0 = group * RASTER;
   const int width = tiles - g0 < RASTER ? tiles - g0 : RASTER, at = local - group * per_group;
   const int n = width == 1 ? at : (int)__umulhi((uint32_t)at, by[width]), m = g0 + at - n * width;
@@ -512,7 +516,7 @@ group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
   for (int e = threadIdx.x; e < p.t.experts; e += GRP_THREADS) {
     int64_t b, n;
     segment(p.t, e, b, n);
-    const int count = (int)(n - b), tiles = (count + TOK - 1) / TOK;
+    const int count = (int)(n - b), tiles = tiles_of(count, p);
     seg[e].row = (int)b;
     seg[e].rows = count;
     seg[e].share = tiles ? ((count + tiles - 1) / tiles + 15) & ~15 : 0;   // equal tiles rather than full ones and a rest
@@ -855,18 +859,19 @@ int run_few(const TokenArgs& a, cudaStream_t st) {
   return launch_few(few_mma_kernel, allowed[3], a, MMA_CHANNELS, 1, st, (int)few_row_bytes(a.rows, a.K));
 }
 
-// Tokens of a tile, from what the host knows: as if all rows belonged to experts, and to all alike.  A tile of s columns takes 0.4 + 0.6 *
+// Most tokens of a tile, from what the host knows: as if all rows belonged to experts, and to all alike.  A tile of s columns takes 0.4 + 0.6 *
 // s / 256 of a full one (less for the MMAs, as much for the weights and the rest), and up to three waves of tiles end with the
 // slowest.  us with 64, 128 and 256: dense 4096x4096 of 256 rows 13.3 / 13.9 / 16.0, 512 20.8 / 14.8 / 17.3, 1000 36 / 24 / 19.0;
 // 64 experts of 1408x4096 with 32 rows each 70 / 68 / 73, 100 100 / 88 / 92, 500 377 / 258 / 223.  Over 100 sizes the choice costs
-// 0.3 % against the best one, 8 % at most.
+// 0.3 % against the best one, 8 % at most.  Where there is one segment the tiles are known, and any multiple of 16 from 64 on may fill the
+// waves better: 439 rows x 9688x7280 48.9 -> 44.3 (160 for 256), 970 x 4768x4096 27.6 -> 25.3, 1705 x 1472x4096 20.0 -> 18.4 (144).
 int tile_tokens(const TokenArgs& a) {
   const int64_t segments = a.experts < a.rows ? a.experts : a.rows, average = (a.rows + segments - 1) / segments;
   const int64_t n_tiles = (a.N + CHANNELS - 1) / CHANNELS;
   const int sms = gemm_cta_budget();
   int best = 0;
   double least = 0;
-  for (int t = 64; t <= 256; t *= 2) {
+  for (int t = 64; t <= 256; t = segments == 1 ? t + 16 : t * 2) {
     double per = 1;   // tiles of a segment; uneven ones need half a tile more than their average
     if (segments == 1) per = (double)((average + t - 1) / t);
     else if (average * 4 > t * 3) per = (double)average / t + 0.5;
@@ -874,7 +879,7 @@ int tile_tokens(const TokenArgs& a) {
     int64_t share = ((average + (int64_t)per - 1) / (int64_t)per + 15) / 16 * 16;
     if (share > t) share = t;
     const double tiles = (double)segments * per * (double)n_tiles, waves = tiles / sms;
-    const double cost = (waves < 3 ? (double)(((int64_t)tiles + sms - 1) / sms) : waves + 0.5) * (0.4 + 0.6 * (double)share / 256);
+    const double cost = (segments == 1 || waves < 3 ? (double)(((int64_t)tiles + sms - 1) / sms) : waves + 0.5) * (0.4 + 0.6 * (double)share / 256);
     if (!best || cost < least) {
       best = t;
       least = cost;
@@ -904,7 +909,7 @@ template <int TOK, int SPLIT = 1> int launch_group(const int8_t* xq, GroupArgs& 
   const TokenArgs& a = p.t;
   I8L_CUDA_OK(allow_smem(group_kernel<TOK, SPLIT>, allowed, G::smem(MAX_EXPERTS)));
   p.n_tiles = (int)((a.N + CHANNELS - 1) / CHANNELS);
-  const int64_t most = (a.rows / TOK + (a.experts < a.rows ? a.experts : a.rows)) * p.n_tiles;   // tiles, whatever the offsets
+  const int64_t most = (a.rows / (16 * p.cap) + (a.experts < a.rows ? a.experts : a.rows)) * p.n_tiles;   // tiles, whatever the offsets
   if (most >= (1ll << 31)) return fail(I8L_ERR_SHAPE, "i8l_token_linear: too large for 32-bit tile numbers");
   p.most = (int)most;
   CUtensorMap mw;
@@ -982,11 +987,13 @@ extern "C" int i8l_token_linear(const void* x, const int8_t* w_q, const float* w
   p.max_polls = gemm_wait_limit();
   p.withhold = gemm_withhold();
   const int tok = tile_tokens(a);
+  p.cap = tok / 16;
+  p.by_cap = 0xffffffffu / p.cap + 1;
   if (tok == 64) switch (k_split(a)) {
       case 8: return launch_group<64, 8>(xq, p, st);
       case 4: return launch_group<64, 4>(xq, p, st);
       case 2: return launch_group<64, 2>(xq, p, st);
     }
-  if (tok == 128) return launch_group<128>(xq, p, st);
-  return tok == 256 ? launch_group<256>(xq, p, st) : launch_group<64>(xq, p, st);
+  if (tok == 64) return launch_group<64>(xq, p, st);
+  return tok <= 128 ? launch_group<128>(xq, p, st) : launch_group<256>(xq, p, st);
 }
