@@ -39,6 +39,7 @@ DENSE = [   # rows, N, K: one row to many, sizes that fill no tile
     (33, 128, 112), (63, 520, 512), (64, 64, 64), (65, 72, 2064), (127, 384, 256), (128, 128, 128), (129, 136, 144), (255, 1000, 272), (257, 264, 400),
     (300, 128, 16), (1000, 2176, 1408), (2048, 512, 1024), (1, 64, 131072), (4, 72, 81936), (40, 72, 40976),
     (20, 200, 2064), (50, 1288, 2304), (100, 3016, 3200), (64, 1024, 4096), (65, 1024, 4096), (129, 2048, 3088),   # K shared by a cluster
+    (700, 2200, 272), (333, 9480, 48), (970, 4768, 144), (439, 9688, 80), (900, 3208, 400), (1537, 2056, 112),   # tiles of 96, 112, 144, 160, 192, 208
 ]
 
 
