@@ -745,7 +745,7 @@ quant_row_kernel(const __nv_bfloat16* __restrict__ x, int64_t cols, int8_t* __re
 // eight 16-byte pieces each, between the maximum and the quantization: one read, no second sweep through the
 // caches, and rows of 4096 elements do not leave half of a CTA idle.  Bound by HBM.  [11008, 4096] 39 -> 29 us,
 // [4096, 4096] 19.5 -> 15.4, [28672, 8192] 115.6 -> 109.4 (6.4 TB/s) against two sweeps by one CTA per row.
-template <int MODE, int T>
+template <int MODE, int T, int P = 8>
 __device__ __forceinline__ void
 quant_row_cached_body(unsigned block, const __nv_bfloat16* __restrict__ x, int64_t rows, int64_t cols, int8_t* __restrict__ q,
                         float* __restrict__ scale, int first, int64_t stride = 0) {
@@ -756,12 +756,12 @@ quant_row_cached_body(unsigned block, const __nv_bfloat16* __restrict__ x, int64
   const uint4* xr = reinterpret_cast<const uint4*>(x + row * cols);
   const int nchunks = live ? (int)(cols / 8) : 0;
   chain_start(first);
-  uint4 cache[8];
+  uint4 cache[P];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) cache[i] = i * T + t < nchunks ? chain_load(xr + i * T + t) : make_uint4(0, 0, 0, 0);
+  for (int i = 0; i < P; ++i) cache[i] = i * T + t < nchunks ? chain_load(xr + i * T + t) : make_uint4(0, 0, 0, 0);
   __nv_bfloat162 hm = __floats2bfloat162_rn(0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < P; ++i) {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&cache[i]);
 #pragma unroll
     for (int k = 0; k < 4; ++k) hm = __hmax2_nan(hm, __habs2(h[k]));
@@ -771,7 +771,7 @@ quant_row_cached_body(unsigned block, const __nv_bfloat16* __restrict__ x, int64
   if (!finite) {   // the maximum leaves NaNs out
     hm = __floats2bfloat162_rn(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) hm = absmax8(cache[i], hm);
+    for (int i = 0; i < P; ++i) hm = absmax8(cache[i], hm);
     m = hmax_of(hm);
   }
 #pragma unroll
@@ -789,7 +789,7 @@ quant_row_cached_body(unsigned block, const __nv_bfloat16* __restrict__ x, int64
   if (live && t == 0) scale[row] = stored;
   uint2* qr = reinterpret_cast<uint2*>(q + row * (stride ? stride : cols));
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < P; ++i)
     if (i * T + t < nchunks) qr[i * T + t] = finite ? quant_piece_finite<MODE>(cache[i], s) : quant_piece<MODE>(cache[i], s);
   chain_wait();
 }
@@ -1264,8 +1264,11 @@ extern "C" int i8l_quant_tile(const void* x, int64_t batch, int64_t rows, int64_
 
 namespace i8l {
 // The rows of a product for serving: any multiple of 8 columns, and none of the rows from *limit on, which belong to nobody.
-template <int T>
-__global__ void __launch_bounds__(256)
+// Rows of up to three quarters of what the threads could hold keep six pieces each instead of eight, in 64 registers: four blocks on an SM
+// instead of three.  With a product of 8 channels behind it, us: 32768 x 1408 37.1 -> 33.8, 7996 x 1408 16.9 -> 15.9, 20000 x 10240
+// 156 -> 148; few or short rows as before.
+template <int T, int P>
+__global__ void __launch_bounds__(256, P == 8 ? 3 : 4)
 quant_token_kernel(const __nv_bfloat16* __restrict__ x, int64_t rows, int64_t cols, int8_t* __restrict__ q, int64_t stride,
                    float* __restrict__ scale, const int32_t* limit, int first) {
   chain_start(first);
@@ -1274,7 +1277,7 @@ quant_token_kernel(const __nv_bfloat16* __restrict__ x, int64_t rows, int64_t co
     rows = end < rows ? end : rows;
     if ((int64_t)blockIdx.x * (256 / T) >= rows) return;
   }
-  quant_row_cached_body<I8L_QMODE_ROWRCP, T>(blockIdx.x, x, rows, cols, q, scale, 0, stride);
+  quant_row_cached_body<I8L_QMODE_ROWRCP, T, P>(blockIdx.x, x, rows, cols, q, scale, 0, stride);
 }
 int quant_token_rows(const void* x, int64_t rows, int64_t cols, int8_t* q, int64_t stride, float* scale, const int32_t* limit,
                      cudaStream_t st) {
@@ -1282,12 +1285,16 @@ int quant_token_rows(const void* x, int64_t rows, int64_t cols, int8_t* q, int64
   auto cached = [&](auto kernel, int per_block) {
     return launch(kernel, dim3((unsigned)((rows + per_block - 1) / per_block)), 256, 0, st, xp, rows, cols, q, stride, scale, limit, chain_first());
   };
-  I8L_CUDA_OK(cols <= 512     ? cached(quant_token_kernel<8>, 32)   // short rows: no lanes without a piece
-              : cols <= 1024  ? cached(quant_token_kernel<16>, 16)
-              : cols <= 2048  ? cached(quant_token_kernel<32>, 8)
-              : cols <= 4096  ? cached(quant_token_kernel<64>, 4)
-              : cols <= 8192  ? cached(quant_token_kernel<128>, 2)
-              : cols <= 16384 ? cached(quant_token_kernel<256>, 1)
+  auto pick = [&](auto threads) {
+    constexpr int T = threads();
+    return cols <= 6 * 8 * T ? cached(quant_token_kernel<T, 6>, 256 / T) : cached(quant_token_kernel<T, 8>, 256 / T);
+  };
+  I8L_CUDA_OK(cols <= 512     ? pick(std::integral_constant<int, 8>{})   // short rows: no lanes without a piece
+              : cols <= 1024  ? pick(std::integral_constant<int, 16>{})
+              : cols <= 2048  ? pick(std::integral_constant<int, 32>{})
+              : cols <= 4096  ? pick(std::integral_constant<int, 64>{})
+              : cols <= 8192  ? pick(std::integral_constant<int, 128>{})
+              : cols <= 16384 ? pick(std::integral_constant<int, 256>{})
                               : launch(quant_row_kernel<I8L_QMODE_ROWRCP, false>, dim3((unsigned)rows), 256, 0, st, xp, cols, q, scale, chain_first()));
   return I8L_OK;
 }
