@@ -323,8 +323,10 @@ Tensor combine(const Tensor& rows, const Tensor& weights, const Tensor& pos) {
         dev);
   return y;
 }
+bool forward_mode(const Tensor& t) { return t._fw_grad(0).defined(); }
 // A gradient that came in, as the kernels read it.
 Tensor incoming(const char* name, const Tensor& d) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!forward_mode(d), "the gradient of ", name, " has no forward-mode derivative");
   const Tensor dy = d.contiguous();
   TORCH_CHECK(plain_thread() && dense(dy), name, ": its gradient cannot be taken under a transform or of a tensor subclass");
   return dy;
@@ -399,7 +401,6 @@ bool exact_tensor(PyObject* o) { return THPVariable_CheckExact(o); }
 bool ints(const Tensor& t, const Tensor& like, at::IntArrayRef shape) {
   return t.scalar_type() == at::kInt && dense(t) && t.device() == like.device() && t.sizes() == shape;
 }
-bool forward_mode(const Tensor& t) { return t._fw_grad(0).defined(); }
 bool at_16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 
 // sort_tokens(x, ids, experts, align) -> (rows, offsets, pos, src), or None

@@ -533,6 +533,14 @@ def token_linear(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, offsets=No
 def refuse_gradient(name: str, *tensors) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{name} has no gradient (its weights are int8): call it under torch.no_grad(), train with Int8Linear")
+    refuse_tangent(name, *tensors)
+
+
+def refuse_tangent(name: str, *tensors) -> None:
+    """A launch sees plain memory only: the derivative of a dual tensor would be lost without a word."""
+    ad = torch.autograd.forward_ad
+    if ad._current_level >= 0 and any(t is not None and ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:

@@ -39,6 +39,7 @@ class _SortFn(torch.autograd.Function):
     def backward(ctx, drows, *_):
         if drows is None:
             return None, None, None, None
+        K.refuse_tangent("the gradient of sort_tokens", drows)
         dx = K.combine(drows.detach(), None, ctx.saved_tensors[0])   # a token's gradient is the sum of its rows'
         return *_once("sort_tokens", [drows], dx), None, None, None
 
@@ -53,6 +54,7 @@ class _CombineFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         saved = ctx.saved_tensors
+        K.refuse_tangent("the gradient of combine", dy)
         grads = K.combine_backward(*(t.detach() for t in saved), dy.detach(), ctx.needs_input_grad[0], ctx.needs_input_grad[1])
         return *_once("combine", [dy, *saved], *grads), None, None
 
@@ -70,6 +72,7 @@ def sort_tokens(x: torch.Tensor, ids: torch.Tensor, experts: int, align: int = 1
         done = K.host().sort_tokens(x, ids, experts, align)
         if done is not None:
             return done
+    K.refuse_tangent("sort_tokens", x)
     if torch.is_grad_enabled() and x.requires_grad:
         return _SortFn.apply(x, ids, experts, align)
     return K.sort_tokens(x, ids, experts, align)
@@ -83,6 +86,7 @@ def combine(rows: torch.Tensor, weights: torch.Tensor, pos: torch.Tensor, src: t
         y = K.host().combine(rows, weights, pos, src)
         if y is not None:
             return y
+    K.refuse_tangent("combine", rows, weights)
     K._check_ints(src, "src", tuple(rows.shape[:1]))   # also where no gradient will need it
     if src.device != rows.device:
         raise ValueError(f"rows are on {rows.device}, src on {src.device}")
