@@ -2,6 +2,7 @@
 current CUDA stream.  These are the building blocks of the fwd_32 / bwd_33 variants."""
 from __future__ import annotations
 
+import sys
 import threading
 
 import torch
@@ -534,6 +535,7 @@ def refuse_gradient(name: str, *tensors) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{name} has no gradient (its weights are int8): call it under torch.no_grad(), train with Int8Linear")
     refuse_tangent(name, *tensors)
+    refuse_proxies(name)
 
 
 def refuse_tangent(name: str, *tensors) -> None:
@@ -541,6 +543,25 @@ def refuse_tangent(name: str, *tensors) -> None:
     ad = torch.autograd.forward_ad
     if ad._current_level >= 0 and any(t is not None and ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError(f"{name} has no forward-mode derivative")
+
+
+def refuse_proxies(name: str) -> None:
+    """A graph of operators (make_fx) would hold the allocation of a result and no launch."""
+    proxies = sys.modules.get("torch.fx.experimental.proxy_tensor")   # not imported: nobody records
+    if proxies is not None and proxies.get_proxy_mode() is not None:
+        raise RuntimeError(f"{name} cannot be recorded by make_fx: its kernels are no torch operators")
+
+
+class untraced:
+    """Inside a Python function that torch.jit.trace records as one node: sizes are plain numbers, and nothing else is recorded."""
+
+    def __enter__(self):
+        self.state = torch._C._get_tracing_state()
+        torch._C._set_tracing_state(None)
+
+    def __exit__(self, *exc):
+        torch._C._set_tracing_state(self.state)
+        return False
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:

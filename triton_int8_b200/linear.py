@@ -157,6 +157,19 @@ def linear_backward(dy2: torch.Tensor, weight: torch.Tensor, saved_xt, cfg: Int8
     return dx, dw
 
 
+class TokenLinearFn(torch.autograd.Function):
+    """K.token_linear as one node of a trace, which would see the allocation of y otherwise and nothing that fills it."""
+
+    @staticmethod
+    def forward(ctx, x, wq, ws, offsets, bias, out_dtype):
+        with K.untraced():
+            return K.token_linear(x, wq, ws, offsets, bias, out_dtype)
+
+    @staticmethod
+    def backward(ctx, dy):
+        raise RuntimeError("the product with kept weights has no gradient")
+
+
 def linear_w8a8(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, bias=None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The product for serving, with weights that were quantized once: x bf16 [..., K], wq int8 [N, K], ws fp32 [N], bias bf16 [N]
     -> [..., N], bf16 or fp32.  One scale a row of x and one an output channel, as double_channel has them
@@ -169,7 +182,8 @@ def linear_w8a8(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, bias=None, 
     K.refuse_gradient("linear_w8a8", x, ws, bias)
     if wq.dim() != 2 or ws.dim() != 1 or (bias is not None and bias.dim() != 1):
         raise ValueError("linear_w8a8: wq [N, K], ws [N], bias [N]")
-    y = K.token_linear(x.reshape(-1, x.shape[-1]), wq[None], ws[None], None, None if bias is None else bias[None], out_dtype)
+    product = TokenLinearFn.apply if torch.jit.is_tracing() else K.token_linear
+    y = product(x.reshape(-1, x.shape[-1]), wq[None], ws[None], None, None if bias is None else bias[None], out_dtype)
     return y.view(*x.shape[:-1], wq.shape[0])
 
 

@@ -15,7 +15,7 @@ from torch import nn
 
 from . import _lib as L
 from . import kernels as K
-from .linear import DEFAULT, Int8Config, Int8Linear
+from .linear import DEFAULT, Int8Config, Int8Linear, TokenLinearFn
 
 
 def _once(name: str, inputs, *results):
@@ -29,7 +29,8 @@ def _once(name: str, inputs, *results):
 class _SortFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, ids, experts, align):
-        rows, offsets, pos, src = K.sort_tokens(x, ids, experts, align)
+        with K.untraced():
+            rows, offsets, pos, src = K.sort_tokens(x, ids, experts, align)
         ctx.mark_non_differentiable(offsets, pos, src)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(pos)
@@ -47,9 +48,10 @@ class _SortFn(torch.autograd.Function):
 class _CombineFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, weights, pos, src):
-        src = K._check_ints(src, "src", (rows.shape[0],))
-        ctx.save_for_backward(rows, weights, pos, src)
-        return K.combine(rows, weights, pos)
+        with K.untraced():
+            src = K._check_ints(src, "src", (rows.shape[0],))
+            ctx.save_for_backward(rows, weights, pos, src)
+            return K.combine(rows, weights, pos)
 
     @staticmethod
     def backward(ctx, dy):
@@ -73,7 +75,8 @@ def sort_tokens(x: torch.Tensor, ids: torch.Tensor, experts: int, align: int = 1
         if done is not None:
             return done
     K.refuse_tangent("sort_tokens", x)
-    if torch.is_grad_enabled() and x.requires_grad:
+    K.refuse_proxies("sort_tokens")
+    if torch.jit.is_tracing() or (torch.is_grad_enabled() and x.requires_grad):   # a trace records the function, not the launches
         return _SortFn.apply(x, ids, experts, align)
     return K.sort_tokens(x, ids, experts, align)
 
@@ -87,10 +90,11 @@ def combine(rows: torch.Tensor, weights: torch.Tensor, pos: torch.Tensor, src: t
         if y is not None:
             return y
     K.refuse_tangent("combine", rows, weights)
+    K.refuse_proxies("combine")
     K._check_ints(src, "src", tuple(rows.shape[:1]))   # also where no gradient will need it
     if src.device != rows.device:
         raise ValueError(f"rows are on {rows.device}, src on {src.device}")
-    if torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
+    if torch.jit.is_tracing() or (torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad)):
         return _CombineFn.apply(rows, weights, pos, src)
     return K.combine(rows, weights, pos)
 
@@ -116,6 +120,8 @@ def expert_linear(rows: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, offset
     K.refuse_gradient("expert_linear", rows, ws, bias)
     if offsets is None:
         raise ValueError("expert_linear: offsets are needed (linear_w8a8 takes one matrix for all rows)")
+    if torch.jit.is_tracing():
+        return TokenLinearFn.apply(rows, wq, ws, offsets, bias, out_dtype)
     return K.token_linear(rows, wq, ws, offsets, bias, out_dtype)
 
 
@@ -187,6 +193,9 @@ class Int8MoE(nn.Module):
             gate, up = expert_linear(rows, gate_up_q, gate_up_s, offsets, gate_up_b).chunk(2, -1)
             rows = expert_linear(F.silu(gate) * up, down_q, down_s, offsets, down_b)
         else:
+            if torch.jit.is_tracing():
+                raise RuntimeError("Int8MoE reads the sizes of its experts' segments from the device and a trace would keep them: trace a frozen "
+                                   "layer (freeze()), without gradients")
             rows, offsets, pos, src = sort_tokens(x2, ids, self.experts, align=128)
             ends = offsets.tolist()
             parts = []
