@@ -132,6 +132,10 @@ def _biases(linears):
     return torch.stack([m.weight.new_zeros(m.weight.shape[0]) if m.bias is None else m.bias for m in linears]).to(torch.bfloat16)
 
 
+def _thaw_loaded(module, keys) -> None:   # a function of the module's: the layer can be pickled
+    module._thaw()
+
+
 class Int8MoE(nn.Module):
     """Gated experts: y[t] = sum over the top_k experts e of token t of p_e * down_e(silu(gate_e(x)) * up_e(x)), p = softmax over the logits of
     the chosen ones.  hidden and mlp are multiples of 128.
@@ -155,7 +159,7 @@ class Int8MoE(nn.Module):
         self.up_proj = nn.ModuleList(linear(hidden, mlp) for _ in range(experts))
         self.down_proj = nn.ModuleList(linear(mlp, hidden) for _ in range(experts))
         self._frozen = None
-        self.register_load_state_dict_post_hook(lambda module, keys: module._thaw())
+        self.register_load_state_dict_post_hook(_thaw_loaded)
 
     def _thaw(self) -> None:
         self._frozen = None
