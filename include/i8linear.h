@@ -347,8 +347,9 @@ I8L_API int i8l_sort_tokens(const void* x, const void* ids, int ids64, int64_t t
  * [n_rows, cols] and y [tokens, cols] of `dtype`, weights [tokens, k] of fp32 or `dtype` (wdtype), NULL for ones (the gradient of
  * i8l_sort_tokens).  A choice whose pos is outside [0, n_rows) adds nothing, whatever its weight.
  * i8l_combine_backward: drows[pos[t, j]] = weights[t, j] * dy[t], rows whose src is negative zero, and dweights[t, j] = the sum of
- * dy[t] * rows[pos[t, j]] in fp32, zero for dropped choices; either may be NULL.  pos and src are inverse to one another, as
- * i8l_sort_tokens makes them; where they are not, the gradients are undefined, but nothing outside of them is touched.
+ * dy[t] * rows[pos[t, j]] in fp32, zero for dropped choices; either of these two may be NULL, src may not.  pos and src are inverse
+ * to one another, as i8l_sort_tokens makes them; where they are not, the gradients are undefined, but nothing outside of them is
+ * touched.
  * No counterpart in the reference.
  */
 I8L_API int i8l_combine(const void* rows, const void* weights, const int32_t* pos, int64_t n_rows, int64_t tokens, int64_t cols,

@@ -910,7 +910,7 @@ extern "C" int i8l_combine_backward(const void* rows, const void* weights, const
                                     void* stream) {
   if (int e = check_rows("i8l_combine_backward", tokens, cols, n_rows, k, dtype, wdtype)) return e;
   if ((!tokens || !dweights) && (!n_rows || !drows)) return I8L_OK;
-  if ((tokens && (!pos || !dy || !weights)) || (n_rows && (!rows || (drows && !src)))) return fail(I8L_ERR_ARG, "i8l_combine_backward: null pointer");
+  if ((tokens && (!pos || !dy || !weights)) || (n_rows && (!rows || !src))) return fail(I8L_ERR_ARG, "i8l_combine_backward: null pointer");
   const int size = elem_size(dtype);
   const int wsize = wdtype == I8L_DTYPE_F32 ? 4 : 2;
   if (!aligned_to(rows, size) || !aligned_to(dy, size) || !aligned_to(drows, size) || !aligned_to(weights, wsize) || !aligned_to(dweights, wsize))
