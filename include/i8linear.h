@@ -350,7 +350,7 @@ I8L_API int i8l_sort_tokens(const void* x, const void* ids, int ids64, int64_t t
  * dy[t] * rows[pos[t, j]] in fp32, zero for dropped choices; either of these two may be NULL, src may not.  pos and src are inverse
  * to one another, as i8l_sort_tokens makes them; where they are not, the gradients are undefined, but nothing outside of them is
  * touched.
- * No counterpart in the reference.
+ * Pointers are aligned to their elements.  No counterpart in the reference.
  */
 I8L_API int i8l_combine(const void* rows, const void* weights, const int32_t* pos, int64_t n_rows, int64_t tokens, int64_t cols,
                    int k, int dtype, int wdtype, void* y, void* stream);
@@ -367,7 +367,7 @@ I8L_API int i8l_combine_backward(const void* rows, const void* weights, const in
  *   of offsets[0] and from offsets[experts] on come out zero.  Offsets outside [0, rows] are cut off; if they decrease y is
  *   undefined, but nothing outside of it is touched.
  * N a multiple of 8, K of 16 and at most 131072 (the int32 sum cannot overflow), experts <= 1024, rows from 0 to 2^30.  x, w_q, y, bias
- * 16-byte aligned.  workspace: i8l_token_linear_workspace bytes, 256-byte aligned, may be NULL where that is 0.
+ * 16-byte aligned, w_scale, offsets and status to their elements.  workspace: i8l_token_linear_workspace bytes, 256-byte aligned, may be NULL where that is 0.
  * The row and channel scales are those of the reference's double_channel variant (triton/double-channle_fwd32.py:295-311).
  */
 I8L_API int64_t i8l_token_linear_workspace(int64_t rows, int experts, int64_t N, int64_t K);

@@ -854,7 +854,8 @@ extern "C" int i8l_sort_tokens(const void* x, const void* ids, int ids64, int64_
   if (rows < need) return fail(I8L_ERR_SHAPE, "i8l_sort_tokens: %lld rows, %lld are needed", (long long)rows, (long long)need);
   if (!offsets || (tokens && (!x || !ids || !pos)) || (rows && (!out || !src))) return fail(I8L_ERR_ARG, "i8l_sort_tokens: null pointer");
   const int size = elem_size(dtype);
-  if (!aligned_to(x, size) || !aligned_to(out, size) || !aligned_to(ids, ids64 ? 8 : 4))
+  if (!aligned_to(x, size) || !aligned_to(out, size) || !aligned_to(ids, ids64 ? 8 : 4) || !aligned_to(offsets, 4) || !aligned_to(pos, 4) ||
+      !aligned_to(src, 4) || !aligned_to(workspace, 4))
     return fail(I8L_ERR_ALIGN, "i8l_sort_tokens: pointers are aligned to their elements");
   if (workspace_bytes < i8l_sort_workspace(tokens, k, experts) || (i8l_sort_workspace(tokens, k, experts) && !workspace))
     return fail(I8L_ERR_ARG, "i8l_sort_tokens: workspace of %lld bytes is too small", (long long)workspace_bytes);
@@ -913,7 +914,8 @@ extern "C" int i8l_combine_backward(const void* rows, const void* weights, const
   if ((tokens && (!pos || !dy || !weights)) || (n_rows && (!rows || !src))) return fail(I8L_ERR_ARG, "i8l_combine_backward: null pointer");
   const int size = elem_size(dtype);
   const int wsize = wdtype == I8L_DTYPE_F32 ? 4 : 2;
-  if (!aligned_to(rows, size) || !aligned_to(dy, size) || !aligned_to(drows, size) || !aligned_to(weights, wsize) || !aligned_to(dweights, wsize))
+  if (!aligned_to(rows, size) || !aligned_to(dy, size) || !aligned_to(drows, size) || !aligned_to(weights, wsize) || !aligned_to(dweights, wsize) ||
+      !aligned_to(pos, 4) || !aligned_to(src, 4))
     return fail(I8L_ERR_ALIGN, "i8l_combine_backward: pointers are aligned to their elements");
   if (int e = check_arch()) return e;
   CombineArgs a{};

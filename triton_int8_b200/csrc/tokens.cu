@@ -962,6 +962,8 @@ extern "C" int i8l_token_linear(const void* x, const int8_t* w_q, const float* w
   if (!w_q || !w_scale || (rows && (!x || !y))) return fail(I8L_ERR_ARG, "i8l_token_linear: null pointer");
   if (!aligned16(x) || !aligned16(w_q) || !aligned16(y) || !aligned16(bias) || (reinterpret_cast<uintptr_t>(workspace) & 255))
     return fail(I8L_ERR_ALIGN, "i8l_token_linear: x, w_q, y and bias must be 16-byte aligned, the workspace 256-byte");
+  if ((reinterpret_cast<uintptr_t>(w_scale) | reinterpret_cast<uintptr_t>(offsets) | reinterpret_cast<uintptr_t>(status)) & 3)
+    return fail(I8L_ERR_ALIGN, "i8l_token_linear: w_scale, offsets and status are aligned to their elements");
   const int64_t need = i8l_token_linear_workspace(rows, experts, N, K);
   if (need && (!workspace || workspace_bytes < need))
     return fail(I8L_ERR_ARG, "i8l_token_linear: workspace of %lld bytes is too small", (long long)workspace_bytes);
