@@ -334,7 +334,8 @@ I8L_API int i8l_test_set_wait_limit(uint32_t max_polls, int withhold_one_load);
  *   src     int32 [rows]: the choice of a row, -1 if it has none
  * rows >= tokens * k + min(experts, tokens * k) * (align - 1), rounded up to `align`.  The result depends on the inputs only (a
  * stable counting sort, no atomics on places).  experts <= 1024, k <= 64, tokens * k <= 2^30, align <= 65536, cols from 1 to 2^28.
- * Pointers are aligned to their elements.  workspace: i8l_sort_workspace bytes, 4-byte aligned, may be NULL where that is 0.
+ * Pointers are aligned to their elements.  workspace: i8l_sort_workspace bytes (0 for sizes that are refused), 4-byte aligned, may be NULL
+ * where that is 0.
  * No counterpart in the reference, which has no expert layers.
  */
 I8L_API int64_t i8l_sort_workspace(int64_t tokens, int k, int experts);

@@ -417,7 +417,7 @@ PyObject* py_sort_tokens(PyObject*, PyObject* const* args, Py_ssize_t n) {
   constexpr int64_t MOST = 1ll << 30;   // sizes whose products fit 64 bits; the library refuses what is too large for it
   if (!plain_thread() || !dense(x) || dtype_of(x) < 0 || x.dim() != 2 || !dense(ids) || ids.dim() != 2 || ids.device() != x.device() ||
       (ids.scalar_type() != at::kInt && ids.scalar_type() != at::kLong) || ids.size(0) != x.size(0) || x.size(0) > MOST || ids.size(1) > MOST ||
-      experts < 1 || experts > 65536 || align < 1 || align > 65536 || forward_mode(x))
+      experts < 1 || experts > 1024 || align < 1 || align > 65536 || forward_mode(x))
     Py_RETURN_NONE;
   Sorted s;
   {

@@ -838,7 +838,8 @@ int run_combine(CombineArgs a, int64_t cols, int dtype, int wdtype, bool backwar
 using namespace i8l;
 
 extern "C" int64_t i8l_sort_workspace(int64_t tokens, int k, int experts) {
-  if (tokens < 0 || k < 1 || experts < 1 || tokens * k <= SMALL_SORT) return 0;
+  if (tokens < 0 || k < 1 || k > MAX_CHOICES || tokens > (1ll << 30) / k || experts < 1 || experts > MAX_EXPERTS) return 0;   // refused
+  if (tokens * k <= SMALL_SORT) return 0;
   const int64_t chunk = sort_chunk(tokens * k, experts);
   return (tokens * k + chunk - 1) / chunk * experts * (int64_t)sizeof(int32_t);
 }

@@ -445,6 +445,8 @@ def sort_tokens(x: torch.Tensor, ids: torch.Tensor, experts: int, align: int = 1
         raise ValueError(f"ids must be [{T}, k], got {tuple(ids.shape)}")
     if experts < 1 or align < 1:
         raise ValueError(f"experts and align must be positive, got {experts} and {align}")
+    if experts > 1024 or align > 65536:   # before results of that size are made, and before they are cut to a C int
+        raise L.I8LError(-1, f"sort_tokens: experts={experts} and align={align}, at most 1024 and 65536 are possible")
     ids = ids.contiguous()
     k, dev = ids.shape[1], x.device
     R = sorted_rows(T, k, experts, align)
