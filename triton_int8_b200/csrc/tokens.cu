@@ -844,7 +844,8 @@ template <typename Kernel, typename... Args>
 int launch_few(Kernel kernel, std::atomic<int>* allowed, const TokenArgs& a, int64_t channels, int warps, cudaStream_t st, Args... args) {
   I8L_CUDA_OK(allow_smem(kernel, allowed, FEW_SMEM));
   const int64_t segments = a.experts < a.rows ? a.experts : a.rows, units = segments * ((a.N + channels - 1) / channels);
-  const int64_t blocks = (units + warps - 1) / warps, resident = 2 * sm_count();
+  const int64_t blocks = (units + warps - 1) / warps, budget = gemm_cta_budget();
+  const int64_t resident = budget < sm_count() ? budget : 2 * sm_count();   // under a limit no more CTAs than it says
   const LaunchChain chain(st);
   (void)chain_first();   // it always waits
   I8L_CUDA_OK(launch(kernel, dim3((unsigned)(blocks < resident ? blocks : resident)), FEW_THREADS, (size_t)(a.rows * few_row_bytes(a.rows, a.K)), st,
