@@ -253,6 +253,9 @@ class Int8Linear(nn.Module):
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, {self.config}"
 
 
+_FROZEN_TYPES = {"weight_q": torch.int8, "weight_scale": torch.float32, "bias": torch.bfloat16}
+
+
 class Int8FrozenLinear(nn.Module):
     """A linear layer for serving: int8 weights with one scale an output channel, kept; activations quantized per row (linear_w8a8).  Any
     number of tokens, in_features a multiple of 16, out_features of 8.  Buffers weight_q, weight_scale and bias; no gradient."""
@@ -264,11 +267,13 @@ class Int8FrozenLinear(nn.Module):
         self.register_buffer("weight_scale", weight_scale)
         self.register_buffer("bias", bias)
 
-    def _apply(self, fn, *args, **kwargs):   # to(bfloat16) and the like leave the scales in 32 bits
-        scale = self.weight_scale
+    def _apply(self, fn, *args, **kwargs):   # to(float16) and the like leave the scales in 32 bits and the bias in bf16, as the product reads them
+        kept = {name: t for name, t in self._buffers.items() if t is not None and t.dtype == _FROZEN_TYPES.get(name)}
         super()._apply(fn, *args, **kwargs)
-        if self.weight_scale.dtype != scale.dtype:
-            self.weight_scale = scale.to(self.weight_scale.device)
+        for name, t in kept.items():
+            now = self._buffers[name]
+            if now.dtype != t.dtype:
+                self._buffers[name] = t.to(now.device)
         return self
 
     @classmethod
