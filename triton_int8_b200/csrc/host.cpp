@@ -41,6 +41,7 @@ decltype(&i8l_combine) lib_combine = nullptr;
 decltype(&i8l_combine_backward) lib_combine_backward = nullptr;
 decltype(&i8l_token_linear_workspace) lib_token_workspace = nullptr;
 decltype(&i8l_token_linear) lib_token_linear = nullptr;
+PyObject* py_combine_backward = nullptr;   // (rows or None, weights, pos, src, dy, wants drows, wants dweights) -> (drows, dweights)
 PyObject* on_error = nullptr;       // (entry point, code, device index): raises
 PyObject* on_timeout = nullptr;     // (device index): raises, or returns where there is nothing to report now
 PyObject* open_status = nullptr;    // (device index) -> (status word, poller), as integers
@@ -323,6 +324,9 @@ Tensor combine(const Tensor& rows, const Tensor& weights, const Tensor& pos) {
         dev);
   return y;
 }
+bool ints(const Tensor& t, const Tensor& like, at::IntArrayRef shape) {
+  return t.scalar_type() == at::kInt && dense(t) && t.device() == like.device() && t.sizes() == shape;
+}
 bool forward_mode(const Tensor& t) { return t._fw_grad(0).defined(); }
 // A gradient that came in, as the kernels read it.
 Tensor incoming(const char* name, const Tensor& d) {
@@ -338,6 +342,28 @@ Tensor once(const char* name, const Tensor& result, const Tensor& dy) {
   return (*error)({result.detach().requires_grad_(true)})[0];
 }
 
+// The Python path of both backward passes, for what the native one does not take; it makes contiguous what is not and refuses what does not
+// fit.  rows undefined: sort_tokens'.
+variable_list combine_backward_in_python(const Tensor& rows, const Tensor& weights, const Tensor& pos, const Tensor& src, const Tensor& dy,
+                                         bool need_rows, bool need_weights) {
+  const WithGil gil;
+  auto wrap = [](const Tensor& t) {
+    if (!t.defined()) Py_RETURN_NONE;
+    return THPVariable_Wrap(t.detach());
+  };
+  PyObject* r = PyObject_CallFunction(py_combine_backward, "NNNNNii", wrap(rows), wrap(weights), wrap(pos), wrap(src), wrap(dy), (int)need_rows,
+                                      (int)need_weights);
+  if (!r) throw_python_error();
+  PyObject *a = nullptr, *b = nullptr;
+  const int ok = PyArg_ParseTuple(r, "OO", &a, &b);
+  variable_list grads(2);
+  if (ok && THPVariable_Check(a)) grads[0] = THPVariable_Unpack(a);
+  if (ok && THPVariable_Check(b)) grads[1] = THPVariable_Unpack(b);
+  Py_DECREF(r);
+  if (!ok) throw_python_error();
+  return grads;
+}
+
 struct SortNode : torch::autograd::Function<SortNode> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& ids, int64_t experts, int64_t align) {
     const Sorted s = sort_tokens(x, ids, (int)experts, align);
@@ -349,7 +375,9 @@ struct SortNode : torch::autograd::Function<SortNode> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
     const Tensor pos = ctx->get_saved_variables()[0], dy = incoming("sort_tokens", grads[0]);
-    return {once("sort_tokens", combine(dy.detach(), Tensor(), pos), grads[0]), Tensor(), Tensor(), Tensor()};   // the sum of a token's rows
+    const bool ok = pos.dim() == 2 && ints(pos, dy, pos.sizes());   // hooks on saved tensors give back what they like
+    const Tensor dx = ok ? combine(dy.detach(), Tensor(), pos) : combine_backward_in_python(Tensor(), Tensor(), pos, Tensor(), dy, true, false)[0];
+    return {once("sort_tokens", dx, grads[0]), Tensor(), Tensor(), Tensor()};   // the sum of a token's rows
   }
 };
 
@@ -361,17 +389,27 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &rows = saved[0], &weights = saved[1], &pos = saved[2], &src = saved[3], dy = incoming("combine", grads[0]);
-    const int64_t T = pos.size(0), k = pos.size(1), R = rows.size(0), H = rows.size(1);
-    const int dev = rows.get_device();
-    const c10::cuda::CUDAGuard guard(dev);
+    const bool need_rows = ctx->needs_input_grad(0), need_weights = ctx->needs_input_grad(1);
     Tensor drows, dweights;
-    if (ctx->needs_input_grad(0)) drows = at::empty({R, H}, rows.options());
-    if (ctx->needs_input_grad(1)) dweights = at::empty({T, k}, weights.options());
-    check("i8l_combine_backward",
-          lib_combine_backward(rows.data_ptr(), weights.data_ptr(), at_of<int32_t>(pos), at_of<int32_t>(src), dy.data_ptr(), R, T, H, (int)k,
-                               dtype_of(rows), dtype_of(weights), drows.defined() ? drows.data_ptr() : nullptr,
-                               dweights.defined() ? dweights.data_ptr() : nullptr, stream_of(dev)),
-          dev);
+    if (dense(rows) && rows.dim() == 2 && rows.scalar_type() == dy.scalar_type() && rows.device() == dy.device() && rows.size(1) == dy.size(1) &&
+        dense(weights) && weights.dim() == 2 && weights.size(0) == dy.size(0) && weights.device() == dy.device() &&
+        (weights.scalar_type() == at::kFloat || weights.scalar_type() == dy.scalar_type()) && ints(pos, dy, weights.sizes()) &&
+        ints(src, dy, {rows.size(0)})) {
+      const int64_t T = pos.size(0), k = pos.size(1), R = rows.size(0), H = rows.size(1);
+      const int dev = rows.get_device();
+      const c10::cuda::CUDAGuard guard(dev);
+      if (need_rows) drows = at::empty({R, H}, rows.options());
+      if (need_weights) dweights = at::empty({T, k}, weights.options());
+      check("i8l_combine_backward",
+            lib_combine_backward(rows.data_ptr(), weights.data_ptr(), at_of<int32_t>(pos), at_of<int32_t>(src), dy.data_ptr(), R, T, H, (int)k,
+                                 dtype_of(rows), dtype_of(weights), drows.defined() ? drows.data_ptr() : nullptr,
+                                 dweights.defined() ? dweights.data_ptr() : nullptr, stream_of(dev)),
+            dev);
+    } else {   // hooks on saved tensors give back what they like
+      const variable_list r = combine_backward_in_python(rows, weights, pos, src, dy, need_rows, need_weights);
+      drows = r[0];
+      dweights = r[1];
+    }
     // a graph of the gradients would lead to dy, the rows and the weights alike
     const Tensor& any = rows.requires_grad() ? rows : weights.requires_grad() ? weights : grads[0];
     return {once("combine", drows, any), once("combine", dweights, any), Tensor(), Tensor()};
@@ -398,9 +436,6 @@ Tensor token_linear(const Tensor& x, const Tensor& wq, const Tensor& ws, const T
 
 // ------------------------------------------------------------------------------------------------ Python
 bool exact_tensor(PyObject* o) { return THPVariable_CheckExact(o); }
-bool ints(const Tensor& t, const Tensor& like, at::IntArrayRef shape) {
-  return t.scalar_type() == at::kInt && dense(t) && t.device() == like.device() && t.sizes() == shape;
-}
 bool at_16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 
 // sort_tokens(x, ids, experts, align) -> (rows, offsets, pos, src), or None
@@ -581,10 +616,14 @@ PyObject* py_setup(PyObject*, PyObject* args) {
 }
 
 // setup_experts(addresses of i8l_sort_workspace, i8l_sort_tokens, i8l_combine, i8l_combine_backward, i8l_token_linear_workspace,
-// i8l_token_linear)
+// i8l_token_linear, combine_backward_in_python)
 PyObject* py_setup_experts(PyObject*, PyObject* args) {
   unsigned long long a[6];
-  if (!PyArg_ParseTuple(args, "KKKKKK", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5])) return nullptr;
+  PyObject* backward = nullptr;
+  if (!PyArg_ParseTuple(args, "KKKKKKO", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &backward)) return nullptr;
+  Py_INCREF(backward);
+  Py_XDECREF(py_combine_backward);
+  py_combine_backward = backward;
   lib_sort_workspace = reinterpret_cast<decltype(lib_sort_workspace)>(a[0]);
   lib_sort_tokens = reinterpret_cast<decltype(lib_sort_tokens)>(a[1]);
   lib_combine = reinterpret_cast<decltype(lib_combine)>(a[2]);

@@ -138,6 +138,12 @@ def _backward_in_python(dy, w, xqt, xst, gran, qmode, hadamard, flags, whole_k, 
                            *post, 0 if whole_k else flags, bool(need_dx), bool(need_dw))
 
 
+def _combine_backward_in_python(rows, weights, pos, src, dy, need_rows, need_weights):
+    if rows is None:   # sort_tokens': a token's gradient is the sum of its rows'
+        return combine(dy, None, pos), None
+    return combine_backward(rows, weights, pos, src, dy, bool(need_rows), bool(need_weights))
+
+
 def host():
     """The native module, bound to the loaded library."""
     global _host
@@ -154,7 +160,8 @@ def host():
         mod.setup(L.address("i8l_quant_gemm"), L.address("i8l_linear_backward_bias"), L.address("i8l_status_peek"), _on_error,
                   _on_timeout, _open_status, _backward_in_python)
         mod.setup_experts(*(L.address(n) for n in ("i8l_sort_workspace", "i8l_sort_tokens", "i8l_combine", "i8l_combine_backward",
-                                                   "i8l_token_linear_workspace", "i8l_token_linear")))
+                                                   "i8l_token_linear_workspace", "i8l_token_linear")),
+                          _combine_backward_in_python)
         _host = mod
     return _host
 
