@@ -328,12 +328,10 @@ bool ints(const Tensor& t, const Tensor& like, at::IntArrayRef shape) {
   return t.scalar_type() == at::kInt && dense(t) && t.device() == like.device() && t.sizes() == shape;
 }
 bool forward_mode(const Tensor& t) { return t._fw_grad(0).defined(); }
-// A gradient that came in, as the kernels read it.
+// A gradient that came in, contiguous.
 Tensor incoming(const char* name, const Tensor& d) {
   TORCH_CHECK_NOT_IMPLEMENTED(!forward_mode(d), "the gradient of ", name, " has no forward-mode derivative");
-  const Tensor dy = d.contiguous();
-  TORCH_CHECK(plain_thread() && dense(dy), name, ": its gradient cannot be taken under a transform or of a tensor subclass");
-  return dy;
+  return d.contiguous();
 }
 // The gradients have no gradient of their own: where a graph of them is made, going back through it is an error.
 Tensor once(const char* name, const Tensor& result, const Tensor& dy) {
@@ -375,7 +373,7 @@ struct SortNode : torch::autograd::Function<SortNode> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
     const Tensor pos = ctx->get_saved_variables()[0], dy = incoming("sort_tokens", grads[0]);
-    const bool ok = pos.dim() == 2 && ints(pos, dy, pos.sizes());   // hooks on saved tensors give back what they like
+    const bool ok = plain_thread() && dense(dy) && pos.dim() == 2 && ints(pos, dy, pos.sizes());
     const Tensor dx = ok ? combine(dy.detach(), Tensor(), pos) : combine_backward_in_python(Tensor(), Tensor(), pos, Tensor(), dy, true, false)[0];
     return {once("sort_tokens", dx, grads[0]), Tensor(), Tensor(), Tensor()};   // the sum of a token's rows
   }
@@ -391,8 +389,8 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
     const Tensor &rows = saved[0], &weights = saved[1], &pos = saved[2], &src = saved[3], dy = incoming("combine", grads[0]);
     const bool need_rows = ctx->needs_input_grad(0), need_weights = ctx->needs_input_grad(1);
     Tensor drows, dweights;
-    if (dense(rows) && rows.dim() == 2 && rows.scalar_type() == dy.scalar_type() && rows.device() == dy.device() && rows.size(1) == dy.size(1) &&
-        dense(weights) && weights.dim() == 2 && weights.size(0) == dy.size(0) && weights.device() == dy.device() &&
+    if (plain_thread() && dense(dy) && dense(rows) && rows.dim() == 2 && rows.scalar_type() == dy.scalar_type() &&
+        rows.device() == dy.device() && rows.size(1) == dy.size(1) && dense(weights) && weights.dim() == 2 && weights.size(0) == dy.size(0) && weights.device() == dy.device() &&
         (weights.scalar_type() == at::kFloat || weights.scalar_type() == dy.scalar_type()) && ints(pos, dy, weights.sizes()) &&
         ints(src, dy, {rows.size(0)})) {
       const int64_t T = pos.size(0), k = pos.size(1), R = rows.size(0), H = rows.size(1);
@@ -405,7 +403,7 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
                                  dtype_of(rows), dtype_of(weights), drows.defined() ? drows.data_ptr() : nullptr,
                                  dweights.defined() ? dweights.data_ptr() : nullptr, stream_of(dev)),
             dev);
-    } else {   // hooks on saved tensors give back what they like
+    } else {   // a mode that the forward pass did not see, or hooks on saved tensors, which give back what they like
       const variable_list r = combine_backward_in_python(rows, weights, pos, src, dy, need_rows, need_weights);
       drows = r[0];
       dweights = r[1];
