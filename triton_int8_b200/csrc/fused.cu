@@ -9,11 +9,11 @@
 //   warp 1       tcgen05.mma kind::i8 issuer (M = 128, N = 128, K = 32, four per stage), accumulators alternate
 //                between two 128-column tensor-memory buffers per K step, tcgen05.commit frees the stage.
 //   warps 4-19   sixteen worker warps that each do both remaining jobs, one K step apart.  Transform: read a
-//                share of the staged tiles (16-byte vectors, 16 lanes per row) into registers and give the
-//                staging slot back at once; absmax per A tile and per B row (forward) or per B tile
-//                (backward), scale = 127 / (amax + 1e-5), q = floor(x * scale + 0.5), int8 written into the
-//                K-major 128B-swizzled shared-memory stage the tensor core reads, fence.proxy.async and an
-//                arrival on the stage's "full" barrier; the step's factors go to a small ring in shared
+//                share of the staged tiles (16-byte vectors, 16 lanes per row) into registers; absmax per A tile
+//                and per B row (forward) or per B tile (backward), behind which the staging slot is given back;
+//                scale = 127 / (amax + 1e-5), q = floor(x * scale + 0.5), int8 written into the K-major
+//                128B-swizzled shared-memory stage the tensor core reads, fence.proxy.async and an arrival on
+//                the stage's "full" barrier; the step's factors go to a small ring in shared
 //                memory.  Drain: the int32 partial product of the PREVIOUS step (its MMAs ran meanwhile) leaves
 //                tensor memory, acc += P / (s_a * s_b[n]) (a multiplication by the rounded reciprocal unless
 //                the reference operation order is asked for); after the last step the final cast and store.
@@ -87,7 +87,7 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     }
     for (int s = 0; s < NB; ++s) {
       mbar_init(smem_u32(&ctl.bfull[s]), 1);
-      mbar_init(smem_u32(&ctl.bempty[s]), WORKERS);
+      mbar_init(smem_u32(&ctl.bempty[s]), 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(smem_u32(&ctl.tfull[b]), 1);
@@ -205,7 +205,6 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             ra[i] = *reinterpret_cast<const uint4*>(smem_raw + (smem_bfa - smem_u32(smem_raw)) + sb * BF_A + r * 256 + 16 * cc);
             rb[i] = *reinterpret_cast<const uint4*>(smem_raw + (smem_bfb - smem_u32(smem_raw)) + sb * BF_B + r * 256 + 16 * cc);
           }
-          mbar_arrive(smem_u32(&ctl.bempty[sb]));   // the tiles are in registers: the slot can be refilled
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const __nv_bfloat162* ha = reinterpret_cast<const __nv_bfloat162*>(&ra[i]);
@@ -234,6 +233,10 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
           }
         }
         named_sync(BAR_XF, WORKERS);
+        // The maxima that every warp has left here come from all that it has read, so the slot can be refilled.  With an arrival of every
+        // thread right behind its loads, nothing but their issue order kept them in front of the refill: of 10000 calls behind a kernel that
+        // had emptied the instruction cache 10 had pieces of a row of A from two steps on.
+        if (ok && xtid == 0) mbar_arrive(smem_u32(&ctl.bempty[sb]));
         if (ok) {
           float am = ctl.red_a[step & 1][0], bm = ctl.red_b[step & 1][0];
 #pragma unroll
