@@ -43,8 +43,8 @@ def _launches(call):
 @pytest.mark.parametrize("experts", [1, 6])
 def test_few_rows(rows, experts):
     g = torch.Generator(device=DEV).manual_seed(rows)
-    wq = torch.randint(-127, 128, (experts, 1544, 512), generator=g, device=DEV, dtype=torch.int8)
-    ws, x = torch.rand(experts, 1544, generator=g, device=DEV), torch.randn(rows, 512, generator=g, device=DEV).to(torch.bfloat16)
+    wq = torch.randint(-127, 128, (experts, 296, 512), generator=g, device=DEV, dtype=torch.int8)
+    ws, x = torch.rand(experts, 296, generator=g, device=DEV), torch.randn(rows, 512, generator=g, device=DEV).to(torch.bfloat16)
     offsets = torch.linspace(0, rows, experts + 1, device=DEV).int()
     call = lambda: moe.expert_linear(x, wq, ws, offsets)  # noqa: E731
     want, free = call(), _launches(call)

@@ -831,18 +831,27 @@ group_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
 }
 
 // ------------------------------------------------------------------------------------------ host
-// Whether the kernels for few rows take them: in the shared memory of which two blocks fit on an SM.
-constexpr int FEW_SMEM = 96 * 1024;
 int64_t few_row_bytes(int64_t rows, int64_t K) { return rows <= 4 ? K : (K + MMA_K - 1) / MMA_K * MMA_K; }
-// Above four rows only as long as the weights are few, 2^24 bytes if all rows belong to different experts: 8 rows x 4096x4096 8.9 us here and
-// 11.0 on the tensor cores, but 11008x4096 14.0 and 13.0, 8 of 8 experts of 1408x4096 17.8 and 14.2.
+// Whether the kernels for few rows take them.  Weights from memory, us here and on the tensor cores:
+//   Every block quantizes all rows into its shared memory, 256 threads for as many as the next power of two: that many times K is at most
+//   2^15.  One row x 4096x24576 21.0 and 26.3, x 1024x49152 26.4 and 22.6; two x 2048x16384 13.7 and 14.5, x 1024x40960 28.3 and 20.1;
+//   four x 2048x8192 9.6 and 11.3, x 2048x11008 12.9 and 12.3; eight x 2048x4096 8.1 and 9.3, x 2048x6144 10.9 and 10.2, x 1024x11008 22.8
+//   and 10.1.
+//   Weights, of as many experts as the rows allow: 3 or 4 rows up to 40 MB, 4 x 8192x4096 11.8 and 12.9, x 11008x4096 14.1 and 13.4, 4 experts of
+//   2048x4096 11.6 and 13.7, of 4096x4096 18.0 and 16.4, 3 of 5040x5984 24.7 and 20.0, but any number where K is short, 4 of 8192x2048
+//   14.9 and 17.0; 5 to 8 rows up to 24 MB, 8 x 5120x4096 11.7 and 11.7, x 6144x4096 12.6 and 12.3, x 8192x4096 14.7 and 13.6.
+//   5 to 8 rows of several experts, E if they are as many as the rows allow: an expert's channels are gone through once more by all blocks and
+//   its rows fill less of the instructions, E * E * N up to 12 K.  8 rows, 2 experts of 2048x2048 8.5 and 9.1, of 4096x2048 10.6
+//   and 9.7; 8 of 256x1024 6.6 and 7.3, of 512x1024 8.6 and 7.5; 5 rows, 5 experts of 512x1024 6.5 and 7.4, of 2048x1024 9.0 and 8.1.
+// Over 90 sizes the choice costs 1 % against the better one, 10 % at most.
 bool few_rows(int64_t rows, int64_t K, int64_t experts, int64_t N) {
-  if (rows > FEW_ROWS || rows * few_row_bytes(rows, K) > FEW_SMEM) return false;
-  return rows <= 4 || (experts < rows ? experts : rows) * N * K <= 1 << 24;
+  const int64_t padded = rows <= 2 ? rows : rows <= 4 ? 4 : 8, segments = experts < rows ? experts : rows;
+  if (rows > FEW_ROWS || padded * K > 1 << 15) return false;
+  if (rows <= 4) return rows <= 2 || K <= 2048 || segments * N * K <= 40 << 20;
+  return segments == 1 ? N * K <= 24 << 20 : segments * segments * N <= 12 << 10;
 }
 template <typename Kernel, typename... Args>
-int launch_few(Kernel kernel, std::atomic<int>* allowed, const TokenArgs& a, int64_t channels, int warps, cudaStream_t st, Args... args) {
-  I8L_CUDA_OK(allow_smem(kernel, allowed, FEW_SMEM));
+int launch_few(Kernel kernel, const TokenArgs& a, int64_t channels, int warps, cudaStream_t st, Args... args) {
   const int64_t segments = a.experts < a.rows ? a.experts : a.rows, units = segments * ((a.N + channels - 1) / channels);
   const int64_t blocks = (units + warps - 1) / warps, budget = gemm_cta_budget();
   const int64_t resident = budget < sm_count() ? budget : 2 * sm_count();   // under a limit no more CTAs than it says
@@ -853,11 +862,10 @@ int launch_few(Kernel kernel, std::atomic<int>* allowed, const TokenArgs& a, int
   return I8L_OK;
 }
 int run_few(const TokenArgs& a, cudaStream_t st) {
-  static std::atomic<int> allowed[4][MAX_SMEM_DEVICES];
-  if (a.rows == 1) return launch_few(few_dp_kernel<1>, allowed[0], a, DP_CHANNELS, FEW_WARPS, st);
-  if (a.rows == 2) return launch_few(few_dp_kernel<2>, allowed[1], a, DP_CHANNELS, FEW_WARPS, st);
-  if (a.rows <= 4) return launch_few(few_dp_kernel<4>, allowed[2], a, DP_CHANNELS, FEW_WARPS, st);
-  return launch_few(few_mma_kernel, allowed[3], a, MMA_CHANNELS, 1, st, (int)few_row_bytes(a.rows, a.K));
+  if (a.rows == 1) return launch_few(few_dp_kernel<1>, a, DP_CHANNELS, FEW_WARPS, st);
+  if (a.rows == 2) return launch_few(few_dp_kernel<2>, a, DP_CHANNELS, FEW_WARPS, st);
+  if (a.rows <= 4) return launch_few(few_dp_kernel<4>, a, DP_CHANNELS, FEW_WARPS, st);
+  return launch_few(few_mma_kernel, a, MMA_CHANNELS, 1, st, (int)few_row_bytes(a.rows, a.K));
 }
 
 // Most tokens of a tile, from what the host knows: as if all rows belonged to experts, and to all alike.  A tile of s columns takes 0.4 + 0.6 *
