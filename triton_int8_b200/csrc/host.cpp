@@ -121,6 +121,7 @@ bool dense(const Tensor& t) {
                                           c10::DispatchKey::FuncTorchBatchedDecomposition, c10::DispatchKey::BatchedNestedTensor,
                                           c10::DispatchKey::Batched}));
 }
+bool forward_mode(const Tensor& t) { return t._fw_grad(0).defined(); }
 bool plain(const Tensor& t) { return t.scalar_type() == at::kBFloat16 && dense(t); }
 // No mode, transform or tracer looks at what this thread does.
 bool plain_thread() {
@@ -222,13 +223,13 @@ void linear_backward(const Tensor& dy, const Tensor& weight, const Tensor& q, co
                      bool need_dw, bool need_db, Tensor& dx, Tensor& dw, Tensor& db) {
   const int64_t M = dy.size(0), N = dy.size(1), K = weight.size(1);
   const int gran = c.whole_k ? I8L_GRAN_ROW : c.gran;
-  bool ok = plain_thread() && plain(dy) && plain(weight) && weight.size(0) == N && weight.device() == dy.device();
+  bool ok = plain_thread() && plain(dy) && !forward_mode(dy) && plain(weight) && weight.size(0) == N && weight.device() == dy.device();
   if (ok && need_dw) {
     ok = q.defined() && s.defined() && q.device() == dy.device() && s.device() == dy.device() && q.scalar_type() == at::kChar &&
          s.scalar_type() == at::kFloat && q.is_contiguous() && s.is_contiguous() && q.sizes() == at::IntArrayRef({1, K, M}) &&
          s.numel() == scale_count(gran, 1, K, M);
   }
-  // torch's sum where its graph is wanted (create_graph), and where the kernel's 16-byte loads do not fit
+  // torch's sum where its graph (create_graph) or tangent is wanted, and where the kernel's 16-byte loads do not fit
   const bool own_sum = need_db && ok && !at::GradMode::is_enabled() && reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16 == 0;
   if (need_db && !own_sum) db = dy.sum(0);
   if (!ok) {
@@ -327,7 +328,6 @@ Tensor combine(const Tensor& rows, const Tensor& weights, const Tensor& pos) {
 bool ints(const Tensor& t, const Tensor& like, at::IntArrayRef shape) {
   return t.scalar_type() == at::kInt && dense(t) && t.device() == like.device() && t.sizes() == shape;
 }
-bool forward_mode(const Tensor& t) { return t._fw_grad(0).defined(); }
 // A gradient that came in, contiguous.
 Tensor incoming(const char* name, const Tensor& d) {
   TORCH_CHECK_NOT_IMPLEMENTED(!forward_mode(d), "the gradient of ", name, " has no forward-mode derivative");

@@ -133,6 +133,7 @@ def _open_status(index: int):
 
 
 def _backward_in_python(dy, w, xqt, xst, gran, qmode, hadamard, flags, whole_k, need_dx, need_dw):
+    refuse_tangent("the gradient of Int8Linear", dy)
     post = [1.0 / hadamard if hadamard else 1.0] * 2
     return linear_backward(dy, w, (xqt, xst), L.GRAN_ROW if whole_k else gran, L.QMODE_ROWRCP if whole_k else qmode, hadamard,
                            *post, 0 if whole_k else flags, bool(need_dx), bool(need_dw))
@@ -547,10 +548,14 @@ def refuse_gradient(name: str, *tensors) -> None:
     refuse_proxies(name)
 
 
+def has_tangent(t: torch.Tensor) -> bool:
+    ad = torch.autograd.forward_ad
+    return ad._current_level >= 0 and ad.unpack_dual(t).tangent is not None
+
+
 def refuse_tangent(name: str, *tensors) -> None:
     """A launch sees plain memory only: the derivative of a dual tensor would be lost without a word."""
-    ad = torch.autograd.forward_ad
-    if ad._current_level >= 0 and any(t is not None and ad.unpack_dual(t).tangent is not None for t in tensors):
+    if any(t is not None and has_tangent(t) for t in tensors):
         raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 

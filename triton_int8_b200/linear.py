@@ -209,11 +209,14 @@ class Int8LinearFn(torch.autograd.Function):
         weight, *saved = ctx.saved_tensors
         dy2 = dy.reshape(-1, dy.shape[-1]).contiguous()
         need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        if need_dx or need_dw:
+            K.refuse_tangent("the gradient of Int8Linear", dy)
         dx, dw = linear_backward(dy2, weight, tuple(saved) if saved else None, ctx.cfg, need_dx, need_dw)
         db = None
         if ctx.has_bias and ctx.needs_input_grad[2]:
-            # torch's sum where its graph is wanted, under a transform, and where the kernel's 16-byte loads do not fit
-            own = not torch.is_grad_enabled() and torch._C._has_storage(dy2) and dy2.data_ptr() % 16 == 0
+            # torch's sum where its graph or tangent is wanted, under a transform, and where the kernel's 16-byte loads do not fit
+            own = (not torch.is_grad_enabled() and not K.has_tangent(dy) and torch._C._has_storage(dy2)
+                   and dy2.data_ptr() % 16 == 0)
             db = K.col_sum(dy2) if own else dy2.sum(0).to(dy.dtype)
         return (dx.view(ctx.x_shape) if dx is not None else None), dw, db, None, None
 
