@@ -363,7 +363,7 @@ I8L_API int i8l_combine_backward(const void* rows, const void* weights, const in
  * A product whose weights stay int8, for any number of rows, by expert: rows [offsets[e], offsets[e + 1]) of x bf16 [rows, K]
  * are quantized with one scale a row (I8L_QMODE_ROWRCP, I8L_HAD_NONE), multiplied exactly with w_q[e] (int8 [experts, N, K]) and
  *   y = (float(acc) * x_scale[row]) * w_scale[e, n] + bias[e, n]
- * is rounded once to bf16 (fp32 with I8L_GEMM_OUT_F32).  w_scale fp32 [experts, N]; bias bf16 [experts, N] or NULL.
+ * is rounded once to bf16 (fp32 with I8L_GEMM_OUT_F32).  An infinity makes its row NaN, a NaN counts as zero.  w_scale fp32 [experts, N]; bias bf16 [experts, N] or NULL.
  *   offsets int32 [experts + 1] on the device, non-decreasing, or NULL: one matrix (experts = 1) for all rows.  Rows in front
  *   of offsets[0] and from offsets[experts] on come out zero.  Offsets outside [0, rows] are cut off; if they decrease y is
  *   undefined, but nothing outside of it is touched.

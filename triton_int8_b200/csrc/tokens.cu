@@ -144,8 +144,9 @@ __device__ __forceinline__ void fetch_l2(const TokenArgs& a, const FewShared& sh
 }
 
 // Up to four rows: a warp takes two channels at a time over all of K, 512 bytes of each a load, and multiplies by dp4a; a batch is 2 KB of
-// each.  11008x4096: one row 9.3 us, two 9.8, four 12.2 (without the fetch into L2 11.5, 12.1, 13.8); 4096x4096 4.4, 5.0, 6.7;
-// one token x 2 of 8 experts of 11008x4096 17.9 (14 of bytes).
+// each.  Weights from memory, 11008x4096: one row 11.7 us, two 12.1, four x 10240x4096 14.1; 4096x4096 6.3, 6.6, 7.8; one token x 2 of 8
+// experts of 11008x4096 19.2 (14 of bytes).  Weights in L2 8.1, 8.7 and 11.2, 4.6, 5.0 and 6.6.  The fetch into L2 ahead took one, two and four rows x
+// 11008x4096 from 11.5, 12.1 and 13.8 to 9.3, 9.8 and 12.2 where part of the weights were there.
 constexpr int DP_CHANNELS = 2, DP_STEPS = 4, DP_BATCH = DP_STEPS * 512;
 struct DpBatch {
   uint4 w[DP_CHANNELS][DP_STEPS];
@@ -253,8 +254,9 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_dp_kernel(const TokenArgs 
 
 // Five to eight rows, which dp4a is too slow for: a block takes 16 channels at a time, its warps split K into pieces of 128 and multiply by
 // mma.sync m16n8k32, channels times rows.  The order of K inside a product does not matter, so a lane's 16 contiguous bytes serve
-// as its fragments as they are, for weights and rows alike.  8 rows x 11008x4096 13.8 us, 4096x4096 8.8, 1024x1024 3.8 (dp4a 17.9, 9.8,
-// 3.9; one row 10.8, 5.7, 3.3 against 9.3, 4.4, 2.8: lines of four rows a load and the sum over the warps cost more there).
+// as its fragments as they are, for weights and rows alike.  8 rows, weights from memory, x 4096x4096 10.2 us, 6144x4096 12.4, 1024x1024 3.6; in
+// L2 8.6 and 10.2.  There dp4a took 9.8 for 4096x4096; one row 5.7 against 4.4 (lines of four rows a load and the sum over the warps cost
+// more).
 constexpr int MMA_CHANNELS = 16, MMA_K = 128, MMA_PIECES = 2;
 struct MmaBatch {
   uint4 w[MMA_PIECES][2][2];   // piece of K, channel g or g + 8, half of the piece

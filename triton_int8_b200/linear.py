@@ -173,8 +173,9 @@ class TokenLinearFn(torch.autograd.Function):
 def linear_w8a8(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, bias=None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The product for serving, with weights that were quantized once: x bf16 [..., K], wq int8 [N, K], ws fp32 [N], bias bf16 [N]
     -> [..., N], bf16 or fp32.  One scale a row of x and one an output channel, as double_channel has them
-    (triton/double-channle_fwd32.py:295-311 without the rotation), any number of rows, N a multiple of 8, K of 16.  There is no
-    gradient: inputs that want one are refused."""
+    (triton/double-channle_fwd32.py:295-311 without the rotation), any number of rows, N a multiple of 8, K of 16.  As there, an
+    infinity makes its row NaN and a NaN counts as zero.  There is no gradient: inputs that want one, or carry a tangent, are refused.
+    torch.jit.trace records the call as a Python function."""
     if out_dtype in (torch.bfloat16, torch.float32) and not torch.compiler.is_compiling():   # plain tensors
         y = K.host().token_linear(x, wq, ws, None, bias, out_dtype == torch.float32)
         if y is not None:
@@ -261,7 +262,8 @@ _FROZEN_TYPES = {"weight_q": torch.int8, "weight_scale": torch.float32, "bias": 
 
 class Int8FrozenLinear(nn.Module):
     """A linear layer for serving: int8 weights with one scale an output channel, kept; activations quantized per row (linear_w8a8).  Any
-    number of tokens, in_features a multiple of 16, out_features of 8.  Buffers weight_q, weight_scale and bias; no gradient."""
+    number of tokens, in_features a multiple of 16 (of 128 where from_linear quantizes), out_features of 8.  Buffers weight_q (int8),
+    weight_scale (fp32) and bias (bf16), which keep their types when the layer is cast; no gradient."""
 
     def __init__(self, weight_q: torch.Tensor, weight_scale: torch.Tensor, bias=None):
         super().__init__()

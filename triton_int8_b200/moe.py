@@ -4,8 +4,9 @@
     ...                                                        # any computation that keeps the rows in their places
     y = combine(rows, weights, pos, src)                       # y[t] = sum over j of weights[t, j] * rows[pos[t, j]]
 
-Both are differentiable and neither waits for the device: shapes depend on the sizes, not on the choices.  expert_linear multiplies the
-rows with their experts' kept int8 weights (serving); Int8MoE puts all of them together.  The reference has no expert layers.
+Both have a gradient (no second one, no forward-mode derivative: both are refused) and neither waits for the device: shapes depend on the sizes,
+not on the choices.  expert_linear multiplies the rows with their experts' kept int8 weights (serving); Int8MoE puts all of them together.
+torch.jit.trace records each of them as a Python function.  The reference has no expert layers.
 """
 from __future__ import annotations
 
@@ -109,8 +110,8 @@ def expert_linear(rows: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, offset
                   out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The experts' products for serving: rows bf16 [R, K] in the order of their experts, wq int8 [E, N, K] and ws fp32 [E, N]
     (quantize_experts), offsets int32 [E + 1] (sort_tokens), bias bf16 [E, N] -> [R, N], bf16 or fp32.  A row is quantized with
-    one scale, the sum over K is exact, y = (sum * row scale) * channel scale + bias is rounded once.  Rows from offsets[E] on
-    come out zero.  N a multiple of 8, K of 16; any number of rows, one included.
+    one scale (an infinity makes its row NaN, a NaN counts as zero), the sum over K is exact, y = (sum * row scale) * channel scale +
+    bias is rounded once.  Rows from offsets[E] on come out zero.  N a multiple of 8, K of 16; any number of rows, one included.
     The weights are integers, there is no gradient: inputs that want one are refused.  Int8Linear trains, on segments of
     sort_tokens(align=128)."""
     if out_dtype in (torch.bfloat16, torch.float32) and offsets is not None and not torch.compiler.is_compiling():
