@@ -425,7 +425,7 @@ def _check_rows(x: torch.Tensor, name: str) -> torch.Tensor:
         raise TypeError(f"{name} must be bfloat16, float16 or float32, got {x.dtype}")
     if x.dim() != 2:
         raise ValueError(f"{name} must have two dimensions, got {tuple(x.shape)}")
-    return x.contiguous()
+    return x.resolve_neg().contiguous()   # the imaginary part of a conjugate is its negative in name only
 
 
 def _check_ints(t: torch.Tensor, name: str, shape: tuple) -> torch.Tensor:
@@ -474,7 +474,7 @@ def _check_weights(weights, rows, shape):
         raise TypeError(f"weights must be float32 or {rows.dtype}, got {weights.dtype}")
     if tuple(weights.shape) != shape:
         raise ValueError(f"weights have shape {tuple(weights.shape)}, expected {shape}")
-    return weights.contiguous()
+    return weights.resolve_neg().contiguous()
 
 
 def combine(rows: torch.Tensor, weights, pos: torch.Tensor) -> torch.Tensor:
