@@ -25,6 +25,9 @@ def _call(name: str, dev: torch.device, *args, tensors=()) -> None:
     for t in tensors:
         if t is not None and t.device != dev:
             raise ValueError(f"{name}: operands on different devices ({t.device} vs {dev})")
+    if torch._C._get_tracing_state() is not None:   # see untraced
+        raise RuntimeError(f"{name}: torch.jit.trace sees no launches; the layers and the product for serving can be traced")
+    refuse_proxies(name)
     index = dev.index
     if index == _current_device():   # the usual case, without the context manager (4 us of host time)
         L.call(name, *args, _raw_stream(index))

@@ -193,6 +193,11 @@ class Int8LinearFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, cfg: Int8Config, grad_enabled: bool = True):
+        with K.untraced():
+            return Int8LinearFn._forward(ctx, x, weight, bias, cfg, grad_enabled)
+
+    @staticmethod
+    def _forward(ctx, x, weight, bias, cfg: Int8Config, grad_enabled: bool):
         x2 = x.reshape(-1, x.shape[-1])
         # Every GEMM reports a device-side wait that gave up into the device's status word; look at it
         # here without blocking (the copy was started by the previous call) and raise if it is set.
